@@ -361,6 +361,88 @@ typedef struct h3a_adaln_params {
 } h3a_adaln_params;
 int32_t h3a_adaln_norm(const h3a_adaln_params* p, void* stream);
 
+/*
+ * Paged K/V cache: rows of 128 values per token and K/V head, kept between calls in fixed-size pages, and the attention
+ * of new rows over it.  The reference keeps nothing between evaluations (src/pika_h3/core/sampling.py:87-109,160-169 runs
+ * the whole sequence through the model six times); this is for callers whose K and V of some tokens stay the same: text or
+ * condition tokens over the sampler's evaluations, a clip that grows by a few frames at a time, a prompt model.
+ *
+ * Pools are addressed x[page * stride_page + at * stride_token + head * stride_head + c], c in [0,128) contiguous, strides
+ * in ELEMENTS (bf16, or bytes when quantised); [pages, heads, page_size, 128] storage keeps a head's rows of a page together.
+ * Quantised: e4m3 codes (never NaN) and one byte e per row, in exps[page, at, head] with strides of their own; a code
+ * stands for code * 2^(e - 127).  e - 127 is the smallest integer, at least -120, with max|row| <= 448 * 2^(e - 127); the
+ * values are exact bf16 numbers.  A row that holds a NaN or an infinity has e = 255 and reads back as NaNs.
+ */
+typedef struct h3a_cache {
+  void* k;
+  void* v;
+  uint8_t* k_exp; /* quantised only, else NULL */
+  uint8_t* v_exp;
+  int64_t k_stride_page, k_stride_token, k_stride_head;
+  int64_t v_stride_page, v_stride_token, v_stride_head;
+  int64_t k_exp_stride_page, k_exp_stride_token, k_exp_stride_head;
+  int64_t v_exp_stride_page, v_exp_stride_token, v_exp_stride_head;
+  int32_t n_pages;
+  int32_t page_size; /* tokens, a multiple of 16, at most 65536 */
+  int32_t heads;     /* K/V heads */
+  int32_t d;         /* must be 128 */
+  int32_t quantised; /* 0: bf16, 1: e4m3 codes and exponent bytes */
+} h3a_cache;
+
+/*
+ * Which tokens a call is about.  Sequence b holds lengths[b] tokens, token p in row p % page_size of page
+ * pages[b * pages_stride + p / page_size].  Rows starts[b] .. starts[b + 1] - 1 of a packed [rows, heads, 128] tensor are
+ * its LAST n_b = starts[b + 1] - starts[b] tokens: row starts[b] + i is the token at position lengths[b] - n_b + i.  A
+ * negative position is outside the cache: it is not written, reads back as zeros and sees nothing under a causal mask.
+ * Rows outside every sequence are left as they are.  The arrays live on the device and may change between the replays of
+ * a captured graph.  They are checked there: a page outside [0, n_pages), a length outside [0, max_pages * page_size] or
+ * offsets that leave [0, rows] or decrease are never followed (the number is clamped, a row without a page is dropped) and
+ * the status word (when given) receives code 10 (H3A_ERR_INDEX); that call's results must not be used.
+ */
+typedef struct h3a_cache_batch {
+  const int32_t* pages;   /* [n_seqs, max_pages] */
+  int64_t pages_stride;
+  const int32_t* lengths; /* [n_seqs] */
+  const int32_t* starts;  /* [n_seqs + 1], non-decreasing */
+  int32_t n_seqs, max_pages;
+  int32_t rows;           /* rows of the packed tensors */
+} h3a_cache_batch;
+
+/*
+ * Packed rows of K and V -> cache (quantised on the way if the cache is), and back (bf16).  k, v: [rows, heads, 128] bf16
+ * by element strides, 16-byte aligned.  No two rows of a write may name the same row of the cache: a page that is written to belongs to
+ * one sequence of the batch (pages that are only read may be shared), and which of two rows stays is not defined.
+ */
+int32_t h3a_cache_write(const h3a_cache* cache, const h3a_cache_batch* batch, const void* k, int64_t k_stride_l, int64_t k_stride_h,
+                        const void* v, int64_t v_stride_l, int64_t v_stride_h, int32_t* status_word, void* stream);
+int32_t h3a_cache_read(const h3a_cache* cache, const h3a_cache_batch* batch, void* k, int64_t k_stride_l, int64_t k_stride_h,
+                       void* v, int64_t v_stride_l, int64_t v_stride_h, int32_t* status_word, void* stream);
+
+/*
+ * Attention of the batch's rows over the cached keys of their sequences: query row of token p sees the keys at positions
+ * 0 .. lengths[b] - 1, or with `causal` 0 .. p (the rows' own K and V are written first).  Query head h reads K/V head
+ * h / (heads / cache.heads).  Without a causal mask the rows need not be tokens of the cache: cross attention to cached
+ * states of any other length.  A row that sees no key is zeros, its log-sum-exp -inf.  What lies in a page behind a
+ * sequence's last key, and values that the causal mask hides, never reach a result, NaN and infinities included.
+ */
+typedef struct h3a_cache_attn_params {
+  h3a_cache cache;
+  h3a_cache_batch batch;  /* batch.rows = rows of q and o */
+  const void* q;          /* [rows, heads, 128] bf16 */
+  void* o;                /* [rows, heads, 128] bf16 */
+  float* lse;             /* optional [heads, rows] fp32, natural logarithm */
+  int64_t q_stride_l, q_stride_h, o_stride_l, o_stride_h;
+  int32_t heads;          /* query heads, a multiple of cache.heads */
+  int32_t causal;
+  float softmax_scale;    /* <= 0 selects 1/sqrt(d) */
+  void* workspace;        /* h3a_cache_attn_workspace_bytes() bytes, 16-byte aligned; used by this call alone until it is done */
+  size_t workspace_bytes;
+  int32_t* status_word;   /* as in h3a_attn_params */
+  int64_t wait_limit_ns;  /* as in h3a_attn_params */
+} h3a_cache_attn_params;
+int32_t h3a_cache_attn_workspace_bytes(const h3a_cache_attn_params* p, size_t* bytes);
+int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream);
+
 /* Copy the device status word to the host after synchronising `stream`.  Returns H3A_OK for 0, H3A_ERR_INDEX when a
  * block index failed its device-side check (low byte 10), H3A_ERR_BOUND when a logit bound did not hold (low byte
  * 11), H3A_ERR_TIMEOUT for every other non-zero value; *raw (optional)

@@ -10,6 +10,7 @@ from ._lib import (
     MODE_FP8_QK,
     H3AError,
 )
+from .cache import CacheBatch, KVCache, cache_attn, cache_attn_workspace_bytes, cache_read, cache_write
 from .graphs import StepGraph, renoise_sample
 from .host_path import HostJointAttention
 from .layout import position_grid
@@ -34,4 +35,5 @@ __all__ = [
     "_lib", "ops", "H3AError", "MODE_DENSE_BF16", "MODE_FP8_QK", "MODE_BLOCK_SPARSE",
     "BlockIndex", "adaln_norm", "attn_fwd", "attn_fwd_sparse_static", "static_scratch_capacity", "build_block_index", "joint_attention", "proj_fwd", "qk_prep",
     "read_status", "check_status", "StatusWord", "rope_table", "rope_table_from_cos_sin", "position_grid", "HostJointAttention", "StepGraph", "renoise_sample",
+    "KVCache", "CacheBatch", "cache_write", "cache_read", "cache_attn", "cache_attn_workspace_bytes",
 ]

@@ -49,6 +49,10 @@ EXPORTS = (
     "h3a_peer_open",
     "h3a_peer_close",
     "h3a_peer_free",
+    "h3a_cache_write",
+    "h3a_cache_read",
+    "h3a_cache_attn_workspace_bytes",
+    "h3a_cache_attn",
 )
 
 
@@ -108,6 +112,34 @@ class AdaLnParams(C.Structure):
         ("idx", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p),
         ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("scale_stride", C.c_int64), ("shift_stride", C.c_int64),
         ("L", C.c_int32), ("D", C.c_int32), ("T", C.c_int32), ("rms", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+class Cache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+        ("k_stride_page", C.c_int64), ("k_stride_token", C.c_int64), ("k_stride_head", C.c_int64),
+        ("v_stride_page", C.c_int64), ("v_stride_token", C.c_int64), ("v_stride_head", C.c_int64),
+        ("k_exp_stride_page", C.c_int64), ("k_exp_stride_token", C.c_int64), ("k_exp_stride_head", C.c_int64),
+        ("v_exp_stride_page", C.c_int64), ("v_exp_stride_token", C.c_int64), ("v_exp_stride_head", C.c_int64),
+        ("n_pages", C.c_int32), ("page_size", C.c_int32), ("heads", C.c_int32), ("d", C.c_int32), ("quantised", C.c_int32),
+    ]
+
+
+class CacheBatch(C.Structure):
+    _fields_ = [
+        ("pages", C.c_void_p), ("pages_stride", C.c_int64), ("lengths", C.c_void_p), ("starts", C.c_void_p),
+        ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("rows", C.c_int32),
+    ]
+
+
+class CacheAttnParams(C.Structure):
+    _fields_ = [
+        ("cache", Cache), ("batch", CacheBatch),
+        ("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+        ("q_stride_l", C.c_int64), ("q_stride_h", C.c_int64), ("o_stride_l", C.c_int64), ("o_stride_h", C.c_int64),
+        ("heads", C.c_int32), ("causal", C.c_int32), ("softmax_scale", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status_word", C.c_void_p), ("wait_limit_ns", C.c_int64),
     ]
 
 
@@ -171,6 +203,15 @@ def load() -> C.CDLL:
     lib.h3a_peer_close.restype = C.c_int32
     lib.h3a_peer_free.argtypes = [C.c_void_p]
     lib.h3a_peer_free.restype = C.c_int32
+    rows = [C.POINTER(Cache), C.POINTER(CacheBatch), C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]
+    lib.h3a_cache_write.argtypes = rows
+    lib.h3a_cache_write.restype = C.c_int32
+    lib.h3a_cache_read.argtypes = rows
+    lib.h3a_cache_read.restype = C.c_int32
+    lib.h3a_cache_attn_workspace_bytes.argtypes = [C.POINTER(CacheAttnParams), C.POINTER(C.c_size_t)]
+    lib.h3a_cache_attn_workspace_bytes.restype = C.c_int32
+    lib.h3a_cache_attn.argtypes = [C.POINTER(CacheAttnParams), C.c_void_p]
+    lib.h3a_cache_attn.restype = C.c_int32
     _lib = lib
     return lib
 

@@ -6,9 +6,10 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "h3attn_api.cu")
+SRCS = [os.path.join(HERE, "csrc", f) for f in ("h3attn_api.cu", "kv_cache_api.cu")]
 OUT = os.path.join(HERE, "libh3attn.so")
-DEPS = [SRC] + [os.path.join(HERE, "csrc", f) for f in ("attn_fwd.cuh", "attn_fwd_pair.cuh", "qk_prep.cuh", "qkv_proj.cuh", "adaln.cuh", "ptx.cuh")] + [
+DEPS = SRCS + [os.path.join(HERE, "csrc", f) for f in ("attn_fwd.cuh", "attn_fwd_pair.cuh", "qk_prep.cuh", "qkv_proj.cuh", "adaln.cuh", "ptx.cuh",
+                                                       "kv_cache.cuh", "cache_attn.cuh")] + [
     os.path.join(HERE, "..", "include", "h3attn.h")
 ]
 
@@ -31,7 +32,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return OUT
     nvcc = os.environ.get("NVCC", "nvcc")
-    cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", OUT, SRC, "-lcudart"]
+    cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", OUT] + SRCS + ["-lcudart"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)

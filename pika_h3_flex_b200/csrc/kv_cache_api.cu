@@ -1,0 +1,225 @@
+// C-ABI entry points of the paged K/V cache: argument validation and kernel launches.  Contracts live in include/h3attn.h.
+#include "../../include/h3attn.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <mutex>
+
+#include "cache_attn.cuh"
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// rows can be moved 16 bytes at a time; what is only read may repeat a row (stride 0)
+bool rows16(int64_t stride, int64_t elem, bool read_only = false) { return (stride > 0 || (read_only && stride == 0)) && (stride * elem) % 16 == 0; }
+
+struct Device {
+  int id = -1, sms = 0, major = 0;
+};
+int32_t current_device(Device* d) {
+  static Device known[kMaxDevices];
+  static std::mutex lock;
+  int id = 0;
+  if (cudaGetDevice(&id) != cudaSuccess || id < 0 || id >= kMaxDevices) return H3A_ERR_LAUNCH;
+  std::lock_guard<std::mutex> g(lock);
+  if (known[id].id < 0) {
+    Device n;
+    if (cudaDeviceGetAttribute(&n.major, cudaDevAttrComputeCapabilityMajor, id) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n.sms, cudaDevAttrMultiProcessorCount, id) != cudaSuccess)
+      return H3A_ERR_LAUNCH;
+    n.id = id;
+    known[id] = n;
+  }
+  *d = known[id];
+  return d->major == 10 ? H3A_OK : H3A_ERR_ARCH;
+}
+
+// Checks a cache and a batch and fills the kernels' view of them.
+int32_t cache_args(const h3a_cache* c, const h3a_cache_batch* b, int32_t* status, h3a::CacheArgs* a) {
+  if (!c || !b || !c->k || !c->v || !b->pages || !b->lengths || !b->starts) return H3A_ERR_ARG;
+  if (c->quantised != 0 && c->quantised != 1) return H3A_ERR_ARG;
+  if (c->quantised ? (!c->k_exp || !c->v_exp) : (c->k_exp || c->v_exp)) return H3A_ERR_ARG;
+  if (c->d != 128 || c->n_pages <= 0 || c->heads <= 0 || c->page_size <= 0 || c->page_size % 16 || c->page_size > 65536) return H3A_ERR_SHAPE;
+  if (b->n_seqs <= 0 || b->max_pages <= 0 || b->rows <= 0) return H3A_ERR_SHAPE;
+  if (static_cast<int64_t>(b->max_pages) * c->page_size > (1ll << 28)) return H3A_ERR_SHAPE;
+  if (static_cast<int64_t>(b->rows) * 2 * c->heads >= (1ll << 31)) return H3A_ERR_SHAPE;
+  if (b->pages_stride < 0) return H3A_ERR_ARG;
+  const int64_t es = c->quantised ? 1 : 2;
+  if (!aligned16(c->k) || !aligned16(c->v)) return H3A_ERR_ALIGN;
+  const int64_t strides[2][3] = {{c->k_stride_page, c->k_stride_token, c->k_stride_head}, {c->v_stride_page, c->v_stride_token, c->v_stride_head}};
+  for (auto& s : strides)
+    for (int64_t x : s)
+      if (!rows16(x, es)) return H3A_ERR_ALIGN;
+  std::memset(a, 0, sizeof(*a));
+  a->pool[0] = static_cast<uint8_t*>(c->k);
+  a->pool[1] = static_cast<uint8_t*>(c->v);
+  for (int x = 0; x < 2; ++x) {
+    a->page_bytes[x] = strides[x][0] * es;
+    a->token_bytes[x] = strides[x][1] * es;
+    a->head_bytes[x] = strides[x][2] * es;
+  }
+  a->exps[0] = c->k_exp;
+  a->exps[1] = c->v_exp;
+  a->exp_page[0] = c->k_exp_stride_page;
+  a->exp_token[0] = c->k_exp_stride_token;
+  a->exp_head[0] = c->k_exp_stride_head;
+  a->exp_page[1] = c->v_exp_stride_page;
+  a->exp_token[1] = c->v_exp_stride_token;
+  a->exp_head[1] = c->v_exp_stride_head;
+  a->pages = b->pages;
+  a->pages_stride = b->pages_stride;
+  a->lengths = b->lengths;
+  a->starts = b->starts;
+  a->n_seqs = b->n_seqs;
+  a->max_pages = b->max_pages;
+  a->n_pages = c->n_pages;
+  a->page_size = c->page_size;
+  a->kv_heads = c->heads;
+  a->rows = b->rows;
+  a->status = status;
+  return H3A_OK;
+}
+
+int32_t move_rows(bool write, const h3a_cache* c, const h3a_cache_batch* b, void* k, int64_t k_sl, int64_t k_sh, void* v, int64_t v_sl,
+                  int64_t v_sh, int32_t* status, void* stream) {
+  h3a::RowsArgs a;
+  int32_t rc = cache_args(c, b, status, &a.c);
+  if (rc != H3A_OK) return rc;
+  if (!k || !v) return H3A_ERR_ARG;
+  if (!aligned16(k) || !aligned16(v) || !rows16(k_sl, 2, write) || !rows16(k_sh, 2, write) || !rows16(v_sl, 2, write) || !rows16(v_sh, 2, write))
+    return H3A_ERR_ALIGN;
+  Device dev;
+  if ((rc = current_device(&dev)) != H3A_OK) return rc;
+  a.x[0] = static_cast<uint8_t*>(k);
+  a.x[1] = static_cast<uint8_t*>(v);
+  a.row_bytes[0] = k_sl * 2;
+  a.head_bytes[0] = k_sh * 2;
+  a.row_bytes[1] = v_sl * 2;
+  a.head_bytes[1] = v_sh * 2;
+  const int64_t units = static_cast<int64_t>(b->rows) * 2 * c->heads, per_block = h3a::kRowThreads / 16;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((units + per_block - 1) / per_block, 8ll * dev.sms));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (write) {
+    if (c->quantised) h3a::cache_rows_kernel<true, true><<<grid, h3a::kRowThreads, 0, st>>>(a);
+    else h3a::cache_rows_kernel<true, false><<<grid, h3a::kRowThreads, 0, st>>>(a);
+  } else {
+    if (c->quantised) h3a::cache_rows_kernel<false, true><<<grid, h3a::kRowThreads, 0, st>>>(a);
+    else h3a::cache_rows_kernel<false, false><<<grid, h3a::kRowThreads, 0, st>>>(a);
+  }
+  return cudaGetLastError() == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
+}
+
+constexpr int kFewMinShare = 3;  // units (a tile, or an item's set-up) below which a share is not worth a CTA
+
+// What a call of this shape launches.
+struct AttnPlan {
+  int item_rows = 0, item_tokens = 0, shares = 0;
+  size_t bytes = 0;
+};
+AttnPlan attn_plan(const h3a_cache_attn_params* p, int sms) {
+  AttnPlan n;
+  n.item_rows = h3a::kFewRows;
+  n.shares = sms;
+  n.bytes = static_cast<size_t>(n.shares) * (4 * sizeof(int) + 2ull * n.item_rows * (h3a::kCacheDim + 2) * sizeof(float));
+  return n;
+}
+
+template <typename K>
+int32_t allow_smem(K kernel, int bytes, int dev, std::once_flag* once, cudaError_t* err) {
+  std::call_once(once[dev], [&] { err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+  return err[dev] == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
+}
+
+template <bool kFp8>
+int32_t launch_few(const h3a::CacheAttnArgs& a, int shares, const Device& dev, cudaStream_t st) {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  const int32_t rc = allow_smem(h3a::cache_attn_few_kernel<kFp8>, h3a::kFewSmemBytes, dev.id, once, err);
+  if (rc != H3A_OK) return rc;
+  h3a::cache_attn_few_kernel<kFp8><<<shares, h3a::kFewThreads, h3a::kFewSmemBytes, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
+}
+
+int32_t launch_join(const h3a::CacheAttnArgs& a, int shares, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(shares, (a.item_rows + h3a::kJoinRows - 1) / h3a::kJoinRows);
+  cfg.blockDim = dim3(h3a::kJoinRows * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the end of the kernel before it
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, h3a::cache_attn_join_kernel, a) == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t h3a_cache_write(const h3a_cache* cache, const h3a_cache_batch* batch, const void* k, int64_t k_stride_l, int64_t k_stride_h,
+                        const void* v, int64_t v_stride_l, int64_t v_stride_h, int32_t* status_word, void* stream) {
+  return move_rows(true, cache, batch, const_cast<void*>(k), k_stride_l, k_stride_h, const_cast<void*>(v), v_stride_l, v_stride_h,
+                   status_word, stream);
+}
+
+int32_t h3a_cache_read(const h3a_cache* cache, const h3a_cache_batch* batch, void* k, int64_t k_stride_l, int64_t k_stride_h,
+                       void* v, int64_t v_stride_l, int64_t v_stride_h, int32_t* status_word, void* stream) {
+  return move_rows(false, cache, batch, k, k_stride_l, k_stride_h, v, v_stride_l, v_stride_h, status_word, stream);
+}
+
+int32_t h3a_cache_attn_workspace_bytes(const h3a_cache_attn_params* p, size_t* bytes) {
+  if (!p || !bytes) return H3A_ERR_ARG;
+  if (p->cache.heads <= 0 || p->heads <= 0 || p->heads % p->cache.heads || p->batch.rows <= 0 || p->batch.n_seqs <= 0) return H3A_ERR_SHAPE;
+  Device dev;
+  const int32_t rc = current_device(&dev);
+  if (rc != H3A_OK) return rc;
+  *bytes = attn_plan(p, dev.sms).bytes;
+  return H3A_OK;
+}
+
+int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
+  if (!p || !p->q || !p->o) return H3A_ERR_ARG;
+  h3a::CacheAttnArgs a;
+  std::memset(&a, 0, sizeof(a));
+  int32_t rc = cache_args(&p->cache, &p->batch, p->status_word, &a.c);
+  if (rc != H3A_OK) return rc;
+  if (p->heads <= 0 || p->heads % p->cache.heads || static_cast<int64_t>(p->batch.rows) * p->heads >= (1ll << 31)) return H3A_ERR_SHAPE;
+  if (p->causal != 0 && p->causal != 1) return H3A_ERR_ARG;
+  if (!aligned16(p->q) || !aligned16(p->o) || !rows16(p->q_stride_l, 2, true) || !rows16(p->q_stride_h, 2, true) || !rows16(p->o_stride_l, 2) ||
+      !rows16(p->o_stride_h, 2))
+    return H3A_ERR_ALIGN;
+  Device dev;
+  if ((rc = current_device(&dev)) != H3A_OK) return rc;
+  const AttnPlan n = attn_plan(p, dev.sms);
+  if (!p->workspace || p->workspace_bytes < n.bytes) return H3A_ERR_WORKSPACE;
+  if (!aligned16(p->workspace)) return H3A_ERR_ALIGN;
+  a.q = static_cast<const uint8_t*>(p->q);
+  a.q_row_bytes = p->q_stride_l * 2;
+  a.q_head_bytes = p->q_stride_h * 2;
+  a.o = static_cast<__nv_bfloat16*>(p->o);
+  a.o_stride_l = p->o_stride_l;
+  a.o_stride_h = p->o_stride_h;
+  a.lse = p->lse;
+  a.heads = p->heads;
+  a.group = p->heads / p->cache.heads;
+  a.causal = p->causal;
+  a.item_rows = n.item_rows;
+  a.item_tokens = n.item_tokens;
+  a.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / std::sqrt(128.0f)) * 1.4426950408889634f;
+  a.desc = static_cast<int*>(p->workspace);
+  a.part = reinterpret_cast<float*>(a.desc + 4 * n.shares);
+  a.min_share = kFewMinShare;
+  a.wait_ns = p->wait_limit_ns > 0 ? p->wait_limit_ns : 2000000000ll;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  rc = p->cache.quantised ? launch_few<true>(a, n.shares, dev, st) : launch_few<false>(a, n.shares, dev, st);
+  return rc == H3A_OK ? launch_join(a, n.shares, st) : rc;
+}
+
+}  // extern "C"
