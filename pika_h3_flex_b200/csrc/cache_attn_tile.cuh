@@ -1,0 +1,648 @@
+// Attention of many new rows over a paged K/V cache: tcgen05 MMAs, the work distribution of cache_attn.cuh.
+//
+// One CTA per SM walks its share of the units piece by piece.  A piece is up to 2 x 128 query rows (two "streams", each
+// floor(128 / group) tokens x the group's heads, so that shared K/V heads fill the rows) against a run of 128-key tiles.
+//   warps 0-3 / 4-7  softmax of stream 0 / 1, one row per thread (TMEM lane == row): running maximum, exp2, row sum,
+//                    P written back over S as packed bf16, lazy rescale of O (when the maximum grows by more than 2^8)
+//   warp 8           producer: TMA loads of Q and of the K and V tiles, page by page, into a ring
+//   warps 9, 10      issuers, one per stream: S = Q K^T (N = 64 keys), O += P V (P from TMEM), tcgen05.commit
+//   warps 12-15      helpers, one cache row per thread.  e4m3: widen a staged tile to bf16 (exact, the row's power of two
+//                    included) into the ring.  bf16: let tiles through, except the V tiles that not every row sees whole:
+//                    P is 0 for a key a row does not see, and 0 x NaN is NaN, so rows behind the last key become zeros
+//                    and values that are not finite become zeros until the epilogue puts them back for the rows that
+//                    do see them.
+// Each 128-key tile is processed as two 64-key halves with S buffers of their own, so that a stream has two S / P buffers
+// in flight, as in the dense kernels.  TMEM: stream t: S/P buffer h at columns [128 t + 64 h, +64), O at [256 + 128 t, +128).
+//
+// Every wait is bounded: when the limit runs out the CTA records a code in the status word, raises a CTA-wide flag that the
+// other waits poll, lets copies in flight land, frees TMEM and returns.
+#pragma once
+#include "cache_attn.cuh"
+
+namespace h3a {
+
+constexpr int kTileThreads = 512;
+constexpr int kTileSoftmaxRegs = 192, kTileOtherRegs = 64, kTileLaunchRegs = 128;
+static_assert(256 * kTileSoftmaxRegs + 256 * kTileOtherRegs <= kTileLaunchRegs * kTileThreads, "setmaxnreg budget exceeds the launch allocation");
+constexpr int kTileRows = 256;         // rows of an item
+constexpr int kTileBytes = 32768;      // 128 rows of 128 bf16
+constexpr int kTileHalf = 16384;       // one [128 rows][128 bytes] swizzled box
+constexpr int kCodeBytes = 16384;      // 128 rows of 128 codes
+template <bool kFp8>
+struct TileRing {
+  static constexpr int kRing = kFp8 ? 3 : 5;     // bf16 tiles
+  static constexpr int kStaged = kFp8 ? 4 : 0;   // e4m3 tiles as loaded
+  static constexpr int kBytes = kRing * kTileBytes + kStaged * kCodeBytes;
+};
+
+struct TileBars {
+  uint64_t full[5];        // ring slot: copies have landed (bf16)
+  uint64_t ready[5];       // ring slot: may be read by MMAs
+  uint64_t empty[5];       // ring slot: both issuers' MMAs are done with it
+  uint64_t staged[4];      // e4m3: copies have landed
+  uint64_t unstaged[4];    // e4m3: widened
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2][2], p_full[2][2], o_full[2][2];  // [stream][half]
+  uint64_t o_free[2];
+  uint32_t tmem_base;
+  uint32_t early_exit;
+  volatile uint32_t abort_flag;
+  volatile uint32_t poison;  // some V value counted as zero: from then on every epilogue looks for such values
+};
+constexpr int kTileSmemBytes = 2 * kTileBytes + TileRing<false>::kBytes + 1024 + 512;
+static_assert(TileRing<true>::kBytes <= TileRing<false>::kBytes && sizeof(TileBars) <= 512, "shared memory layout");
+static_assert(kTileSmemBytes + sizeof(ShareStart) <= 232448, "shared memory budget");
+
+enum : int {  // status codes of waits that ran out (low byte of the status word)
+  kTileWaitEmpty = 33, kTileWaitFull, kTileWaitReady, kTileWaitUnstaged, kTileWaitStaged, kTileWaitQFull, kTileWaitQEmpty,
+  kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree
+};
+
+struct TileWait {
+  const CacheAttnArgs& a;
+  TileBars* bars;
+  __device__ __forceinline__ bool one(uint64_t& barrier, uint32_t parity, int code) const {
+    const uint32_t bar = smem_u32(&barrier);
+    if (mbar_try_wait(bar, parity)) return true;
+    uint32_t polls = 0;
+    uint64_t t0 = 0;
+    while (!mbar_try_wait(bar, parity)) {
+      if ((++polls & 63u) == 0u) {
+        if (bars->abort_flag) return false;
+        const uint64_t now = global_timer_ns();
+        if (t0 == 0) {
+          t0 = now;
+        } else if (static_cast<long long>(now - t0) > a.wait_ns) {
+          bars->abort_flag = 1u;
+          if (a.c.status) atomicCAS(a.c.status, 0, code | (static_cast<int>(blockIdx.x) << 8));
+          return false;
+        }
+      }
+    }
+    return true;
+  }
+  // the whole warp, with one verdict
+  __device__ __forceinline__ bool operator()(uint64_t& barrier, uint32_t parity, int code) const {
+    return __all_sync(0xFFFFFFFFu, one(barrier, parity, code));
+  }
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// What every role derives from a piece in the same way.
+struct TilePiece {
+  int tok0;        // first token of stream 0
+  int n_tiles;
+  int end[2];      // key tiles of the piece that the stream takes part in: [0, end)
+  int lim_min, lim_max;
+  __device__ __forceinline__ TilePiece(const CacheAttnArgs& a, const Piece& p) {
+    const int T = a.item_tokens >> 1;
+    tok0 = p.it * a.item_tokens;
+    n_tiles = p.t1 - p.t0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int first = tok0 + t * T, last = min(p.s.n, first + T) - 1;
+      end[t] = last >= first ? max(0, min(p.t1, (key_limit(a, p.s, last) + kKeyTile - 1) / kKeyTile) - p.t0) : 0;
+    }
+    lim_min = key_limit(a, p.s, tok0);
+    lim_max = key_limit(a, p.s, item_last_token(a, p.s, p.it));
+  }
+};
+
+// rows [0, box_rows) of a 4-D page box are whole keys of one page: box_rows divides the page size and the tile
+template <bool kFp8>
+__global__ void __launch_bounds__(kTileThreads, 1)
+cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const int box_rows, const __grid_constant__ CacheAttnArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ ShareStart start;
+  using R = TileRing<kFp8>;
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw_addr);
+  const uint32_t q_smem = base, ring = base + 2 * kTileBytes, staging = ring + R::kRing * kTileBytes;
+  TileBars* bars = reinterpret_cast<TileBars*>(smem + 2 * kTileBytes + TileRing<false>::kBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < R::kRing; ++i) {
+      mbar_init(smem_u32(&bars->full[i]), 1);
+      mbar_init(smem_u32(&bars->ready[i]), 4);   // one arrive per helper warp
+      mbar_init(smem_u32(&bars->empty[i]), 2);   // one commit per issuer
+    }
+    for (int i = 0; i < R::kStaged; ++i) {
+      mbar_init(smem_u32(&bars->staged[i]), 1);
+      mbar_init(smem_u32(&bars->unstaged[i]), 4);
+    }
+    mbar_init(smem_u32(&bars->q_full), 1);
+    mbar_init(smem_u32(&bars->q_empty), 2);
+    for (int t = 0; t < 2; ++t) {
+      for (int hf = 0; hf < 2; ++hf) {
+        mbar_init(smem_u32(&bars->s_full[t][hf]), 1);
+        mbar_init(smem_u32(&bars->p_full[t][hf]), 128);
+        mbar_init(smem_u32(&bars->o_full[t][hf]), 1);
+      }
+      mbar_init(smem_u32(&bars->o_free[t]), 4);
+    }
+    bars->abort_flag = 0;
+    bars->poison = 0;
+    bars->early_exit = (a.c.status != nullptr && *reinterpret_cast<volatile int*>(a.c.status) != 0) ? 1u : 0u;
+    fence_mbar_init();
+    a.desc[4 * blockIdx.x] = -1;
+  }
+  if (warp == 8 && lane == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
+  ShareIter iter = share_begin(a, &start);  // has block-wide barriers
+  if (bars->early_exit) return;
+  if (warp == 9) {
+    tmem_alloc(smem_u32(&bars->tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = bars->tmem_base;
+  const TileWait wait{a, bars};
+  const int T = a.item_tokens >> 1;
+  Piece p;
+
+  if (warp >= 12) {
+    // =========================================================== helpers: thread r owns row r of every tile
+    setmaxnreg_dec<kTileOtherRegs>();
+    const int row = threadIdx.x - 384;
+    const uint32_t swz = row & 7;
+    int cnt = 0;
+    bool ok = true;
+    while (ok && iter.next(a, p)) {
+      const TilePiece tp(a, p);
+      if (tp.n_tiles == 0) continue;
+      uint32_t ex[2] = {0, 0};  // e4m3: exponent bytes of this thread's row of the tile to come
+      auto fetch_ex = [&](int tile) {
+        const int key = tile * kKeyTile + row;
+        if (kFp8 && key < tp.lim_max) {
+          const int slot = key / a.c.page_size, at = key - slot * a.c.page_size;
+          const long long id = checked_page(a, p.b, slot);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) ex[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + p.h * a.c.exp_head[x]);
+        }
+      };
+      fetch_ex(p.t0);
+      for (int it = 0; ok && it < tp.n_tiles; ++it) {
+        const int tile = p.t0 + it, key = tile * kKeyTile + row;
+        const bool special = (tile + 1) * kKeyTile > tp.lim_min;
+        const uint32_t e_now[2] = {ex[0], ex[1]};
+        if (it + 1 < tp.n_tiles) fetch_ex(tile + 1);
+#pragma unroll
+        for (int x = 0; x < 2; ++x, ++cnt) {  // K, then V
+          const int s = cnt % R::kRing;
+          const uint32_t ph = (cnt / R::kRing) & 1;
+          const uint32_t dst = ring + s * kTileBytes + row * 128;
+          if constexpr (kFp8) {
+            const int g = cnt % R::kStaged;
+            ok = wait(bars->staged[g], (cnt / R::kStaged) & 1, kTileWaitStaged) && wait(bars->empty[s], ph ^ 1u, kTileWaitEmpty);
+            if (!ok) break;
+            const uint32_t src = staging + g * kCodeBytes + row * 128;
+            uint32_t f = e4m3_factor(e_now[x]) * 0x10001u;
+            const uint32_t f2 = e4m3_factor2(e_now[x]) * 0x10001u;
+            if (key >= tp.lim_max) {
+              f = 0;
+            } else if (x == 1 && special && e_now[x] == 255u) {
+              f = 0;
+              bars->poison = 1u;
+            }
+            const bool two = __any_sync(0xFFFFFFFFu, e_now[x] > kOneStepExp);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint4 w;
+              ld_shared_v4(src + ((c ^ swz) << 4), w);
+              const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+              uint32_t o[8];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                o[2 * y] = mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x1404)), f);
+                o[2 * y + 1] = mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x3424)), f);
+              }
+              if (two) {
+#pragma unroll
+                for (int y = 0; y < 8; ++y) o[y] = mul_bf16x2(o[y], f2);
+              }
+              const uint32_t at = dst + (c >> 2) * kTileHalf;
+              st_shared_v4(at + (((2 * (c & 3)) ^ swz) << 4), o[0], o[1], o[2], o[3]);
+              st_shared_v4(at + (((2 * (c & 3) + 1) ^ swz) << 4), o[4], o[5], o[6], o[7]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(smem_u32(&bars->ready[s]));
+              mbar_arrive(smem_u32(&bars->unstaged[g]));
+            }
+          } else {
+            ok = wait(bars->full[s], ph, kTileWaitFull);
+            if (!ok) break;
+            if (x == 1 && special) {
+              const bool gone = key >= tp.lim_max;
+              bool bad = false;
+#pragma unroll 4
+              for (int c = 0; c < 16; ++c) {
+                const uint32_t at = dst + (c >> 3) * kTileHalf + (((c & 7) ^ swz) << 4);
+                uint4 w = make_uint4(0, 0, 0, 0);
+                bool put = gone;
+                if (!gone) {
+                  ld_shared_v4(at, w);
+                  put = non_finite2(w.x) || non_finite2(w.y) || non_finite2(w.z) || non_finite2(w.w);
+                  bad |= put;
+                  w = make_uint4(finite_or_zero2(w.x), finite_or_zero2(w.y), finite_or_zero2(w.z), finite_or_zero2(w.w));
+                }
+                if (put) st_shared_v4(at, w.x, w.y, w.z, w.w);
+              }
+              if (bad) bars->poison = 1u;
+              fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars->ready[s]));
+          }
+        }
+      }
+    }
+  } else if (warp >= 8) {
+    setmaxnreg_dec<kTileOtherRegs>();
+    if (warp == 8) {
+      // ========================================================= producer: lane x copies sub-box x of a tile
+      const int n_boxes = kKeyTile / box_rows;
+      const int box_bytes = box_rows * (kFp8 ? kCacheDim : 2 * kCacheDim);
+      const uint32_t q_bytes = T * a.group * 256;
+      int cnt = 0;
+      uint32_t g = 0;  // pieces with work so far: the phase of q_full / q_empty
+      bool ok = true;
+      while (ok && iter.next(a, p)) {
+        const TilePiece tp(a, p);
+        if (tp.n_tiles == 0) continue;
+        // Q is free late in the previous piece, ring slots earlier: the first two key tiles go ahead of Q
+        const int q_at = g > 0 ? min(2, tp.n_tiles - 1) : 0;
+        bool q_loaded = false;
+        // page and place of this lane's sub-box of a tile; none behind the last key
+        int id = -1;
+        auto fetch_page = [&](int tile) {
+          const int key = tile * kKeyTile + lane * box_rows;
+          id = lane < n_boxes && key < tp.lim_max ? checked_page(a, p.b, key / a.c.page_size) : -1;
+        };
+        fetch_page(p.t0);
+        for (int it = 0; ok && it < tp.n_tiles; ++it) {
+          if (!q_loaded) {
+            bool q_free = g == 0 || __all_sync(0xFFFFFFFFu, mbar_test_wait(smem_u32(&bars->q_empty), (g - 1) & 1));
+            if (!q_free && it >= q_at) {
+              ok = wait(bars->q_empty, (g - 1) & 1, kTileWaitQEmpty);
+              if (!ok) break;
+              q_free = true;
+            }
+            if (q_free) {
+              if (lane == 0) {
+                const uint32_t bar = smem_u32(&bars->q_full);
+                const bool second = tp.tok0 + T < p.s.n;
+                mbar_arrive_expect_tx(bar, second ? 2 * q_bytes : q_bytes);
+                for (int t = 0; t < (second ? 2 : 1); ++t)
+                  for (int hf = 0; hf < 2; ++hf)
+                    tma_load_3d(q_smem + t * kTileBytes + hf * kTileHalf, &tm_q, bar, 64 * hf, p.h * a.group, p.s.s0 + tp.tok0 + t * T);
+              }
+              __syncwarp();
+              q_loaded = true;
+            }
+          }
+          const int tile = p.t0 + it;
+          const int now = id, at = (tile * kKeyTile + lane * box_rows) % a.c.page_size;
+          const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, now >= 0)) * box_bytes;
+          if (it + 1 < tp.n_tiles) fetch_page(tile + 1);
+#pragma unroll
+          for (int x = 0; x < 2; ++x, ++cnt) {
+            const CUtensorMap* tm = x ? &tm_v : &tm_k;
+            uint32_t dst, bar;
+            if constexpr (kFp8) {
+              const int s = cnt % R::kStaged;
+              ok = wait(bars->unstaged[s], ((cnt / R::kStaged) & 1) ^ 1u, kTileWaitUnstaged);
+              dst = staging + s * kCodeBytes + lane * box_rows * 128;
+              bar = smem_u32(&bars->staged[s]);
+            } else {
+              const int s = cnt % R::kRing;
+              ok = wait(bars->empty[s], ((cnt / R::kRing) & 1) ^ 1u, kTileWaitEmpty);
+              dst = ring + s * kTileBytes + lane * box_rows * 128;
+              bar = smem_u32(&bars->full[s]);
+            }
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+            __syncwarp();
+            if (now >= 0) {
+              tma_load_4d(dst, tm, bar, 0, at, p.h, now);
+              if constexpr (!kFp8) tma_load_4d(dst + kTileHalf, tm, bar, 64, at, p.h, now);
+            }
+            __syncwarp();
+          }
+        }
+        ++g;
+      }
+    } else if (warp < 11) {
+      // ========================================================= issuers, one warp per stream
+      const int t = warp - 9;
+      const uint32_t leader = elect_one();
+      constexpr uint32_t idesc_s = umma_idesc(UMMA_FMT_BF16, UMMA_FMT_BF16, 0, 0, 128, 64);
+      constexpr uint32_t idesc_pv = umma_idesc(UMMA_FMT_BF16, UMMA_FMT_BF16, 0, 1, 128, 128);
+      const uint64_t q_desc = umma_desc_sw128(q_smem + t * kTileBytes, 16, 1024);
+      const uint64_t k_desc0 = umma_desc_sw128(ring, 16, 1024);
+      const uint64_t v_desc0 = umma_desc_sw128(ring, kTileHalf, 1024);
+      const uint32_t s_tmem = tmem + t * 128, o_tmem = tmem + 256 + t * 128;
+      uint32_t p_cnt[2] = {0, 0};  // P halves consumed so far: the phase of p_full
+      uint32_t pv_cnt = 0;         // P V groups of the current piece: the first one overwrites O
+      uint32_t g = 0;              // pieces with work so far
+      uint32_t own = 0;            // pieces in which this stream had work: the phase of o_free
+      int c0 = 0;                  // ring tiles before the current piece
+      bool ok = true;
+      auto issue_s = [&](int hf, int s) {
+        const uint64_t kd = k_desc0 + static_cast<uint64_t>((s * kTileBytes + hf * 8192) >> 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t off = ((k >> 2) * kTileHalf + (k & 3) * 32) >> 4;
+          umma_bf16_ss_if(leader, s_tmem + hf * 64, q_desc + off, kd + off, idesc_s, k > 0);
+        }
+        umma_commit_if(leader, smem_u32(&bars->s_full[t][hf]));
+      };
+      auto issue_pv = [&](int hf, int s) {
+        const uint64_t vd = v_desc0 + static_cast<uint64_t>((s * kTileBytes + hf * 8192) >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_bf16_ts_if(leader, o_tmem, s_tmem + hf * 64 + k * 8, vd + (k * 2048 >> 4), idesc_pv, (pv_cnt > 0 || k > 0) ? 1u : 0u);
+        ++pv_cnt;
+        umma_commit_if(leader, smem_u32(&bars->o_full[t][hf]));
+      };
+      auto ready = [&](int c) {
+        const bool got = wait(bars->ready[c % R::kRing], (c / R::kRing) & 1, kTileWaitReady);
+        tc_fence_after_sync();
+        return got;
+      };
+      while (ok && iter.next(a, p)) {
+        const TilePiece tp(a, p);
+        if (tp.n_tiles == 0) continue;
+        const int n_mine = tp.end[t];
+        ok = wait(bars->q_full, g & 1, kTileWaitQFull) && ready(c0);
+        if (!ok) break;
+        pv_cnt = 0;
+        if (n_mine > 0) {
+          issue_s(0, c0 % R::kRing);
+          issue_s(1, c0 % R::kRing);
+        }
+        umma_commit_if(leader, smem_u32(&bars->empty[c0 % R::kRing]));
+        for (int it = 0; ok && it < tp.n_tiles; ++it) {
+          const bool has_next = it + 1 < tp.n_tiles;
+          const int cv = c0 + 2 * it + 1, ck = cv + 1;
+          if (!has_next) umma_commit_if(leader, smem_u32(&bars->q_empty));  // every S MMA of the piece has been issued
+          ok = ready(cv);
+          if (!ok) break;
+          bool k_ready = false;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            if (ok && it < n_mine) {
+              ok = wait(bars->p_full[t][hf], p_cnt[hf] & 1, kTileWaitP);
+              // the stream's softmax warps have read the previous piece's O
+              if (ok && pv_cnt == 0 && own > 0) ok = wait(bars->o_free[t], (own - 1) & 1, kTileWaitOFree);
+              if (ok) {
+                ++p_cnt[hf];
+                tc_fence_after_sync();
+                issue_pv(hf, cv % R::kRing);
+              }
+            }
+            if (ok && has_next && !k_ready) {
+              ok = ready(ck);
+              k_ready = ok;
+            }
+            if (ok && has_next && it + 1 < n_mine) issue_s(hf, ck % R::kRing);
+          }
+          if (!ok) break;
+          umma_commit_if(leader, smem_u32(&bars->empty[cv % R::kRing]));
+          if (has_next) umma_commit_if(leader, smem_u32(&bars->empty[ck % R::kRing]));
+        }
+        c0 += 2 * tp.n_tiles;
+        ++g;
+        if (n_mine > 0) ++own;
+      }
+    }
+    __syncwarp();
+  } else {
+    // =========================================================== softmax, rescaling, results
+    setmaxnreg_inc<kTileSoftmaxRegs>();
+    const int t = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + t * 128, o_addr = tmem + lane_base + 256 + t * 128;
+    uint32_t j = 0;  // key tiles the stream has processed: the phase of s_full / o_full
+    bool ok = true;
+    uint32_t ra[64], rb[64];
+    auto load_s = [&](uint32_t (&r)[64], int hf) {
+      tc_fence_after_sync();
+      tmem_ld32(s_addr + hf * 64, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+      tmem_ld32(s_addr + hf * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+    };
+    auto fetch_s = [&](uint32_t (&r)[64], int hf, uint32_t jt) {
+      const bool got = wait(bars->s_full[t][hf], jt & 1, kTileWaitS);
+      if (got) load_s(r, hf);
+      return got;
+    };
+    auto try_fetch_s = [&](uint32_t (&r)[64], int hf, uint32_t jt) {
+      const bool there = __all_sync(0xFFFFFFFFu, mbar_test_wait(smem_u32(&bars->s_full[t][hf]), jt & 1));
+      if (there) load_s(r, hf);
+      return there;
+    };
+    auto publish_p = [&](uint32_t (&s)[64], int hf) {
+      tmem_st32(s_addr + hf * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+      tmem_wait_st();
+      tc_fence_before_sync();
+      mbar_arrive(smem_u32(&bars->p_full[t][hf]));
+    };
+    while (ok && iter.next(a, p)) {
+      const TilePiece tp(a, p);
+      const int n_mine = tp.end[t];
+      const int first = tp.tok0 + t * T;
+      const int token = first + row / a.group;  // row r: token r / group, head r % group
+      const bool have_row = row < T * a.group && token < p.s.n;
+      const int lim = have_row ? key_limit(a, p.s, token) : 0;
+      const int lim_first = key_limit(a, p.s, first);  // the stream's first row sees fewest keys
+      float m_ref = kNoMax, l_sum = 0.f;
+
+      auto softmax_half = [&](uint32_t (&s)[64], int hf, int it) -> bool {
+        const int key0 = (p.t0 + it) * kKeyTile + hf * 64;
+        if (key0 + 64 > lim_first) {
+          const int valid = lim - key0;
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= valid) s[i] = 0xFF800000u;  // -inf
+        }
+        float mx0 = fmax3(__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]));
+        float mx1 = fmax3(__uint_as_float(s[3]), __uint_as_float(s[4]), __uint_as_float(s[5]));
+        float mx2 = fmax3(__uint_as_float(s[6]), __uint_as_float(s[7]), __uint_as_float(s[8]));
+        float mx3 = fmax3(__uint_as_float(s[9]), __uint_as_float(s[10]), __uint_as_float(s[11]));
+#pragma unroll
+        for (int i = 12; i < 60; i += 8) {
+          mx0 = fmax3(mx0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          mx1 = fmax3(mx1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+          mx2 = fmax3(mx2, __uint_as_float(s[i + 4]), __uint_as_float(s[i + 5]));
+          mx3 = fmax3(mx3, __uint_as_float(s[i + 6]), __uint_as_float(s[i + 7]));
+        }
+        mx0 = fmax3(mx0, __uint_as_float(s[60]), __uint_as_float(s[61]));
+        mx1 = fmax3(mx1, __uint_as_float(s[62]), __uint_as_float(s[63]));
+        const float m_tile = fmax3(fmaxf(mx0, mx1), mx2, mx3) * a.scale_log2;
+        if (it == 0 && hf == 0) {
+          m_ref = fmaxf(m_tile, kNoMax);
+        } else if (__any_sync(0xFFFFFFFFu, m_tile - m_ref > 8.0f)) {
+          const float m_new = fmaxf(m_ref, m_tile);
+          const float alpha = ex2_approx(m_ref - m_new);
+          m_ref = m_new;
+          l_sum *= alpha;
+          // the stream's previous P V must be complete; MMAs complete in issue order, so it is the only one that can run
+          if (!wait(bars->o_full[t][hf ^ 1], (hf ? j : j - 1) & 1, kTileWaitO)) return false;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + 32 * i, o);
+            tmem_wait_ld();
+            reg_fence32(o);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+            tmem_st32(o_addr + 32 * i, o);
+          }
+        }
+        // P = 2^(s c - m), rounded to bf16 once; the row sum keeps the unrounded terms
+        uint64_t acc0 = 0, acc1 = 0;
+        const uint64_t c2 = pack2(a.scale_log2, a.scale_log2), nm2 = pack2(-m_ref, -m_ref);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float x0, x1;
+          unpack2(fma2(pack2u(s[2 * i], s[2 * i + 1]), c2, nm2), x0, x1);
+          const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+          if (i & 1) acc1 = add2(acc1, pack2(p0, p1));
+          else acc0 = add2(acc0, pack2(p0, p1));
+          s[i] = pack_bf16x2(p0, p1);
+        }
+        float a0, a1, a2, a3;
+        unpack2(acc0, a0, a1);
+        unpack2(acc1, a2, a3);
+        l_sum += (a0 + a1) + (a2 + a3);
+        return true;
+      };
+
+      if (n_mine > 0) ok = fetch_s(ra, 0, j);
+      for (int it = 0; ok && it < n_mine; ++it) {
+        tmem_wait_ld();
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[0]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[32]));
+        ok = softmax_half(ra, 0, it);
+        if (!ok) break;
+        const bool early1 = try_fetch_s(rb, 1, j);
+        publish_p(ra, 0);
+        if (!early1) ok = fetch_s(rb, 1, j);
+        if (!ok) break;
+        tmem_wait_ld();
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&rb[0]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&rb[32]));
+        ok = softmax_half(rb, 1, it);
+        if (!ok) break;
+        const bool more = it + 1 < n_mine;
+        const bool early0 = more && try_fetch_s(ra, 0, j + 1);
+        publish_p(rb, 1);
+        ++j;
+        if (more && !early0) ok = fetch_s(ra, 0, j);
+      }
+      if (!ok) break;
+
+      // ---- O leaves TMEM first: the next piece's first P V may overwrite it while the rows are stored
+      if (n_mine > 0) {
+        ok = wait(bars->o_full[t][1], (j - 1) & 1, kTileWaitO);
+        if (!ok) break;
+        tc_fence_after_sync();
+        tmem_ld32(o_addr, *reinterpret_cast<uint32_t(*)[32]>(&ra[0]));
+        tmem_ld32(o_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&ra[32]));
+        tmem_ld32(o_addr + 64, *reinterpret_cast<uint32_t(*)[32]>(&rb[0]));
+        tmem_ld32(o_addr + 96, *reinterpret_cast<uint32_t(*)[32]>(&rb[32]));
+        tmem_wait_ld();
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[0]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[32]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&rb[0]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&rb[32]));
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->o_free[t]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) ra[i] = rb[i] = 0u;
+      }
+      const int head = p.h * a.group + row % a.group;
+      // rare: values that the helpers left out are added to the stored row, for the rows that see them
+      auto put_back = [&](auto* dst) {
+        const int end = min(lim, p.t1 * kKeyTile);
+        for (int key = max(tp.lim_min & ~(kKeyTile - 1), p.t0 * kKeyTile); key < end; ++key)
+          for (int d = 0; d < kCacheDim; ++d) {
+            const float v = v_value<kFp8>(a, p.b, p.h, key, d);
+            if (!isfinite(v)) dst[d] = static_cast<float>(dst[d]) + v;
+          }
+      };
+      const bool poisoned = bars->poison != 0u;
+      if (p.first && p.last) {
+        if (have_row) {
+          const float inv = l_sum == 0.f ? 0.f : 1.0f / l_sum;
+          __nv_bfloat16* dst = a.o + (p.s.s0 + token) * a.o_stride_l + head * a.o_stride_h;
+#pragma unroll
+          for (int x = 0; x < 128; x += 8) {
+            const uint32_t* o = x < 64 ? &ra[x] : &rb[x - 64];
+            uint4 w;
+            w.x = pack_bf16x2(__uint_as_float(o[0]) * inv, __uint_as_float(o[1]) * inv);
+            w.y = pack_bf16x2(__uint_as_float(o[2]) * inv, __uint_as_float(o[3]) * inv);
+            w.z = pack_bf16x2(__uint_as_float(o[4]) * inv, __uint_as_float(o[5]) * inv);
+            w.w = pack_bf16x2(__uint_as_float(o[6]) * inv, __uint_as_float(o[7]) * inv);
+            *reinterpret_cast<uint4*>(dst + x) = w;
+          }
+          if (poisoned) put_back(dst);
+          if (a.lse)
+            a.lse[static_cast<long long>(head) * a.c.rows + p.s.s0 + token] = l_sum == 0.f ? -INFINITY : (m_ref + log2f(l_sum)) * 0.6931471805599453f;
+        }
+      } else {
+        if (have_row) {
+          float* part = part_slot(a, blockIdx.x, p.first);
+          const int r = t * T * a.group + row;
+#pragma unroll
+          for (int x = 0; x < 128; x += 4) {
+            const uint32_t* o = x < 64 ? &ra[x] : &rb[x - 64];
+            *reinterpret_cast<uint4*>(part + r * kCacheDim + x) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+          if (poisoned) put_back(part + r * kCacheDim);
+          part[kTileRows * kCacheDim + r] = m_ref;
+          part[kTileRows * kCacheDim + kTileRows + r] = l_sum;
+        }
+        if (threadIdx.x == 0 && p.first) {  // the item goes on in later shares: say where it ends
+          const long long item_end = iter.item_base + 1 + item_tiles(a, p.s, p.it);
+          const int last = static_cast<int>((item_end * iter.n_shares + iter.total - 1) / iter.total) - 1;
+          *reinterpret_cast<int4*>(a.desc + 4 * blockIdx.x) = make_int4(p.b, p.h, p.it, last);
+        }
+      }
+    }
+  }
+
+  // ---- tear-down
+  tc_fence_before_sync();
+  __syncthreads();
+  if (bars->abort_flag) {  // a wait gave up: give copies and MMAs in flight a bounded time to land
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 9) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace h3a

@@ -10,6 +10,7 @@
 #include <mutex>
 
 #include "cache_attn.cuh"
+#include "cache_attn_tile.cuh"
 
 namespace {
 
@@ -115,6 +116,38 @@ int32_t move_rows(bool write, const h3a_cache* c, const h3a_cache_batch* b, void
   return cudaGetLastError() == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// x[..., row of 128]: outer dimensions with strides in bytes; a box of 128 bytes of a row, 128-byte swizzle
+int32_t row_map(CUtensorMap* m, const void* ptr, bool codes, int n_outer, const int64_t* sizes, const int64_t* strides, const int* box_outer) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return H3A_ERR_DRIVER;
+  cuuint64_t dims[4] = {128}, str[3];
+  cuuint32_t box[4] = {codes ? 128u : 64u}, step[4] = {1, 1, 1, 1};
+  for (int i = 0; i < n_outer; ++i) {
+    dims[i + 1] = static_cast<cuuint64_t>(sizes[i]);
+    str[i] = static_cast<cuuint64_t>(strides[i]);
+    box[i + 1] = static_cast<cuuint32_t>(box_outer[i]);
+  }
+  return enc(m, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, n_outer + 1, const_cast<void*>(ptr), dims, str, box,
+             step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? H3A_OK : H3A_ERR_LAUNCH;
+}
+
+constexpr int kTileMinShare = 4;
 constexpr int kFewMinShare = 3;  // units (a tile, or an item's set-up) below which a share is not worth a CTA
 
 // What a call of this shape launches.
@@ -124,7 +157,15 @@ struct AttnPlan {
 };
 AttnPlan attn_plan(const h3a_cache_attn_params* p, int sms) {
   AttnPlan n;
-  n.item_rows = h3a::kFewRows;
+  const int group = p->heads / p->cache.heads;
+  // query rows per K/V head of an average sequence: the lengths themselves are known on the device only
+  const int64_t rows = (static_cast<int64_t>(p->batch.rows) + p->batch.n_seqs - 1) / p->batch.n_seqs * group;
+  if (rows > h3a::kFewRows && group <= 128) {
+    n.item_rows = h3a::kTileRows;
+    n.item_tokens = 2 * (128 / group);
+  } else {
+    n.item_rows = h3a::kFewRows;
+  }
   n.shares = sms;
   n.bytes = static_cast<size_t>(n.shares) * (4 * sizeof(int) + 2ull * n.item_rows * (h3a::kCacheDim + 2) * sizeof(float));
   return n;
@@ -143,6 +184,36 @@ int32_t launch_few(const h3a::CacheAttnArgs& a, int shares, const Device& dev, c
   const int32_t rc = allow_smem(h3a::cache_attn_few_kernel<kFp8>, h3a::kFewSmemBytes, dev.id, once, err);
   if (rc != H3A_OK) return rc;
   h3a::cache_attn_few_kernel<kFp8><<<shares, h3a::kFewThreads, h3a::kFewSmemBytes, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
+}
+
+template <bool kFp8>
+int32_t launch_tile(const h3a_cache_attn_params* p, const h3a::CacheAttnArgs& a, int shares, const Device& dev, cudaStream_t st) {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t err[kMaxDevices];
+  std::call_once(once[dev.id], [&] {
+    cudaError_t e = cudaFuncSetAttribute(h3a::cache_attn_tile_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, h3a::kTileSmemBytes);
+    // the in-kernel register re-allocation would block forever if the launch allocation were smaller
+    cudaFuncAttributes fa;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, h3a::cache_attn_tile_kernel<kFp8>);
+    if (e == cudaSuccess && fa.numRegs < h3a::kTileLaunchRegs) e = cudaErrorLaunchOutOfResources;
+    err[dev.id] = e;
+  });
+  if (err[dev.id] != cudaSuccess) return H3A_ERR_LAUNCH;
+  CUtensorMap mq, mk, mv;
+  const h3a_cache& c = p->cache;
+  const int box_rows = std::min(128, c.page_size & -c.page_size);
+  const int64_t q_sizes[2] = {p->heads, p->batch.rows}, q_strides[2] = {a.q_head_bytes, a.q_row_bytes};
+  const int q_box[2] = {a.group, a.item_tokens / 2};
+  int32_t rc = row_map(&mq, p->q, false, 2, q_sizes, q_strides, q_box);
+  const int64_t sizes[3] = {c.page_size, c.heads, c.n_pages};
+  const int box[3] = {box_rows, 1, 1};
+  for (int x = 0; x < 2 && rc == H3A_OK; ++x) {
+    const int64_t strides[3] = {a.c.token_bytes[x], a.c.head_bytes[x], a.c.page_bytes[x]};
+    rc = row_map(x ? &mv : &mk, x ? c.v : c.k, kFp8, 3, sizes, strides, box);
+  }
+  if (rc != H3A_OK) return rc;
+  h3a::cache_attn_tile_kernel<kFp8><<<shares, h3a::kTileThreads, h3a::kTileSmemBytes, st>>>(mq, mk, mv, box_rows, a);
   return cudaGetLastError() == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
 }
 
@@ -215,10 +286,13 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   a.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / std::sqrt(128.0f)) * 1.4426950408889634f;
   a.desc = static_cast<int*>(p->workspace);
   a.part = reinterpret_cast<float*>(a.desc + 4 * n.shares);
-  a.min_share = kFewMinShare;
+  a.min_share = n.item_tokens > 0 ? kTileMinShare : kFewMinShare;
   a.wait_ns = p->wait_limit_ns > 0 ? p->wait_limit_ns : 2000000000ll;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  rc = p->cache.quantised ? launch_few<true>(a, n.shares, dev, st) : launch_few<false>(a, n.shares, dev, st);
+  if (n.item_tokens > 0)
+    rc = p->cache.quantised ? launch_tile<true>(p, a, n.shares, dev, st) : launch_tile<false>(p, a, n.shares, dev, st);
+  else
+    rc = p->cache.quantised ? launch_few<true>(a, n.shares, dev, st) : launch_few<false>(a, n.shares, dev, st);
   return rc == H3A_OK ? launch_join(a, n.shares, st) : rc;
 }
 
