@@ -6,6 +6,9 @@
 //                    P written back over S as packed bf16, lazy rescale of O (when the maximum grows by more than 2^8)
 //   warp 8           producer: TMA loads of Q and of the K and V tiles, page by page, into a ring
 //   warps 9, 10      issuers, one per stream: S = Q K^T (N = 64 keys), O += P V (P from TMEM), tcgen05.commit
+//   warp 11          cuts the share into pieces and hands them to the others through a small ring: the bookkeeping would
+//                    cost every role some 40 registers (with each role walking the share on its own the softmax warps
+//                    spilled 1.4 KB and the kernel ran at half the speed)
 //   warps 12-15      helpers, one cache row per thread.  e4m3: widen a staged tile to bf16 (exact, the row's power of two
 //                    included) into the ring.  bf16: let tiles through, except the V tiles that not every row sees whole:
 //                    P is 0 for a key a row does not see, and 0 x NaN is NaN, so rows behind the last key become zeros
@@ -22,7 +25,7 @@
 namespace h3a {
 
 constexpr int kTileThreads = 512;
-constexpr int kTileSoftmaxRegs = 192, kTileOtherRegs = 64, kTileLaunchRegs = 128;
+constexpr int kTileSoftmaxRegs = 200, kTileOtherRegs = 56, kTileLaunchRegs = 128;
 static_assert(256 * kTileSoftmaxRegs + 256 * kTileOtherRegs <= kTileLaunchRegs * kTileThreads, "setmaxnreg budget exceeds the launch allocation");
 constexpr int kTileRows = 256;         // rows of an item
 constexpr int kTileBytes = 32768;      // 128 rows of 128 bf16
@@ -44,6 +47,7 @@ struct TileBars {
   uint64_t q_full, q_empty;
   uint64_t s_full[2][2], p_full[2][2], o_full[2][2];  // [stream][half]
   uint64_t o_free[2];
+  uint64_t piece_full[4], piece_empty[4];
   uint32_t tmem_base;
   uint32_t early_exit;
   volatile uint32_t abort_flag;
@@ -51,11 +55,9 @@ struct TileBars {
 };
 constexpr int kTileSmemBytes = 2 * kTileBytes + TileRing<false>::kBytes + 1024 + 512;
 static_assert(TileRing<true>::kBytes <= TileRing<false>::kBytes && sizeof(TileBars) <= 512, "shared memory layout");
-static_assert(kTileSmemBytes + sizeof(ShareStart) <= 232448, "shared memory budget");
-
 enum : int {  // status codes of waits that ran out (low byte of the status word)
   kTileWaitEmpty = 33, kTileWaitFull, kTileWaitReady, kTileWaitUnstaged, kTileWaitStaged, kTileWaitQFull, kTileWaitQEmpty,
-  kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree
+  kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitPiece
 };
 
 struct TileWait {
@@ -94,25 +96,75 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, 
       : "memory");
 }
 
-// What every role derives from a piece in the same way.
+// 16 columns at a time: for the rescale path, which runs with both register images of S alive
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void reg_fence16(uint32_t (&r)[16]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+// A piece as the roles see it.
 struct TilePiece {
-  int tok0;        // first token of stream 0
-  int n_tiles;
-  int end[2];      // key tiles of the piece that the stream takes part in: [0, end)
-  int lim_min, lim_max;
-  __device__ __forceinline__ TilePiece(const CacheAttnArgs& a, const Piece& p) {
-    const int T = a.item_tokens >> 1;
-    tok0 = p.it * a.item_tokens;
-    n_tiles = p.t1 - p.t0;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int first = tok0 + t * T, last = min(p.s.n, first + T) - 1;
-      end[t] = last >= first ? max(0, min(p.t1, (key_limit(a, p.s, last) + kKeyTile - 1) / kKeyTile) - p.t0) : 0;
-    }
-    lim_min = key_limit(a, p.s, tok0);
-    lim_max = key_limit(a, p.s, item_last_token(a, p.s, p.it));
-  }
+  int n_tiles;       // key tiles [t0, t0 + n_tiles)
+  int t0;
+  int end[2];        // the stream takes part in the first `end` of them
+  int lim_min, lim_max;  // keys that the item's first and last row see
+  int b, h;
+  int row0;          // packed row of the item's first token
+  int tok0, n, len;  // its number in the sequence; new rows and length of the sequence
+  int whole;         // the piece is the whole item; otherwise its results are partial
+  int tail;          // ... and go to the share's tail slot (the item begins here)
+  int it, last_share;
 };
+constexpr int kPieceRing = 4;
+constexpr int kPieceReaders = 15;  // warps
+
+__device__ __forceinline__ int piece_limit(const CacheAttnArgs& a, const TilePiece& q, int token) {
+  return a.causal ? max(0, min(q.len, q.len - q.n + token + 1)) : q.len;
+}
+__device__ __forceinline__ void describe_piece(const CacheAttnArgs& a, const ShareIter& iter, const Piece& p, TilePiece& q) {
+  const int T = a.item_tokens >> 1;
+  q.tok0 = p.it * a.item_tokens;
+  q.n_tiles = p.t1 - p.t0;
+  q.t0 = p.t0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = q.tok0 + t * T, last = min(p.s.n, first + T) - 1;
+    q.end[t] = last >= first ? max(0, min(p.t1, (key_limit(a, p.s, last) + kKeyTile - 1) / kKeyTile) - p.t0) : 0;
+  }
+  q.lim_min = key_limit(a, p.s, q.tok0);
+  q.lim_max = key_limit(a, p.s, item_last_token(a, p.s, p.it));
+  q.b = p.b;
+  q.h = p.h;
+  q.row0 = p.s.s0 + q.tok0;
+  q.n = p.s.n;
+  q.len = p.s.len;
+  q.whole = p.first && p.last;
+  q.tail = p.first;
+  q.it = p.it;
+  q.last_share = -1;
+  if (p.first && !p.last) {  // the item goes on in later shares: where it ends
+    const long long item_end = iter.item_base + 1 + item_tiles(a, p.s, p.it);
+    q.last_share = static_cast<int>((item_end * iter.n_shares + iter.total - 1) / iter.total) - 1;
+  }
+}
 
 // rows [0, box_rows) of a 4-D page box are whole keys of one page: box_rows divides the page size and the tile
 template <bool kFp8>
@@ -121,6 +173,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                        const __grid_constant__ CUtensorMap tm_v, const int box_rows, const __grid_constant__ CacheAttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ ShareStart start;
+  __shared__ TilePiece pieces[kPieceRing];  // n_tiles < 0: no more
+  static_assert(kTileSmemBytes + sizeof(ShareStart) + sizeof(TilePiece) * kPieceRing <= 232448, "shared memory budget");
   using R = TileRing<kFp8>;
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -149,6 +203,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       mbar_init(smem_u32(&bars->o_free[t]), 4);
     }
+    for (int i = 0; i < kPieceRing; ++i) {
+      mbar_init(smem_u32(&bars->piece_full[i]), 1);
+      mbar_init(smem_u32(&bars->piece_empty[i]), kPieceReaders);
+    }
     bars->abort_flag = 0;
     bars->poison = 0;
     bars->early_exit = (a.c.status != nullptr && *reinterpret_cast<volatile int*>(a.c.status) != 0) ? 1u : 0u;
@@ -172,7 +230,18 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const uint32_t tmem = bars->tmem_base;
   const TileWait wait{a, bars};
   const int T = a.item_tokens >> 1;
-  Piece p;
+  // the readers' side of the ring of pieces
+  uint32_t n_pieces = 0;
+  auto piece = [&]() -> const TilePiece* {
+    const uint32_t i = n_pieces % kPieceRing;
+    if (!wait(bars->piece_full[i], (n_pieces / kPieceRing) & 1, kTileWaitPiece) || pieces[i].n_tiles < 0) return nullptr;
+    return &pieces[i];
+  };
+  auto piece_done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&bars->piece_empty[n_pieces % kPieceRing]));
+    ++n_pieces;
+  };
 
   if (warp >= 12) {
     // =========================================================== helpers: thread r owns row r of every tile
@@ -181,25 +250,26 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const uint32_t swz = row & 7;
     int cnt = 0;
     bool ok = true;
-    while (ok && iter.next(a, p)) {
-      const TilePiece tp(a, p);
-      if (tp.n_tiles == 0) continue;
+    const TilePiece* q;
+    for (; ok && (q = piece()) != nullptr; piece_done()) {
+      const int n_tiles = q->n_tiles, t0 = q->t0, b = q->b, h = q->h, lim_min = q->lim_min, lim_max = q->lim_max;
+      if (n_tiles == 0) continue;
       uint32_t ex[2] = {0, 0};  // e4m3: exponent bytes of this thread's row of the tile to come
       auto fetch_ex = [&](int tile) {
         const int key = tile * kKeyTile + row;
-        if (kFp8 && key < tp.lim_max) {
+        if (kFp8 && key < lim_max) {
           const int slot = key / a.c.page_size, at = key - slot * a.c.page_size;
-          const long long id = checked_page(a, p.b, slot);
+          const long long id = checked_page(a, b, slot);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) ex[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + p.h * a.c.exp_head[x]);
+          for (int x = 0; x < 2; ++x) ex[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + h * a.c.exp_head[x]);
         }
       };
-      fetch_ex(p.t0);
-      for (int it = 0; ok && it < tp.n_tiles; ++it) {
-        const int tile = p.t0 + it, key = tile * kKeyTile + row;
-        const bool special = (tile + 1) * kKeyTile > tp.lim_min;
+      fetch_ex(t0);
+      for (int it = 0; ok && it < n_tiles; ++it) {
+        const int tile = t0 + it, key = tile * kKeyTile + row;
+        const bool special = (tile + 1) * kKeyTile > lim_min;
         const uint32_t e_now[2] = {ex[0], ex[1]};
-        if (it + 1 < tp.n_tiles) fetch_ex(tile + 1);
+        if (it + 1 < n_tiles) fetch_ex(tile + 1);
 #pragma unroll
         for (int x = 0; x < 2; ++x, ++cnt) {  // K, then V
           const int s = cnt % R::kRing;
@@ -212,7 +282,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const uint32_t src = staging + g * kCodeBytes + row * 128;
             uint32_t f = e4m3_factor(e_now[x]) * 0x10001u;
             const uint32_t f2 = e4m3_factor2(e_now[x]) * 0x10001u;
-            if (key >= tp.lim_max) {
+            if (key >= lim_max) {
               f = 0;
             } else if (x == 1 && special && e_now[x] == 255u) {
               f = 0;
@@ -248,7 +318,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             ok = wait(bars->full[s], ph, kTileWaitFull);
             if (!ok) break;
             if (x == 1 && special) {
-              const bool gone = key >= tp.lim_max;
+              const bool gone = key >= lim_max;
               bool bad = false;
 #pragma unroll 4
               for (int c = 0; c < 16; ++c) {
@@ -282,20 +352,21 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       int cnt = 0;
       uint32_t g = 0;  // pieces with work so far: the phase of q_full / q_empty
       bool ok = true;
-      while (ok && iter.next(a, p)) {
-        const TilePiece tp(a, p);
-        if (tp.n_tiles == 0) continue;
+      const TilePiece* q;
+      for (; ok && (q = piece()) != nullptr; piece_done()) {
+        const int n_tiles = q->n_tiles, t0 = q->t0, b = q->b, h = q->h, lim_max = q->lim_max;
+        if (n_tiles == 0) continue;
         // Q is free late in the previous piece, ring slots earlier: the first two key tiles go ahead of Q
-        const int q_at = g > 0 ? min(2, tp.n_tiles - 1) : 0;
+        const int q_at = g > 0 ? min(2, n_tiles - 1) : 0;
         bool q_loaded = false;
         // page and place of this lane's sub-box of a tile; none behind the last key
         int id = -1;
         auto fetch_page = [&](int tile) {
           const int key = tile * kKeyTile + lane * box_rows;
-          id = lane < n_boxes && key < tp.lim_max ? checked_page(a, p.b, key / a.c.page_size) : -1;
+          id = lane < n_boxes && key < lim_max ? checked_page(a, b, key / a.c.page_size) : -1;
         };
-        fetch_page(p.t0);
-        for (int it = 0; ok && it < tp.n_tiles; ++it) {
+        fetch_page(t0);
+        for (int it = 0; ok && it < n_tiles; ++it) {
           if (!q_loaded) {
             bool q_free = g == 0 || __all_sync(0xFFFFFFFFu, mbar_test_wait(smem_u32(&bars->q_empty), (g - 1) & 1));
             if (!q_free && it >= q_at) {
@@ -306,20 +377,20 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (q_free) {
               if (lane == 0) {
                 const uint32_t bar = smem_u32(&bars->q_full);
-                const bool second = tp.tok0 + T < p.s.n;
+                const bool second = q->tok0 + T < q->n;
                 mbar_arrive_expect_tx(bar, second ? 2 * q_bytes : q_bytes);
                 for (int t = 0; t < (second ? 2 : 1); ++t)
                   for (int hf = 0; hf < 2; ++hf)
-                    tma_load_3d(q_smem + t * kTileBytes + hf * kTileHalf, &tm_q, bar, 64 * hf, p.h * a.group, p.s.s0 + tp.tok0 + t * T);
+                    tma_load_3d(q_smem + t * kTileBytes + hf * kTileHalf, &tm_q, bar, 64 * hf, h * a.group, q->row0 + t * T);
               }
               __syncwarp();
               q_loaded = true;
             }
           }
-          const int tile = p.t0 + it;
+          const int tile = t0 + it;
           const int now = id, at = (tile * kKeyTile + lane * box_rows) % a.c.page_size;
           const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, now >= 0)) * box_bytes;
-          if (it + 1 < tp.n_tiles) fetch_page(tile + 1);
+          if (it + 1 < n_tiles) fetch_page(tile + 1);
 #pragma unroll
           for (int x = 0; x < 2; ++x, ++cnt) {
             const CUtensorMap* tm = x ? &tm_v : &tm_k;
@@ -339,8 +410,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
             __syncwarp();
             if (now >= 0) {
-              tma_load_4d(dst, tm, bar, 0, at, p.h, now);
-              if constexpr (!kFp8) tma_load_4d(dst + kTileHalf, tm, bar, 64, at, p.h, now);
+              tma_load_4d(dst, tm, bar, 0, at, h, now);
+              if constexpr (!kFp8) tma_load_4d(dst + kTileHalf, tm, bar, 64, at, h, now);
             }
             __syncwarp();
           }
@@ -385,10 +456,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         tc_fence_after_sync();
         return got;
       };
-      while (ok && iter.next(a, p)) {
-        const TilePiece tp(a, p);
-        if (tp.n_tiles == 0) continue;
-        const int n_mine = tp.end[t];
+      const TilePiece* q;
+      for (; ok && (q = piece()) != nullptr; piece_done()) {
+        const int n_tiles = q->n_tiles, n_mine = q->end[t];
+        if (n_tiles == 0) continue;
         ok = wait(bars->q_full, g & 1, kTileWaitQFull) && ready(c0);
         if (!ok) break;
         pv_cnt = 0;
@@ -397,8 +468,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           issue_s(1, c0 % R::kRing);
         }
         umma_commit_if(leader, smem_u32(&bars->empty[c0 % R::kRing]));
-        for (int it = 0; ok && it < tp.n_tiles; ++it) {
-          const bool has_next = it + 1 < tp.n_tiles;
+        for (int it = 0; ok && it < n_tiles; ++it) {
+          const bool has_next = it + 1 < n_tiles;
           const int cv = c0 + 2 * it + 1, ck = cv + 1;
           if (!has_next) umma_commit_if(leader, smem_u32(&bars->q_empty));  // every S MMA of the piece has been issued
           ok = ready(cv);
@@ -426,9 +497,21 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           umma_commit_if(leader, smem_u32(&bars->empty[cv % R::kRing]));
           if (has_next) umma_commit_if(leader, smem_u32(&bars->empty[ck % R::kRing]));
         }
-        c0 += 2 * tp.n_tiles;
+        c0 += 2 * n_tiles;
         ++g;
         if (n_mine > 0) ++own;
+      }
+    } else if (lane == 0) {
+      // ========================================================= the share's pieces, one after the other
+      Piece p;
+      for (uint32_t n = 0;; ++n) {
+        const uint32_t i = n % kPieceRing;
+        const bool more = iter.next(a, p);
+        if (!wait.one(bars->piece_empty[i], ((n / kPieceRing) & 1) ^ 1u, kTileWaitPiece)) break;
+        if (more) describe_piece(a, iter, p, pieces[i]);
+        else pieces[i].n_tiles = -1;
+        mbar_arrive(smem_u32(&bars->piece_full[i]));
+        if (!more) break;
       }
     }
     __syncwarp();
@@ -463,18 +546,17 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       tc_fence_before_sync();
       mbar_arrive(smem_u32(&bars->p_full[t][hf]));
     };
-    while (ok && iter.next(a, p)) {
-      const TilePiece tp(a, p);
-      const int n_mine = tp.end[t];
-      const int first = tp.tok0 + t * T;
-      const int token = first + row / a.group;  // row r: token r / group, head r % group
-      const bool have_row = row < T * a.group && token < p.s.n;
-      const int lim = have_row ? key_limit(a, p.s, token) : 0;
-      const int lim_first = key_limit(a, p.s, first);  // the stream's first row sees fewest keys
+    const int row_token = t * T + row / a.group, row_head = row % a.group;  // row r: token r / group, head r % group
+    const TilePiece* q;
+    for (; ok && (q = piece()) != nullptr; piece_done()) {
+      const int n_mine = q->end[t];
+      const bool have_row = row < T * a.group && q->tok0 + row_token < q->n;
+      const int lim = (have_row ? piece_limit(a, *q, q->tok0 + row_token) : 0) - q->t0 * kKeyTile;  // counted from tile t0
+      const int lim_first = piece_limit(a, *q, q->tok0 + t * T) - q->t0 * kKeyTile;  // the stream's first row sees fewest keys
       float m_ref = kNoMax, l_sum = 0.f;
 
       auto softmax_half = [&](uint32_t (&s)[64], int hf, int it) -> bool {
-        const int key0 = (p.t0 + it) * kKeyTile + hf * 64;
+        const int key0 = it * kKeyTile + hf * 64;
         if (key0 + 64 > lim_first) {
           const int valid = lim - key0;
 #pragma unroll
@@ -506,14 +588,14 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (!wait(bars->o_full[t][hf ^ 1], (hf ? j : j - 1) & 1, kTileWaitO)) return false;
           tc_fence_after_sync();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + 32 * i, o);
+          for (int i = 0; i < 8; ++i) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + 16 * i, o);
             tmem_wait_ld();
-            reg_fence32(o);
+            reg_fence16(o);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-            tmem_st32(o_addr + 32 * i, o);
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+            tmem_st16(o_addr + 16 * i, o);
           }
         }
         // P = 2^(s c - m), rounded to bf16 once; the row sum keeps the unrounded terms
@@ -580,21 +662,22 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll
         for (int i = 0; i < 64; ++i) ra[i] = rb[i] = 0u;
       }
-      const int head = p.h * a.group + row % a.group;
+      const int head = q->h * a.group + row_head;
+      const long long out_row = q->row0 + row_token;
       // rare: values that the helpers left out are added to the stored row, for the rows that see them
       auto put_back = [&](auto* dst) {
-        const int end = min(lim, p.t1 * kKeyTile);
-        for (int key = max(tp.lim_min & ~(kKeyTile - 1), p.t0 * kKeyTile); key < end; ++key)
+        const int end = q->t0 * kKeyTile + min(lim, q->n_tiles * kKeyTile);
+        for (int key = max(q->lim_min & ~(kKeyTile - 1), q->t0 * kKeyTile); key < end; ++key)
           for (int d = 0; d < kCacheDim; ++d) {
-            const float v = v_value<kFp8>(a, p.b, p.h, key, d);
+            const float v = v_value<kFp8>(a, q->b, q->h, key, d);
             if (!isfinite(v)) dst[d] = static_cast<float>(dst[d]) + v;
           }
       };
       const bool poisoned = bars->poison != 0u;
-      if (p.first && p.last) {
+      if (q->whole) {
         if (have_row) {
           const float inv = l_sum == 0.f ? 0.f : 1.0f / l_sum;
-          __nv_bfloat16* dst = a.o + (p.s.s0 + token) * a.o_stride_l + head * a.o_stride_h;
+          __nv_bfloat16* dst = a.o + out_row * a.o_stride_l + head * a.o_stride_h;
 #pragma unroll
           for (int x = 0; x < 128; x += 8) {
             const uint32_t* o = x < 64 ? &ra[x] : &rb[x - 64];
@@ -607,11 +690,11 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           }
           if (poisoned) put_back(dst);
           if (a.lse)
-            a.lse[static_cast<long long>(head) * a.c.rows + p.s.s0 + token] = l_sum == 0.f ? -INFINITY : (m_ref + log2f(l_sum)) * 0.6931471805599453f;
+            a.lse[static_cast<long long>(head) * a.c.rows + out_row] = l_sum == 0.f ? -INFINITY : (m_ref + log2f(l_sum)) * 0.6931471805599453f;
         }
       } else {
         if (have_row) {
-          float* part = part_slot(a, blockIdx.x, p.first);
+          float* part = part_slot(a, blockIdx.x, q->tail != 0);
           const int r = t * T * a.group + row;
 #pragma unroll
           for (int x = 0; x < 128; x += 4) {
@@ -622,11 +705,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           part[kTileRows * kCacheDim + r] = m_ref;
           part[kTileRows * kCacheDim + kTileRows + r] = l_sum;
         }
-        if (threadIdx.x == 0 && p.first) {  // the item goes on in later shares: say where it ends
-          const long long item_end = iter.item_base + 1 + item_tiles(a, p.s, p.it);
-          const int last = static_cast<int>((item_end * iter.n_shares + iter.total - 1) / iter.total) - 1;
-          *reinterpret_cast<int4*>(a.desc + 4 * blockIdx.x) = make_int4(p.b, p.h, p.it, last);
-        }
+        if (threadIdx.x == 0 && q->last_share >= 0)  // the item goes on in later shares: say where it ends
+          *reinterpret_cast<int4*>(a.desc + 4 * blockIdx.x) = make_int4(q->b, q->h, q->it, q->last_share);
       }
     }
   }
