@@ -109,122 +109,161 @@ __device__ __forceinline__ int sequence_of_row(const CacheArgs& a, int t) {
   return (__ldg(a.starts + lo) <= t && t < __ldg(a.starts + lo + 1)) ? lo : -1;
 }
 
-// Where one (row, K or V, head) unit lives: offset of its cached row and of its exponent byte.
+// Where a row lives: its sequence's page and the place in it.
 struct RowPlace {
-  long long cached, exp;
-  int state;  // 0: not a row of any sequence, or refused (leave everything alone); 1: no position in the cache; 2: fine
+  int id, at;
+  int state;  // 0: not a row of any sequence (leave everything alone); 1: no position in the cache, or refused; 2: fine
 };
-__device__ __forceinline__ RowPlace place_of_row(const CacheArgs& a, int t, int x, int h) {
-  RowPlace p;
-  p.cached = p.exp = 0;
-  p.state = 0;
+__device__ __forceinline__ RowPlace place_of_row(const CacheArgs& a, int t) {
+  RowPlace p{0, 0, 0};
   const int b = sequence_of_row(a, t);
   if (b < 0) return p;
+  p.state = 1;
   const CacheSeq q = cache_seq(a, b);
   const int pos = q.len - q.n + (t - q.s0);
-  if (pos < 0) {
-    p.state = 1;
-    return p;
-  }
-  const int slot = pos / a.page_size, at = pos - slot * a.page_size;
-  const int id = __ldg(a.pages + b * a.pages_stride + slot);
-  if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.n_pages)) {
+  if (pos < 0) return p;
+  const int slot = pos / a.page_size;
+  p.at = pos - slot * a.page_size;
+  p.id = __ldg(a.pages + b * a.pages_stride + slot);
+  if (static_cast<unsigned>(p.id) >= static_cast<unsigned>(a.n_pages)) {
     report_cache(a, b);
-    p.state = 1;
     return p;
   }
-  p.cached = id * a.page_bytes[x] + at * a.token_bytes[x] + h * a.head_bytes[x];
-  p.exp = id * a.exp_page[x] + at * a.exp_token[x] + h * a.exp_head[x];
   p.state = 2;
   return p;
 }
 
 constexpr int kRowThreads = 256;
-constexpr int kRowUnroll = 4;  // units a half-warp has in flight: 4 x 256 B
+constexpr int kRowGroups = kRowThreads / 16;  // half-warps of a block
 
-// A half-warp owns one row (16 lanes x 16 B) of one head of K or V; consecutive half-warps take consecutive heads, which
-// lie next to each other in the packed rows.  kWrite: packed -> cache; otherwise cache -> packed.
+// A half-warp moves rows of 128 values, 16 lanes x 8 values each: all heads of K and V of one token, or, when there are few
+// tokens, every `per_token`-th of them (per_token half-warps and gridDim.y blocks share a token).  The token's place is
+// looked up once; inside the loop an address is one multiplication away.  kUnroll rows are in flight per half-warp.
+// Looking every (token, head) row up by itself, with a division and a search each, took three times as long (clip of
+// 49,384 x 40 heads into e4m3: 688 us).  kWrite: packed -> cache; otherwise cache -> packed.
 template <bool kWrite, bool kQuantised>
-__global__ void __launch_bounds__(kRowThreads) cache_rows_kernel(const RowsArgs a) {
+constexpr int kUnroll = kWrite && kQuantised ? 4 : 8;  // quantising wants registers for more warps: 301 against 314 us; reading 247 against 256
+constexpr int kExpRows = 256;  // rows of a token between two meetings of the exponent bytes
+template <bool kWrite, bool kQuantised>
+__global__ void __launch_bounds__(kRowThreads) cache_rows_kernel(const __grid_constant__ RowsArgs a, const int per_token) {
   if (a.c.status && *reinterpret_cast<volatile int*>(a.c.status) != 0) return;
-  const int lane = threadIdx.x & 15;
+  constexpr int kRowUnroll = kUnroll<kWrite, kQuantised>;
+  const int lane = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const uint32_t half_mask = (threadIdx.x & 16) ? 0xFFFF0000u : 0x0000FFFFu;
-  const uint32_t per_row = 2u * a.c.kv_heads;
-  const uint32_t n_units = a.c.rows * per_row;  // below 2^31: checked by the host
-  const uint32_t step = gridDim.x * (kRowThreads / 16);
-  for (uint32_t u0 = blockIdx.x * (kRowThreads / 16) + (threadIdx.x >> 4); u0 < n_units; u0 += step * kRowUnroll) {
-    RowPlace p[kRowUnroll];
-    uint4 r[kRowUnroll];
-    uint32_t e[kRowUnroll];
-    uint8_t* packed[kRowUnroll];
-    int x[kRowUnroll];
+  const int t = blockIdx.x * (kRowGroups / per_token) + grp / per_token;
+  RowPlace p{0, 0, 0};
+  if (t < a.c.rows) p = place_of_row(a.c, t);
+  const int step = per_token * gridDim.y, n_rows = 2 * a.c.kv_heads;
+  uint8_t* const cached0 = a.c.pool[0] + p.id * a.c.page_bytes[0] + p.at * a.c.token_bytes[0] + lane * (kQuantised ? 8 : 16);
+  uint8_t* const cached1 = a.c.pool[1] + p.id * a.c.page_bytes[1] + p.at * a.c.token_bytes[1] + lane * (kQuantised ? 8 : 16);
+  uint8_t* const exps0 = kQuantised ? a.c.exps[0] + p.id * a.c.exp_page[0] + p.at * a.c.exp_token[0] : nullptr;
+  uint8_t* const exps1 = kQuantised ? a.c.exps[1] + p.id * a.c.exp_page[1] + p.at * a.c.exp_token[1] : nullptr;
+  uint8_t* const packed0 = a.x[0] + t * a.row_bytes[0] + lane * 16;
+  uint8_t* const packed1 = a.x[1] + t * a.row_bytes[1] + lane * 16;
+  // row y of a token: head y of K, then head y - kv_heads of V
+  auto cached_row = [&](int y) { return y < a.c.kv_heads ? cached0 + y * a.c.head_bytes[0] : cached1 + (y - a.c.kv_heads) * a.c.head_bytes[1]; };
+  auto exp_of = [&](int y, uint8_t* e0, uint8_t* e1) { return y < a.c.kv_heads ? e0 + y * a.c.exp_head[0] : e1 + (y - a.c.kv_heads) * a.c.exp_head[1]; };
+  auto packed_row = [&](int y) { return y < a.c.kv_heads ? packed0 + y * a.head_bytes[0] : packed1 + (y - a.c.kv_heads) * a.head_bytes[1]; };
+  // Exponent bytes of a write meet in shared memory, so that the 16 tokens' bytes of a head leave in one store (they are
+  // neighbours in memory): a store per byte cost a fifth of the time.  With few tokens each lane stores its own.
+  const bool meet = kWrite && kQuantised && per_token == 1 && gridDim.y == 1;
+  __shared__ uint8_t exp_s[kWrite && kQuantised ? kExpRows : 1][kRowGroups];
+  __shared__ uint8_t* exp_at[kRowGroups][2];
+  if (meet) {
+    if (lane == 0) {
+      exp_at[grp][0] = p.state == 2 ? exps0 : nullptr;
+      exp_at[grp][1] = exps1;
+    }
+  } else if (p.state == 0 || (kWrite && p.state == 1)) {
+    return;
+  }
+  for (int c0 = 0; c0 < n_rows; c0 += kExpRows) {
+    const int c1 = min(n_rows, c0 + kExpRows);
+    for (int y0 = c0 + grp % per_token + per_token * blockIdx.y; y0 < c1; y0 += step * kRowUnroll) {
+      uint4 r[kRowUnroll];
+      uint32_t e[kRowUnroll];
 #pragma unroll
-    for (int i = 0; i < kRowUnroll; ++i) {
-      const uint32_t u = u0 + i * step;
-      p[i].state = 0;
-      x[i] = 0;
-      e[i] = 0;
-      r[i] = make_uint4(0, 0, 0, 0);
-      packed[i] = nullptr;
-      if (u < n_units) {
-        const int t = static_cast<int>(u / per_row);
-        const int y = static_cast<int>(u - t * per_row);
-        x[i] = y >= a.c.kv_heads;
-        const int h = y - x[i] * a.c.kv_heads;
-        p[i] = place_of_row(a.c, t, x[i], h);
-        packed[i] = a.x[x[i]] + t * a.row_bytes[x[i]] + h * a.head_bytes[x[i]] + lane * 16;
-        if (p[i].state == 2) {
-          if constexpr (kWrite) {
-            r[i] = ldg_stream(packed[i]);
-          } else if constexpr (kQuantised) {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(a.c.pool[x[i]] + p[i].cached + lane * 8));
-            r[i].x = w.x;
-            r[i].y = w.y;
-            e[i] = __ldg(a.c.exps[x[i]] + p[i].exp);
-          } else {
-            r[i] = ldg_stream(a.c.pool[x[i]] + p[i].cached + lane * 16);
+      for (int i = 0; i < kRowUnroll; ++i) {
+        const int y = y0 + i * step;
+        r[i] = make_uint4(0, 0, 0, 0);
+        e[i] = 127;
+        if (y >= c1 || p.state != 2) continue;
+        if constexpr (kWrite) {
+          r[i] = ldg_stream(packed_row(y));
+        } else if constexpr (kQuantised) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(cached_row(y)));
+          r[i].x = w.x;
+          r[i].y = w.y;
+          e[i] = __ldg(exp_of(y, exps0, exps1));
+        } else {
+          r[i] = ldg_stream(cached_row(y));
+        }
+      }
+      if constexpr (kWrite && kQuantised) {
+        // the largest magnitude by its bits (finite values order as integers, NaN and infinity lie above them), two rows
+        // in the halves of one word
+#pragma unroll
+        for (int i = 0; i < kRowUnroll; i += 2) {
+          uint32_t m[2];
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const uint4& w = r[i + z];
+            m[z] = __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
           }
+          uint32_t both = __vmaxu2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(half_mask, both, o));
+          e[i] = row_exponent(both & 0xFFFFu);
+          e[i + 1] = row_exponent(both >> 16);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kRowUnroll; ++i) {
+        const int y = y0 + i * step;
+        if (y >= c1 || p.state == 0 || (kWrite && p.state == 1)) break;  // the same for the whole half-warp
+        if constexpr (!kWrite) {
+          if constexpr (kQuantised) {
+            const uint32_t f = e4m3_factor(e[i]) * 0x10001u, w0 = r[i].x, w1 = r[i].y;
+            r[i].x = mul_bf16x2(e4m3_pattern(__byte_perm(w0, 0, 0x1404)), f);
+            r[i].y = mul_bf16x2(e4m3_pattern(__byte_perm(w0, 0, 0x3424)), f);
+            r[i].z = mul_bf16x2(e4m3_pattern(__byte_perm(w1, 0, 0x1404)), f);
+            r[i].w = mul_bf16x2(e4m3_pattern(__byte_perm(w1, 0, 0x3424)), f);
+            if (e[i] > kOneStepExp) {
+              const uint32_t f2 = e4m3_factor2(e[i]) * 0x10001u;
+              r[i] = make_uint4(mul_bf16x2(r[i].x, f2), mul_bf16x2(r[i].y, f2), mul_bf16x2(r[i].z, f2), mul_bf16x2(r[i].w, f2));
+            }
+          }
+          *reinterpret_cast<uint4*>(packed_row(y)) = r[i];
+        } else if constexpr (kQuantised) {
+          // 2^-k, exact in bf16 (what it takes below the type's smallest number is a zero in e4m3 anyway)
+          const uint32_t f = (254u - min(e[i], 247u)) * 0x800080u;
+          const uint32_t w[4] = {mul_bf16x2(r[i].x, f), mul_bf16x2(r[i].y, f), mul_bf16x2(r[i].z, f), mul_bf16x2(r[i].w, f)};
+          uint32_t c[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            float lo = __uint_as_float(w[z] << 16), hi = __uint_as_float(w[z] & 0xFFFF0000u);
+            if (e[i] == 247u) {  // the top of the range: a code of 256 would stand for 2^128, 240 is the last one that does not
+              lo = fminf(fmaxf(lo, -240.f), 240.f);
+              hi = fminf(fmaxf(hi, -240.f), 240.f);
+            }
+            c[z] = cvt_e4m3x2(lo, hi);
+          }
+          *reinterpret_cast<uint2*>(cached_row(y)) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+          if (lane == 0) {
+            if (meet) exp_s[y - c0][grp] = static_cast<uint8_t>(e[i]);
+            else *exp_of(y, exps0, exps1) = static_cast<uint8_t>(e[i]);
+          }
+        } else {
+          *reinterpret_cast<uint4*>(cached_row(y)) = r[i];
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < kRowUnroll; ++i) {
-      if constexpr (kWrite) {
-        if constexpr (kQuantised) {
-          // the largest magnitude by its bits: finite values order as integers, NaN and infinity lie above them
-          uint32_t m = __vmaxu2(__vmaxu2(r[i].x & 0x7FFF7FFFu, r[i].y & 0x7FFF7FFFu), __vmaxu2(r[i].z & 0x7FFF7FFFu, r[i].w & 0x7FFF7FFFu));
-          m = max(m >> 16, m & 0xFFFFu);
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(half_mask, m, o));
-          const uint32_t ex = row_exponent(m);
-          // 2^-k; at the top of the type's range a code of 256 would stand for 2^128: 240 is the last one that does not
-          const float f = __uint_as_float((254u - min(ex, 247u)) << 23);
-          const float cap = ex == 247u ? 240.0f : 448.0f;
-          const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-          uint32_t c[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float lo = __uint_as_float(w[y] << 16) * f, hi = __uint_as_float(w[y] & 0xFFFF0000u) * f;
-            c[y] = cvt_e4m3x2(fminf(fmaxf(lo, -cap), cap), fminf(fmaxf(hi, -cap), cap));
-          }
-          if (p[i].state == 2) {
-            *reinterpret_cast<uint2*>(a.c.pool[x[i]] + p[i].cached + lane * 8) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-            if (lane == 0) a.c.exps[x[i]][p[i].exp] = static_cast<uint8_t>(ex);
-          }
-        } else if (p[i].state == 2) {
-          *reinterpret_cast<uint4*>(a.c.pool[x[i]] + p[i].cached + lane * 16) = r[i];
-        }
-      } else if (p[i].state != 0) {  // a row without a position is zeros (r is)
-        if (kQuantised && p[i].state == 2) {
-          const uint32_t f = e4m3_factor(e[i]) * 0x10001u, f2 = e4m3_factor2(e[i]) * 0x10001u;
-          const uint32_t w0 = r[i].x, w1 = r[i].y;
-          r[i].x = mul_bf16x2(mul_bf16x2(e4m3_pattern(__byte_perm(w0, 0, 0x1404)), f), f2);
-          r[i].y = mul_bf16x2(mul_bf16x2(e4m3_pattern(__byte_perm(w0, 0, 0x3424)), f), f2);
-          r[i].z = mul_bf16x2(mul_bf16x2(e4m3_pattern(__byte_perm(w1, 0, 0x1404)), f), f2);
-          r[i].w = mul_bf16x2(mul_bf16x2(e4m3_pattern(__byte_perm(w1, 0, 0x3424)), f), f2);
-        }
-        *reinterpret_cast<uint4*>(packed[i]) = r[i];
-      }
+    if (meet) {
+      __syncthreads();
+      uint8_t *e0 = exp_at[lane][0], *e1 = exp_at[lane][1];  // lane: token of the block
+      if (e0 != nullptr)
+        for (int y = c0 + grp; y < c1; y += kRowGroups) *exp_of(y, e0, e1) = exp_s[y - c0][lane];
+      __syncthreads();
     }
   }
 }

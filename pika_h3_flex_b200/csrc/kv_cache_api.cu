@@ -103,15 +103,21 @@ int32_t move_rows(bool write, const h3a_cache* c, const h3a_cache_batch* b, void
   a.head_bytes[0] = k_sh * 2;
   a.row_bytes[1] = v_sl * 2;
   a.head_bytes[1] = v_sh * 2;
-  const int64_t units = static_cast<int64_t>(b->rows) * 2 * c->heads, per_block = h3a::kRowThreads / 16;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((units + per_block - 1) / per_block, 8ll * dev.sms));
+  // Half-warps per token: one is the cheapest (a token is looked up once), but few tokens are spread over more of them,
+  // up to a block's 16, and over further blocks, until about eight of them run on every SM.
+  const int64_t want = 8ll * dev.sms, n_rows = 2ll * c->heads;
+  int per_token = 1;
+  while (per_token < h3a::kRowGroups && b->rows * static_cast<int64_t>(per_token) < want && per_token < n_rows) per_token *= 2;
+  const int64_t blocks_x = (b->rows + static_cast<int64_t>(h3a::kRowGroups / per_token) - 1) / (h3a::kRowGroups / per_token);
+  const int64_t more = std::max<int64_t>(1, std::min(want / std::max<int64_t>(1, b->rows * static_cast<int64_t>(per_token)), n_rows / per_token));
+  const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>(more));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (write) {
-    if (c->quantised) h3a::cache_rows_kernel<true, true><<<grid, h3a::kRowThreads, 0, st>>>(a);
-    else h3a::cache_rows_kernel<true, false><<<grid, h3a::kRowThreads, 0, st>>>(a);
+    if (c->quantised) h3a::cache_rows_kernel<true, true><<<grid, h3a::kRowThreads, 0, st>>>(a, per_token);
+    else h3a::cache_rows_kernel<true, false><<<grid, h3a::kRowThreads, 0, st>>>(a, per_token);
   } else {
-    if (c->quantised) h3a::cache_rows_kernel<false, true><<<grid, h3a::kRowThreads, 0, st>>>(a);
-    else h3a::cache_rows_kernel<false, false><<<grid, h3a::kRowThreads, 0, st>>>(a);
+    if (c->quantised) h3a::cache_rows_kernel<false, true><<<grid, h3a::kRowThreads, 0, st>>>(a, per_token);
+    else h3a::cache_rows_kernel<false, false><<<grid, h3a::kRowThreads, 0, st>>>(a, per_token);
   }
   return cudaGetLastError() == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
 }
