@@ -9,7 +9,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 SRCS = [os.path.join(HERE, "csrc", f) for f in ("h3attn_api.cu", "kv_cache_api.cu")]
 OUT = os.path.join(HERE, "libh3attn.so")
 DEPS = SRCS + [os.path.join(HERE, "csrc", f) for f in ("attn_fwd.cuh", "attn_fwd_pair.cuh", "qk_prep.cuh", "qkv_proj.cuh", "adaln.cuh", "ptx.cuh",
-                                                       "kv_cache.cuh", "cache_attn.cuh", "cache_attn_tile.cuh")] + [
+                                                       "kv_cache.cuh", "cache_attn.cuh", "cache_attn_few.cuh", "cache_attn_tile.cuh")] + [
     os.path.join(HERE, "..", "include", "h3attn.h")
 ]
 

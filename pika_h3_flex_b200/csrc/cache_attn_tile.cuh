@@ -25,6 +25,7 @@
 namespace h3a {
 
 constexpr int kTileThreads = 512;
+constexpr int kKeyTile = 128, kTileKeyShift = 7;
 constexpr int kTileSoftmaxRegs = 200, kTileOtherRegs = 56, kTileLaunchRegs = 128;
 static_assert(256 * kTileSoftmaxRegs + 256 * kTileOtherRegs <= kTileLaunchRegs * kTileThreads, "setmaxnreg budget exceeds the launch allocation");
 constexpr int kTileRows = 256;         // rows of an item

@@ -9,7 +9,7 @@
 #include <cstring>
 #include <mutex>
 
-#include "cache_attn.cuh"
+#include "cache_attn_few.cuh"
 #include "cache_attn_tile.cuh"
 
 namespace {
@@ -158,7 +158,7 @@ constexpr int kFewMinShare = 3;  // units (a tile, or an item's set-up) below wh
 
 // What a call of this shape launches.
 struct AttnPlan {
-  int item_rows = 0, item_tokens = 0, shares = 0;
+  int item_rows = 0, item_tokens = 0, key_shift = 0, shares = 0;
   size_t bytes = 0;
 };
 AttnPlan attn_plan(const h3a_cache_attn_params* p, int sms) {
@@ -169,27 +169,28 @@ AttnPlan attn_plan(const h3a_cache_attn_params* p, int sms) {
   if (rows > h3a::kFewRows && group <= 128) {
     n.item_rows = h3a::kTileRows;
     n.item_tokens = 2 * (128 / group);
+    n.key_shift = h3a::kTileKeyShift;
+    n.shares = sms;
   } else {
-    n.item_rows = h3a::kFewRows;
+    n.item_rows = rows <= 8 ? 8 : h3a::kFewRows;
+    n.key_shift = h3a::kFewKeyShift;
+    n.shares = sms * (rows <= 8 ? (p->cache.quantised ? h3a::kFewBlocksPerSm<true, 1> : h3a::kFewBlocksPerSm<false, 1>)
+                                : (p->cache.quantised ? h3a::kFewBlocksPerSm<true, 2> : h3a::kFewBlocksPerSm<false, 2>));
   }
-  n.shares = sms;
   n.bytes = static_cast<size_t>(n.shares) * (4 * sizeof(int) + 2ull * n.item_rows * (h3a::kCacheDim + 2) * sizeof(float));
   return n;
 }
 
-template <typename K>
-int32_t allow_smem(K kernel, int bytes, int dev, std::once_flag* once, cudaError_t* err) {
-  std::call_once(once[dev], [&] { err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
-  return err[dev] == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
-}
-
-template <bool kFp8>
+template <bool kFp8, int kNT>
 int32_t launch_few(const h3a::CacheAttnArgs& a, int shares, const Device& dev, cudaStream_t st) {
   static std::once_flag once[kMaxDevices];
   static cudaError_t err[kMaxDevices];
-  const int32_t rc = allow_smem(h3a::cache_attn_few_kernel<kFp8>, h3a::kFewSmemBytes, dev.id, once, err);
-  if (rc != H3A_OK) return rc;
-  h3a::cache_attn_few_kernel<kFp8><<<shares, h3a::kFewThreads, h3a::kFewSmemBytes, st>>>(a);
+  constexpr int kSmem = sizeof(h3a::FewSmem<kNT>);
+  std::call_once(once[dev.id], [&] {
+    err[dev.id] = cudaFuncSetAttribute(h3a::cache_attn_few_kernel<kFp8, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  });
+  if (err[dev.id] != cudaSuccess) return H3A_ERR_LAUNCH;
+  h3a::cache_attn_few_kernel<kFp8, kNT><<<shares, h3a::kFewThreads, kSmem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
 }
 
@@ -289,6 +290,7 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   a.causal = p->causal;
   a.item_rows = n.item_rows;
   a.item_tokens = n.item_tokens;
+  a.key_shift = n.key_shift;
   a.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / std::sqrt(128.0f)) * 1.4426950408889634f;
   a.desc = static_cast<int*>(p->workspace);
   a.part = reinterpret_cast<float*>(a.desc + 4 * n.shares);
@@ -297,8 +299,10 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (n.item_tokens > 0)
     rc = p->cache.quantised ? launch_tile<true>(p, a, n.shares, dev, st) : launch_tile<false>(p, a, n.shares, dev, st);
+  else if (n.item_rows == 8)
+    rc = p->cache.quantised ? launch_few<true, 1>(a, n.shares, dev, st) : launch_few<false, 1>(a, n.shares, dev, st);
   else
-    rc = p->cache.quantised ? launch_few<true>(a, n.shares, dev, st) : launch_few<false>(a, n.shares, dev, st);
+    rc = p->cache.quantised ? launch_few<true, 2>(a, n.shares, dev, st) : launch_few<false, 2>(a, n.shares, dev, st);
   return rc == H3A_OK ? launch_join(a, n.shares, st) : rc;
 }
 
