@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .ops import HEAD_DIM, _lhd, _require_cuda
+from .ops import HEAD_DIM, _require_cuda
 
 PAGE_MULTIPLE = 16
 
@@ -60,6 +60,7 @@ class KVCache:
         self.n_pages, self.page_size, self.heads = (int(x) for x in k.shape[:3])
         self.device = k.device
         c = self._c = _lib.Cache()
+        self._ref = C.byref(c)
         c.n_pages, c.page_size, c.heads, c.d, c.quantised = self.n_pages, self.page_size, self.heads, HEAD_DIM, int(self.quantised)
         for name, t in (("k", k), ("v", v), ("k_exp", k_exp), ("v_exp", v_exp)):
             if t is not None:
@@ -98,37 +99,72 @@ class CacheBatch:
         c.pages, c.lengths, c.starts = pages.data_ptr(), lengths.data_ptr(), starts.data_ptr()
         c.pages_stride = pages.stride(0) if n > 1 else pages.shape[1]
         c.n_seqs, c.max_pages = n, pages.shape[1]
+        self._by_rows = {}
 
-    def _for(self, rows: int) -> "_lib.CacheBatch":
-        c = _lib.CacheBatch.from_buffer_copy(self._c)  # a copy: two threads may use one batch with different row counts
-        c.rows = rows
-        return c
-
-
-def _same_device(cache: KVCache, batch: CacheBatch, *tensors) -> None:
-    for t in (batch, *tensors):
-        if t is not None and t.device != cache.device:
-            raise ValueError(f"expected everything on {cache.device}, got {t.device}")
+    def _for(self, rows: int):
+        """The C description of this batch for packed tensors of so many rows."""
+        ref = self._by_rows.get(rows)
+        if ref is None:
+            c = _lib.CacheBatch.from_buffer_copy(self._c)
+            c.rows = rows
+            if len(self._by_rows) >= 64:
+                self._by_rows.clear()
+            ref = self._by_rows[rows] = C.byref(c)  # holds on to c
+        return ref
 
 
 def _on(device: torch.device):
     """Launches go to the tensors' device, whichever is current."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
-def _rows(t: torch.Tensor, name: str, heads: int) -> Tuple[int, int, int]:
-    L, H, _, _ = _lhd(t, name, (torch.bfloat16,))
-    if H != heads:
-        raise ValueError(f"{name} has {H} heads, expected {heads}")
-    return L, _stride(t, 0), _stride(t, 1)
+_HERE = nullcontext()
 
 
-def _status_ptr(status_word: Optional[torch.Tensor]) -> Optional[int]:
+def _stream(device: torch.device) -> int:
+    """The current stream of a device as CUDA knows it.  (``torch.cuda.current_stream`` builds a Python object around it
+    first: 2.2 us of a call that takes 8.)"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _rows(t: torch.Tensor, name: str, heads: int, device: torch.device) -> Tuple[int, int, int]:
+    """Rows and the two strides of a packed [rows, heads, 128] bf16 tensor (these calls are made for single tokens too,
+    so the checks are few and cheap)."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1:
+        raise ValueError(f"{name}: expected logical [rows, heads, 128] with a contiguous last dim, got {tuple(shape)} / {stride}")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: dtype {t.dtype} is not bfloat16")
+    if shape[1] != heads:
+        raise ValueError(f"{name} has {shape[1]} heads, expected {heads}")
+    if t.device != device:
+        _require_cuda(t)
+        raise ValueError(f"expected everything on {device}, got {name} on {t.device}")
+    return shape[0], stride[0] if shape[0] > 1 else HEAD_DIM, stride[1] if heads > 1 else HEAD_DIM
+
+
+def _status_ptr(status_word: Optional[torch.Tensor], device: torch.device) -> Optional[int]:
     if status_word is None:
         return None
-    if status_word.dtype != torch.int32 or not status_word.is_cuda:
-        raise ValueError("status_word must be an int32 device tensor")
+    if status_word.dtype != torch.int32 or status_word.device != device:
+        raise ValueError(f"status_word must be an int32 tensor on {device}")
     return status_word.data_ptr()
+
+
+def _move(name: str, cache: KVCache, batch: CacheBatch, k: torch.Tensor, v: torch.Tensor, status_word: Optional[torch.Tensor]) -> None:
+    device = cache.device
+    L, ksl, ksh = _rows(k, "k", cache.heads, device)
+    Lv, vsl, vsh = _rows(v, "v", cache.heads, device)
+    if L != Lv:
+        raise ValueError("k and v disagree on the number of rows")
+    if batch.device != device:
+        raise ValueError(f"expected everything on {device}, got the batch on {batch.device}")
+    status = _status_ptr(status_word, device)
+    if L == 0:
+        return
+    with _on(device):
+        check(getattr(_lib.load(), name)(cache._ref, batch._for(L), k.data_ptr(), ksl, ksh, v.data_ptr(), vsl, vsh, status,
+                                         _stream(device)), name)
 
 
 def cache_write(cache: KVCache, batch: CacheBatch, k: torch.Tensor, v: torch.Tensor, status_word: Optional[torch.Tensor] = None) -> None:
@@ -136,16 +172,7 @@ def cache_write(cache: KVCache, batch: CacheBatch, k: torch.Tensor, v: torch.Ten
     smallest power of two that brings the largest magnitude to at most 448, then e4m3).  A page that is written to must
     belong to one sequence only; pages that are only read may be shared."""
     _require_cuda(k, v)
-    _same_device(cache, batch, k, v, status_word)
-    L, ksl, ksh = _rows(k, "k", cache.heads)
-    Lv, vsl, vsh = _rows(v, "v", cache.heads)
-    if L != Lv:
-        raise ValueError("k and v disagree on the number of rows")
-    if L == 0:
-        return
-    with _on(cache.device):
-        check(_lib.load().h3a_cache_write(C.byref(cache._c), C.byref(batch._for(L)), k.data_ptr(), ksl, ksh, v.data_ptr(), vsl, vsh,
-                                          _status_ptr(status_word), torch.cuda.current_stream(cache.device).cuda_stream), "h3a_cache_write")
+    _move("h3a_cache_write", cache, batch, k, v, status_word)
 
 
 def cache_read(cache: KVCache, batch: CacheBatch, rows: Optional[int] = None, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
@@ -158,19 +185,10 @@ def cache_read(cache: KVCache, batch: CacheBatch, rows: Optional[int] = None, ou
     if out is None:
         if rows < 0:
             raise ValueError("rows must not be negative")
-        out = tuple(torch.empty(rows, cache.heads, HEAD_DIM, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+        out = [torch.empty(rows, cache.heads, HEAD_DIM, dtype=torch.bfloat16, device=cache.device) for _ in range(2)]
     k, v = out
     _require_cuda(k, v)
-    _same_device(cache, batch, k, v, status_word)
-    L, ksl, ksh = _rows(k, "k", cache.heads)
-    Lv, vsl, vsh = _rows(v, "v", cache.heads)
-    if L != Lv:
-        raise ValueError("k and v disagree on the number of rows")
-    if L == 0:
-        return k, v
-    with _on(cache.device):
-        check(_lib.load().h3a_cache_read(C.byref(cache._c), C.byref(batch._for(L)), k.data_ptr(), ksl, ksh, v.data_ptr(), vsl, vsh,
-                                         _status_ptr(status_word), torch.cuda.current_stream(cache.device).cuda_stream), "h3a_cache_read")
+    _move("h3a_cache_read", cache, batch, k, v, status_word)
     return k, v
 
 
@@ -198,31 +216,32 @@ def cache_attn(q: torch.Tensor, cache: KVCache, batch: CacheBatch, causal: bool 
     is the token at position ``lengths[b] - n_b + i`` and sees the keys up to itself (write its K and V first); otherwise
     every row sees all ``lengths[b]`` keys.  A row without a key is zeros (lse -inf).  Returns ``out [rows, heads, 128]``
     bf16 (and ``lse [heads, rows]``); rows outside every sequence are not written.  ``softmax_scale`` 0: ``1/sqrt(128)``."""
-    _require_cuda(q, out, workspace)
-    _same_device(cache, batch, q, out, status_word, workspace)
-    L, H, _, _ = _lhd(q, "q", (torch.bfloat16,))
+    _require_cuda(q)
+    device = cache.device
+    H = q.shape[1] if q.dim() == 3 else 0
+    L, qsl, qsh = _rows(q, "q", H, device)
     if H == 0 or H % cache.heads:
         raise ValueError(f"q has {H} heads: not a multiple of the cache's {cache.heads}")
+    if batch.device != device:
+        raise ValueError(f"expected everything on {device}, got the batch on {batch.device}")
     if out is None:
-        out = torch.empty(L, H, HEAD_DIM, dtype=torch.bfloat16, device=q.device)
-    Lo, osl, osh = _rows(out, "out", H)
-    if Lo != L:
-        raise ValueError("out must have q's shape")
-    lse = torch.empty(H, L, dtype=torch.float32, device=q.device) if return_lse else None
+        out = torch.empty(L, H, HEAD_DIM, dtype=torch.bfloat16, device=device)
+        osl, osh = H * HEAD_DIM, HEAD_DIM
+    else:
+        Lo, osl, osh = _rows(out, "out", H, device)
+        if Lo != L:
+            raise ValueError("out must have q's shape")
+    status = _status_ptr(status_word, device)
+    lse = torch.empty(H, L, dtype=torch.float32, device=device) if return_lse else None
     if L == 0:
         return (out, lse) if return_lse else out
     if workspace is None:
-        workspace = torch.empty(_workspace_bytes(cache.device.index, L, batch._c.n_seqs, H, cache.heads, cache.quantised), dtype=torch.uint8, device=q.device)
-    p = _lib.CacheAttnParams()
-    p.cache, p.batch = cache._c, batch._c
+        workspace = torch.empty(_workspace_bytes(device.index, L, batch._c.n_seqs, H, cache.heads, cache.quantised), dtype=torch.uint8, device=device)
+    elif workspace.device != device:
+        raise ValueError(f"expected everything on {device}, got the workspace on {workspace.device}")
+    p = _lib.CacheAttnParams(cache._c, batch._c, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, qsl, qsh, osl, osh,
+                             H, 1 if causal else 0, softmax_scale, workspace.data_ptr(), workspace.nbytes, status, wait_limit_ns)
     p.batch.rows = L
-    p.q, p.o = q.data_ptr(), out.data_ptr()
-    p.lse = lse.data_ptr() if return_lse else None
-    p.q_stride_l, p.q_stride_h, p.o_stride_l, p.o_stride_h = _stride(q, 0), _stride(q, 1), osl, osh
-    p.heads, p.causal, p.softmax_scale = H, int(bool(causal)), float(softmax_scale)
-    p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    p.status_word = _status_ptr(status_word)
-    p.wait_limit_ns = int(wait_limit_ns)
-    with _on(cache.device):
-        check(_lib.load().h3a_cache_attn(C.byref(p), torch.cuda.current_stream(cache.device).cuda_stream), "h3a_cache_attn")
+    with _on(device):
+        check(_lib.load().h3a_cache_attn(C.byref(p), _stream(device)), "h3a_cache_attn")
     return (out, lse) if return_lse else out

@@ -22,14 +22,15 @@ struct CacheAttnArgs {
   long long o_stride_l, o_stride_h;
   float* lse;                        // [heads, rows] or null
   int heads, group;                  // group = heads / kv_heads
+  FastDiv by_group, by_item_tokens, by_item_rows;
   int causal;
   int item_rows;                     // rows per item (the kernel's tile)
   int item_tokens;                   // tokens per item, or 0: items are cut by rows, not by tokens
   int key_shift;                     // log2 of the keys per tile
   float scale_log2;
   float* part;                       // [share][2][item_rows] x (128 + 2) fp32
-  int* desc;                         // [share][4]: the item that a share begins and does not finish
-  int min_share;                     // a share has at least this many units
+  int* desc;                         // [share][kDescInts]: the item that a share begins and does not finish
+  int share_shift;                   // a share has at least 2^this units
   long long wait_ns;
 };
 
@@ -42,7 +43,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const CacheAttnArgs& a, int b) {
   s.s0 = q.s0;
   s.n = q.n;
   s.len = q.len;
-  s.n_items = a.item_tokens > 0 ? (q.n + a.item_tokens - 1) / a.item_tokens : (q.n * a.group + a.item_rows - 1) / a.item_rows;
+  s.n_items = a.item_tokens > 0 ? a.by_item_tokens(q.n + a.item_tokens - 1) : a.by_item_rows(q.n * a.group + a.item_rows - 1);
   return s;
 }
 // keys that token i of the sequence sees
@@ -50,7 +51,7 @@ __device__ __forceinline__ int key_limit(const CacheAttnArgs& a, const AttnSeq& 
   return a.causal ? max(0, min(s.len, s.len - s.n + i + 1)) : s.len;
 }
 __device__ __forceinline__ int item_last_token(const CacheAttnArgs& a, const AttnSeq& s, int it) {
-  return min(s.n, a.item_tokens > 0 ? (it + 1) * a.item_tokens : ((it + 1) * a.item_rows + a.group - 1) / a.group) - 1;
+  return min(s.n, a.item_tokens > 0 ? (it + 1) * a.item_tokens : a.by_group((it + 1) * a.item_rows + a.group - 1)) - 1;
 }
 __device__ __forceinline__ int item_tiles(const CacheAttnArgs& a, const AttnSeq& s, int it) {
   return (key_limit(a, s, item_last_token(a, s, it)) + (1 << a.key_shift) - 1) >> a.key_shift;
@@ -119,14 +120,75 @@ struct ShareIter {
   }
 };
 
-__device__ __forceinline__ int n_shares_of(long long total, int grid, int min_share) {
-  return static_cast<int>(max(1ll, min(static_cast<long long>(grid), total / min_share)));
+// a / b, in 32 bits where they fit: the 64-bit division is a loop of some 70 instructions
+__device__ __forceinline__ long long div_units(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+// which units share c has: [total c / n, total (c + 1) / n)
+__device__ __forceinline__ void share_range(const CacheAttnArgs& a, ShareIter& s) {
+  s.n_shares = static_cast<int>(max(1ll, min(static_cast<long long>(gridDim.x), s.total >> a.share_shift)));
+  const int c = blockIdx.x;
+  const long long q = div_units(s.total, s.n_shares);
+  const uint32_t r = static_cast<uint32_t>(s.total - q * s.n_shares), n = s.n_shares;
+  s.pos = c < s.n_shares ? q * c + r * c / n : 0;
+  s.end = c < s.n_shares ? q * (c + 1) + r * (c + 1) / n : 0;
+}
+// the share's first item, given its first sequence and the units before that
+__device__ __forceinline__ void share_item(const CacheAttnArgs& a, ShareIter& s, long long head_total) {
+  s.h = static_cast<int>(div_units(s.pos - s.item_base, head_total));
+  s.item_base += s.h * head_total;
+  s.it = 0;
+  if (!a.causal) {  // items of equal length
+    const int units = 1 + item_tiles(a, s.s, 0);
+    s.it = static_cast<int>(div_units(s.pos - s.item_base, units));
+    s.item_base += static_cast<long long>(s.it) * units;
+    return;
+  }
+  for (;;) {
+    const int units = 1 + item_tiles(a, s.s, s.it);
+    if (s.pos < s.item_base + units) break;
+    s.item_base += units;
+    ++s.it;
+  }
 }
 
-// Executed by all threads of the block: finds where share `blockIdx.x` begins.  Every thread sums a run of sequences, the
-// block scans the sums, and the thread whose run holds the share's first unit looks it up.
+// Executed by all threads of the block: finds where share `blockIdx.x` begins, the same in every thread.  Up to 32
+// sequences every warp does it by itself, one sequence per lane, without a barrier: a single token's call is over in a few
+// microseconds.  More sequences: every thread sums a run of them, the block scans the sums, and the thread whose run holds
+// the share's first unit looks it up.
 __device__ __forceinline__ ShareIter share_begin(const CacheAttnArgs& a, ShareStart* sh) {
   const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  ShareIter s;
+  if (a.c.n_seqs <= 32) {
+    AttnSeq q{0, 0, 0, 0};
+    long long head_total = 0;
+    if (lane < a.c.n_seqs) {
+      q = attn_seq(a, lane);
+      head_total = head_units(a, q);
+    }
+    const long long own = a.c.kv_heads * head_total;
+    long long incl = own;
+    for (int o = 1; o < a.c.n_seqs; o <<= 1) {
+      const long long v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    s.total = __shfl_sync(0xFFFFFFFFu, incl, a.c.n_seqs - 1);
+    share_range(a, s);
+    const uint32_t here = __ballot_sync(0xFFFFFFFFu, s.pos < s.end && incl - own <= s.pos && s.pos < incl);
+    const int b = max(0, __ffs(here) - 1);
+    s.b = b;
+    s.h = s.it = 0;
+    s.s.s0 = __shfl_sync(0xFFFFFFFFu, q.s0, b);
+    s.s.n = __shfl_sync(0xFFFFFFFFu, q.n, b);
+    s.s.len = __shfl_sync(0xFFFFFFFFu, q.len, b);
+    s.s.n_items = __shfl_sync(0xFFFFFFFFu, q.n_items, b);
+    s.item_base = __shfl_sync(0xFFFFFFFFu, incl - own, b);
+    head_total = __shfl_sync(0xFFFFFFFFu, head_total, b);
+    if (here == 0) s.end = s.pos;  // an empty share
+    else share_item(a, s, head_total);
+    return s;
+  }
   const int per = (a.c.n_seqs + nt - 1) / nt;
   const int b0 = min(a.c.n_seqs, tid * per), b1 = min(a.c.n_seqs, b0 + per);
   long long own = 0;
@@ -147,12 +209,8 @@ __device__ __forceinline__ ShareIter share_begin(const CacheAttnArgs& a, ShareSt
     total += v;
   }
   before += incl - own;
-  ShareIter s;
   s.total = total;
-  s.n_shares = n_shares_of(total, gridDim.x, a.min_share);
-  const int c = blockIdx.x;
-  s.pos = c < s.n_shares ? total * c / s.n_shares : 0;
-  s.end = c < s.n_shares ? total * (c + 1) / s.n_shares : 0;
+  share_range(a, s);
   if (s.pos < s.end && before <= s.pos && s.pos < before + own) {
     long long base = before;
     for (int b = b0; b < b1; ++b) {
@@ -175,15 +233,7 @@ __device__ __forceinline__ ShareIter share_begin(const CacheAttnArgs& a, ShareSt
     return s;
   }
   s.s = attn_seq(a, s.b);
-  const long long w = head_units(a, s.s);
-  s.h = static_cast<int>((s.pos - s.item_base) / w);
-  s.item_base += s.h * w;
-  for (;;) {
-    const int units = 1 + item_tiles(a, s.s, s.it);
-    if (s.pos < s.item_base + units) break;
-    s.item_base += units;
-    ++s.it;
-  }
+  share_item(a, s, head_units(a, s.s));
   return s;
 }
 
@@ -212,7 +262,7 @@ __device__ __forceinline__ uint32_t finite_or_zero2(uint32_t w) {
 // value of dim `d` of a V row, whatever the cache holds it in
 template <bool kFp8>
 __device__ __forceinline__ float v_value(const CacheAttnArgs& a, int b, int h, int key, int d) {
-  const int slot = key / a.c.page_size, at = key - slot * a.c.page_size;
+  const int slot = a.c.by_page(key), at = key - slot * a.c.page_size;
   const long long id = checked_page(a, b, slot);
   const uint8_t* row = a.c.pool[1] + id * a.c.page_bytes[1] + at * a.c.token_bytes[1] + h * a.c.head_bytes[1];
   if constexpr (kFp8) {
@@ -226,43 +276,74 @@ __device__ __forceinline__ float v_value(const CacheAttnArgs& a, int b, int h, i
 
 constexpr float kNoMax = -3.0e38f;  // running maximum of a row that has seen no key: finite, so that differences stay numbers
 
+// lets the launch of the kernel that follows (the join) begin; it waits for this one's results itself
+__device__ __forceinline__ void allow_next_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------------------------------- joining
 constexpr int kJoinRows = 4;  // a warp per row
+constexpr int kDescInts = 8;  // parts (0: no such item), rows, first row (token * group + head in the group), sequence's first packed row, K/V head
+// The item that begins in this share goes on in later ones, up to the one that holds unit item_end - 1.
+__device__ __forceinline__ void describe_join(const CacheAttnArgs& a, const ShareIter& s, long long item_end, int n_rows, int r0, int s0, int h) {
+  const int last = static_cast<int>(div_units(item_end * s.n_shares + s.total - 1, s.total)) - 1;
+  int* d = a.desc + kDescInts * blockIdx.x;
+  *reinterpret_cast<int4*>(d) = make_int4(last - static_cast<int>(blockIdx.x) + 1, n_rows, r0, s0);
+  d[4] = h;
+}
 
-// Block (share, y): rows [4 y, 4 y + 4) of the item that begins in the share and ends in a later one.
-__global__ void __launch_bounds__(kJoinRows * 32) cache_attn_join_kernel(const CacheAttnArgs a) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the partial results are complete from here on
-  if (a.c.status && *reinterpret_cast<volatile int*>(a.c.status) != 0) return;
+// Block (share, y): rows [4 y, 4 y + 4) of the item that begins in the share and ends in a later one.  The kernel is a few
+// dependent loads long, so its launch overlaps the kernel before it, everything it has to know about the item is in the
+// description, and the loads of kJoinParts parts' O wait for nothing else: with the parts one after the other a row of 37
+// parts took 29 us.  16 at a time for small items (up to as many parts as shares), 4 for large ones (two or three, and
+// many rows: registers for more warps).
+template <int kJoinParts>
+__global__ void __launch_bounds__(kJoinRows * 32) cache_attn_join_kernel(const __grid_constant__ CacheAttnArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial results are complete from here on
   const int share = blockIdx.x;
-  const int4 d = *reinterpret_cast<const int4*>(a.desc + 4 * share);  // sequence, head, item, last share
-  if (d.x < 0) return;
-  const AttnSeq s = attn_seq(a, d.x);
+  const int4 d = *reinterpret_cast<const int4*>(a.desc + kDescInts * share);
+  const int kv_head = a.desc[kDescInts * share + 4];
+  if (a.c.status && *reinterpret_cast<volatile int*>(a.c.status) != 0) return;
   const int lane = threadIdx.x & 31;
   const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
-  const int r0 = a.item_tokens > 0 ? d.z * a.item_tokens * a.group : d.z * a.item_rows;
-  const int n_rows = min(s.n * a.group - r0, a.item_tokens > 0 ? a.item_tokens * a.group : a.item_rows);
-  if (r >= n_rows) return;
+  const int n_parts = d.x, n_rows = d.y, r0 = d.z;
+  if (n_parts <= 0 || r >= n_rows) return;
   // parts of the row: the tail slot of this share, then the head slots of the next ones
-  const int n_parts = d.w - share + 1;
-  auto slot = [&](int i) { return part_slot(a, share + i, i == 0); };
-  auto stat = [&](int i, int which) { return slot(i)[a.item_rows * kCacheDim + which * a.item_rows + r]; };
-  float m = kNoMax;
-  for (int i = lane; i < n_parts; i += 32) m = fmaxf(m, stat(i, 0));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  const long long slot = 2ll * a.item_rows * (kCacheDim + 2);
+  const float* first = part_slot(a, share, true);
+  const float* next = part_slot(a, share, false);  // + i slots for part i > 0
+  float m = kNoMax, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < n_parts; ++i) {
-    const float w = ex2_approx(stat(i, 0) - m);
-    const float4 v = *reinterpret_cast<const float4*>(slot(i) + r * kCacheDim + 4 * lane);
-    l += stat(i, 1) * w;
-    acc.x += v.x * w;
-    acc.y += v.y * w;
-    acc.z += v.z * w;
-    acc.w += v.w * w;
+  for (int i0 = 0; i0 < n_parts; i0 += kJoinParts) {
+    const int n = min(kJoinParts, n_parts - i0);
+    float4 v[kJoinParts];
+#pragma unroll
+    for (int i = 0; i < kJoinParts; ++i)
+      if (i < n) v[i] = *reinterpret_cast<const float4*>((i0 + i == 0 ? first : next + (i0 + i) * slot) + r * kCacheDim + 4 * lane);
+    float mi = kNoMax, li = 0.f;
+    if (lane < n) {
+      const float* st = (i0 + lane == 0 ? first : next + (i0 + lane) * slot) + a.item_rows * kCacheDim + r;
+      mi = st[0];
+      li = st[a.item_rows];
+    }
+    float top = mi;
+#pragma unroll
+    for (int o = kJoinParts / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    top = __shfl_sync(0xFFFFFFFFu, top, 0);
+    const float m_new = fmaxf(m, top), f = ex2_approx(m - m_new), wi = ex2_approx(mi - m_new);
+    m = m_new;
+    l *= f;
+    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+    for (int i = 0; i < kJoinParts; ++i)
+      if (i < n) {
+        const float w = __shfl_sync(0xFFFFFFFFu, wi, i);
+        l += w * __shfl_sync(0xFFFFFFFFu, li, i);
+        acc.x += v[i].x * w;
+        acc.y += v[i].y * w;
+        acc.z += v[i].z * w;
+        acc.w += v[i].w * w;
+      }
   }
-  const int row = r0 + r, token = s.s0 + row / a.group, head = d.y * a.group + row % a.group;
+  const int row = r0 + r, i = a.by_group(row), token = d.w + i, head = kv_head * a.group + row - i * a.group;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   uint2 w;
   w.x = pack_bf16x2(acc.x * inv, acc.y * inv);

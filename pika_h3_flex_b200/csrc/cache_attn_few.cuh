@@ -93,31 +93,84 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
   constexpr int kKW = kFp8 ? 2 : 4;  // 16-byte pieces per lane of a K row
   constexpr int kVW = kFp8 ? 1 : 2;  // ... of a V row
 
+  allow_next_launch();
   {
-    const ShareIter iter = share_begin(a, &start);
+    ShareIter iter = share_begin(a, &start);
     if (threadIdx.x == 0) {
+      a.desc[kDescInts * blockIdx.x] = 0;
+      sm.poison = 0;
+      sm.more = iter.next(a, sm.piece);
       sm.iter = iter;
-      a.desc[4 * blockIdx.x] = -1;
     }
   }
   const Piece& p = sm.piece;
   for (;;) {
-    __syncthreads();  // the previous piece's readers of shared memory are done
-    if (threadIdx.x == 0) {
-      sm.poison = 0;
-      sm.more = sm.iter.next(a, sm.piece);
-    }
-    __syncthreads();
+    __syncthreads();  // the piece is there
     if (!sm.more) return;
     const int r0 = p.it * kRows;
     const int n_rows = min(kRows, p.s.n * a.group - r0);
+    const int lim_min = key_limit(a, p.s, a.by_group(r0));
+    const int lim_max = key_limit(a, p.s, item_last_token(a, p.s, p.it));
+
+    // O^T: [i][j] holds, of dims (2 j, gid) and (2 j + 1, gid) of the loads' order, rows 8 i + 2 tig + {0, 1}
+    float o[kNT][8][4];
+#pragma unroll
+    for (int i = 0; i < kNT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+    float m[kNT][2], l[kNT][2];
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) {
+      m[i][0] = m[i][1] = kNoMax;
+      l[i][0] = l[i][1] = 0.f;
+    }
+    uint32_t vr = 0;  // e4m3: O is in units of 2^(vr - 127); 0: none yet
+
+    // The warp's 16 keys of tile t.  Its page number is fetched a step before its rows.
+    const int end_key = min(lim_max, p.t1 << kFewKeyShift);
+    int key0 = (p.t0 << kFewKeyShift) + warp * 16;
+    const int* table = a.c.pages + p.b * a.c.pages_stride;
+    uint4 k[2 * kKW], v[4 * kVW];
+    uint32_t e = 0;  // lanes 0-15: exponent byte of K row `lane`; lanes 16-31: of V row `lane - 16`
+    auto raw_page = [&](int key) { return key < end_key ? __ldg(table + a.c.by_page(key)) : 0; };
+    auto check_page = [&](int id) -> long long {
+      if (static_cast<unsigned>(id) < static_cast<unsigned>(a.c.n_pages)) return id;
+      report_cache(a.c, p.b);
+      return 0;
+    };
+    auto load_k = [&](long long id, int key) {
+      const int at = key - a.c.by_page(key) * a.c.page_size;
+      const uint8_t* src = a.c.pool[0] + id * a.c.page_bytes[0] + (at + gid) * a.c.token_bytes[0] + p.h * a.c.head_bytes[0] + 16 * tig;
+#pragma unroll
+      for (int u = 0; u < 2; ++u, src += 8 * a.c.token_bytes[0])
+#pragma unroll
+        for (int x = 0; x < kKW; ++x) k[u * kKW + x] = ldg_stream(src + 64 * x);
+      if constexpr (kFp8) {
+        const int x = lane >> 4;
+        e = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + (at + (lane & 15)) * a.c.exp_token[x] + p.h * a.c.exp_head[x]);
+      }
+    };
+    auto load_v = [&](long long id, int key) {
+      const uint8_t* src = a.c.pool[1] + id * a.c.page_bytes[1] + (key - a.c.by_page(key) * a.c.page_size + 2 * tig) * a.c.token_bytes[1] + p.h * a.c.head_bytes[1] + 16 * gid;
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int x = 0; x < kVW; ++x) v[y * kVW + x] = ldg_stream(src + ((y & 1) + 8 * (y >> 1)) * a.c.token_bytes[1] + 128 * x);
+    };
+
+    long long id = 0;
+    if (key0 < end_key) {
+      id = check_page(raw_page(key0));
+      load_k(id, key0);
+      load_v(id, key0);
+    }
     // ---- Q as B fragments, dims in the order of the K loads below: half-warps load rows, 8 dims per lane
 #pragma unroll
     for (int r = threadIdx.x >> 4; r < kRows; r += kFewThreads / 16) {
       const int l = threadIdx.x & 15;
       uint4 w = make_uint4(0, 0, 0, 0);
       if (r < n_rows) {
-        const int token = (r0 + r) / a.group, head = p.h * a.group + (r0 + r) - token * a.group;
+        const int token = a.by_group(r0 + r), head = p.h * a.group + (r0 + r) - token * a.group;
         w = __ldg(reinterpret_cast<const uint4*>(a.q + (p.s.s0 + token) * a.q_row_bytes + head * a.q_head_bytes + 16 * l));
       }
       // bf16: piece x = dims 32 x + 8 t + [0, 8) of lane group t; e4m3: pieces 2 c, 2 c + 1 = dims 64 c + 16 t + [0, 16)
@@ -153,64 +206,9 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int r = 8 * i + 2 * tig + c;
-        lim[i][c] = r < n_rows ? key_limit(a, p.s, (r0 + r) / a.group) : 0;
+        lim[i][c] = r < n_rows ? key_limit(a, p.s, a.by_group(r0 + r)) : 0;
         q_unit[i][c] = kFp8 ? sm.q_scale[r] * a.scale_log2 : 0.f;
       }
-    const int lim_min = key_limit(a, p.s, r0 / a.group);
-    const int lim_max = key_limit(a, p.s, item_last_token(a, p.s, p.it));
-
-    // O^T: [i][j] holds, of dims (2 j, gid) and (2 j + 1, gid) of the loads' order, rows 8 i + 2 tig + {0, 1}
-    float o[kNT][8][4];
-#pragma unroll
-    for (int i = 0; i < kNT; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
-    float m[kNT][2], l[kNT][2];
-#pragma unroll
-    for (int i = 0; i < kNT; ++i) {
-      m[i][0] = m[i][1] = kNoMax;
-      l[i][0] = l[i][1] = 0.f;
-    }
-    uint32_t vr = 0;  // e4m3: O is in units of 2^(vr - 127); 0: none yet
-
-    // The warp's 16 keys of tile t.  Its page number is fetched a step before its rows.
-    const int end_key = min(lim_max, p.t1 << kFewKeyShift);
-    int key0 = (p.t0 << kFewKeyShift) + warp * 16;
-    const int* table = a.c.pages + p.b * a.c.pages_stride;
-    uint4 k[2 * kKW], v[4 * kVW];
-    uint32_t e = 0;  // lanes 0-15: exponent byte of K row `lane`; lanes 16-31: of V row `lane - 16`
-    auto raw_page = [&](int key) { return key < end_key ? __ldg(table + key / a.c.page_size) : 0; };
-    auto check_page = [&](int id) -> long long {
-      if (static_cast<unsigned>(id) < static_cast<unsigned>(a.c.n_pages)) return id;
-      report_cache(a.c, p.b);
-      return 0;
-    };
-    auto load_k = [&](long long id, int key) {
-      const int at = key % a.c.page_size;
-      const uint8_t* src = a.c.pool[0] + id * a.c.page_bytes[0] + (at + gid) * a.c.token_bytes[0] + p.h * a.c.head_bytes[0] + 16 * tig;
-#pragma unroll
-      for (int u = 0; u < 2; ++u, src += 8 * a.c.token_bytes[0])
-#pragma unroll
-        for (int x = 0; x < kKW; ++x) k[u * kKW + x] = ldg_stream(src + 64 * x);
-      if constexpr (kFp8) {
-        const int x = lane >> 4;
-        e = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + (at + (lane & 15)) * a.c.exp_token[x] + p.h * a.c.exp_head[x]);
-      }
-    };
-    auto load_v = [&](long long id, int key) {
-      const uint8_t* src = a.c.pool[1] + id * a.c.page_bytes[1] + (key % a.c.page_size + 2 * tig) * a.c.token_bytes[1] + p.h * a.c.head_bytes[1] + 16 * gid;
-#pragma unroll
-      for (int y = 0; y < 4; ++y)
-#pragma unroll
-        for (int x = 0; x < kVW; ++x) v[y * kVW + x] = ldg_stream(src + ((y & 1) + 8 * (y >> 1)) * a.c.token_bytes[1] + 128 * x);
-    };
-
-    long long id = 0;
-    if (key0 < end_key) {
-      id = check_page(raw_page(key0));
-      load_k(id, key0);
-      load_v(id, key0);
-    }
     int id_next = raw_page(key0 + (1 << kFewKeyShift));
     for (; key0 < end_key; key0 += 1 << kFewKeyShift) {
       const int next = key0 + (1 << kFewKeyShift);
@@ -467,7 +465,7 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
         acc[0] += v0.x * f; acc[1] += v0.y * f; acc[2] += v0.z * f; acc[3] += v0.w * f;
         acc[4] += v1.x * f; acc[5] += v1.y * f; acc[6] += v1.z * f; acc[7] += v1.w * f;
       }
-      const int token = (r0 + r) / a.group, head = p.h * a.group + (r0 + r) - token * a.group;
+      const int token = a.by_group(r0 + r), head = p.h * a.group + (r0 + r) - token * a.group;
       if (sm.poison) {  // rare: put back what was left out above, for the rows that see it
         const int end = min(key_limit(a, p.s, token), p.t1 << kFewKeyShift);
         for (int key = max(lim_min & ~15, p.t0 << kFewKeyShift); key < end; ++key)
@@ -495,10 +493,12 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
         }
       }
     }
-    if (threadIdx.x == 0 && p.first && !p.last) {  // the item goes on in later shares: say where it ends
-      const long long item_end = sm.iter.item_base + 1 + item_tiles(a, p.s, p.it);
-      const int last = static_cast<int>((item_end * sm.iter.n_shares + sm.iter.total - 1) / sm.iter.total) - 1;
-      *reinterpret_cast<int4*>(a.desc + 4 * blockIdx.x) = make_int4(p.b, p.h, p.it, last);
+    if (threadIdx.x == 0 && p.first && !p.last)
+      describe_join(a, sm.iter, sm.iter.item_base + 1 + item_tiles(a, p.s, p.it), n_rows, r0, p.s.s0, p.h);
+    __syncthreads();  // everybody is done with this piece's shared memory
+    if (threadIdx.x == 0) {
+      sm.poison = 0;
+      sm.more = sm.iter.next(a, sm.piece);
     }
   }
 }

@@ -132,7 +132,6 @@ struct TilePiece {
   int tok0, n, len;  // its number in the sequence; new rows and length of the sequence
   int whole;         // the piece is the whole item; otherwise its results are partial
   int tail;          // ... and go to the share's tail slot (the item begins here)
-  int it, last_share;
 };
 constexpr int kPieceRing = 4;
 constexpr int kPieceReaders = 15;  // warps
@@ -159,11 +158,9 @@ __device__ __forceinline__ void describe_piece(const CacheAttnArgs& a, const Sha
   q.len = p.s.len;
   q.whole = p.first && p.last;
   q.tail = p.first;
-  q.it = p.it;
-  q.last_share = -1;
-  if (p.first && !p.last) {  // the item goes on in later shares: where it ends
-    const long long item_end = iter.item_base + 1 + item_tiles(a, p.s, p.it);
-    q.last_share = static_cast<int>((item_end * iter.n_shares + iter.total - 1) / iter.total) - 1;
+  if (p.first && !p.last) {
+    const int r0 = q.tok0 * a.group;
+    describe_join(a, iter, iter.item_base + 1 + item_tiles(a, p.s, p.it), min(p.s.n * a.group - r0, a.item_tokens * a.group), r0, p.s.s0, p.h);
   }
 }
 
@@ -212,14 +209,16 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     bars->poison = 0;
     bars->early_exit = (a.c.status != nullptr && *reinterpret_cast<volatile int*>(a.c.status) != 0) ? 1u : 0u;
     fence_mbar_init();
-    a.desc[4 * blockIdx.x] = -1;
+    a.desc[kDescInts * blockIdx.x] = 0;
   }
   if (warp == 8 && lane == 0) {
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
   }
-  ShareIter iter = share_begin(a, &start);  // has block-wide barriers
+  allow_next_launch();
+  ShareIter iter = share_begin(a, &start);
+  __syncthreads();  // barriers and flags are set up
   if (bars->early_exit) return;
   if (warp == 9) {
     tmem_alloc(smem_u32(&bars->tmem_base), 512);
@@ -259,7 +258,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       auto fetch_ex = [&](int tile) {
         const int key = tile * kKeyTile + row;
         if (kFp8 && key < lim_max) {
-          const int slot = key / a.c.page_size, at = key - slot * a.c.page_size;
+          const int slot = a.c.by_page(key), at = key - slot * a.c.page_size;
           const long long id = checked_page(a, b, slot);
 #pragma unroll
           for (int x = 0; x < 2; ++x) ex[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + h * a.c.exp_head[x]);
@@ -364,7 +363,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         int id = -1;
         auto fetch_page = [&](int tile) {
           const int key = tile * kKeyTile + lane * box_rows;
-          id = lane < n_boxes && key < lim_max ? checked_page(a, b, key / a.c.page_size) : -1;
+          id = lane < n_boxes && key < lim_max ? checked_page(a, b, a.c.by_page(key)) : -1;
         };
         fetch_page(t0);
         for (int it = 0; ok && it < n_tiles; ++it) {
@@ -389,7 +388,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
           }
           const int tile = t0 + it;
-          const int now = id, at = (tile * kKeyTile + lane * box_rows) % a.c.page_size;
+          const int now = id, key = tile * kKeyTile + lane * box_rows, at = key - a.c.by_page(key) * a.c.page_size;
           const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, now >= 0)) * box_bytes;
           if (it + 1 < n_tiles) fetch_page(tile + 1);
 #pragma unroll
@@ -706,8 +705,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           part[kTileRows * kCacheDim + r] = m_ref;
           part[kTileRows * kCacheDim + kTileRows + r] = l_sum;
         }
-        if (threadIdx.x == 0 && q->last_share >= 0)  // the item goes on in later shares: say where it ends
-          *reinterpret_cast<int4*>(a.desc + 4 * blockIdx.x) = make_int4(q->b, q->h, q->it, q->last_share);
       }
     }
   }

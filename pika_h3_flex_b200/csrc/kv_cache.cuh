@@ -19,6 +19,20 @@ namespace h3a {
 constexpr int kCacheDim = 128;
 constexpr int kBadCacheIndex = 10;  // status code: a page, a length or a row offset is outside its range (H3A_ERR_INDEX)
 
+// n / d for 0 <= n < 2^31 by one multiplication: m = ceil(2^(31 + s) / d), 2^(s - 1) < d <= 2^s
+struct FastDiv {
+  uint32_t m;
+  int shift;  // 31 + s
+  __host__ static FastDiv of(uint32_t d) {
+    int s = 0;
+    while ((1ull << s) < d) ++s;
+    return FastDiv{static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * m) >> shift);
+  }
+};
+
 struct CacheArgs {
   uint8_t* pool[2];                                           // K, V
   long long page_bytes[2], token_bytes[2], head_bytes[2];     // strides in bytes
@@ -29,6 +43,7 @@ struct CacheArgs {
   const int* lengths;
   const int* starts;
   int n_seqs, max_pages, n_pages, page_size, kv_heads;
+  FastDiv by_page;                                            // division by page_size
   int rows;                                                   // rows of the packed tensors
   int* status;
 };
@@ -122,7 +137,7 @@ __device__ __forceinline__ RowPlace place_of_row(const CacheArgs& a, int t) {
   const CacheSeq q = cache_seq(a, b);
   const int pos = q.len - q.n + (t - q.s0);
   if (pos < 0) return p;
-  const int slot = pos / a.page_size;
+  const int slot = a.by_page(pos);
   p.at = pos - slot * a.page_size;
   p.id = __ldg(a.pages + b * a.pages_stride + slot);
   if (static_cast<unsigned>(p.id) >= static_cast<unsigned>(a.n_pages)) {

@@ -81,6 +81,7 @@ int32_t cache_args(const h3a_cache* c, const h3a_cache_batch* b, int32_t* status
   a->max_pages = b->max_pages;
   a->n_pages = c->n_pages;
   a->page_size = c->page_size;
+  a->by_page = h3a::FastDiv::of(c->page_size);
   a->kv_heads = c->heads;
   a->rows = b->rows;
   a->status = status;
@@ -153,8 +154,8 @@ int32_t row_map(CUtensorMap* m, const void* ptr, bool codes, int n_outer, const 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? H3A_OK : H3A_ERR_LAUNCH;
 }
 
-constexpr int kTileMinShare = 4;
-constexpr int kFewMinShare = 3;  // units (a tile, or an item's set-up) below which a share is not worth a CTA
+// log2 of the units (a tile, or an item's set-up) below which a share is not worth a CTA
+constexpr int kTileShareShift = 2, kFewShareShift = 1;
 
 // What a call of this shape launches.
 struct AttnPlan {
@@ -177,7 +178,7 @@ AttnPlan attn_plan(const h3a_cache_attn_params* p, int sms) {
     n.shares = sms * (rows <= 8 ? (p->cache.quantised ? h3a::kFewBlocksPerSm<true, 1> : h3a::kFewBlocksPerSm<false, 1>)
                                 : (p->cache.quantised ? h3a::kFewBlocksPerSm<true, 2> : h3a::kFewBlocksPerSm<false, 2>));
   }
-  n.bytes = static_cast<size_t>(n.shares) * (4 * sizeof(int) + 2ull * n.item_rows * (h3a::kCacheDim + 2) * sizeof(float));
+  n.bytes = static_cast<size_t>(n.shares) * (h3a::kDescInts * sizeof(int) + 2ull * n.item_rows * (h3a::kCacheDim + 2) * sizeof(float));
   return n;
 }
 
@@ -234,7 +235,8 @@ int32_t launch_join(const h3a::CacheAttnArgs& a, int shares, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, h3a::cache_attn_join_kernel, a) == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
+  const auto kernel = a.item_tokens > 0 ? h3a::cache_attn_join_kernel<4> : h3a::cache_attn_join_kernel<16>;
+  return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -293,8 +295,11 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   a.key_shift = n.key_shift;
   a.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / std::sqrt(128.0f)) * 1.4426950408889634f;
   a.desc = static_cast<int*>(p->workspace);
-  a.part = reinterpret_cast<float*>(a.desc + 4 * n.shares);
-  a.min_share = n.item_tokens > 0 ? kTileMinShare : kFewMinShare;
+  a.part = reinterpret_cast<float*>(a.desc + h3a::kDescInts * n.shares);
+  a.share_shift = n.item_tokens > 0 ? kTileShareShift : kFewShareShift;
+  a.by_group = h3a::FastDiv::of(a.group);
+  a.by_item_rows = h3a::FastDiv::of(n.item_rows);
+  a.by_item_tokens = h3a::FastDiv::of(std::max(1, n.item_tokens));
   a.wait_ns = p->wait_limit_ns > 0 ? p->wait_limit_ns : 2000000000ll;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (n.item_tokens > 0)
