@@ -251,6 +251,25 @@ __device__ __forceinline__ int checked_page(const CacheAttnArgs& a, int b, int s
   return id;
 }
 
+// the e4m3 codes in bytes 0 and 1 of w as fp16
+__device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_high_to_f16x2(uint32_t w) {  // bytes 2 and 3
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 2^e, within the range of normal numbers
+__device__ __forceinline__ float pow2_float(int e) { return __uint_as_float(static_cast<uint32_t>(max(-126, min(e, 127)) + 127) << 23); }
+
 __device__ __forceinline__ bool non_finite2(uint32_t w) {
   return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
 }
@@ -290,7 +309,7 @@ __device__ __forceinline__ void describe_join(const CacheAttnArgs& a, const Shar
   d[4] = h;
 }
 
-// Block (share, y): rows [4 y, 4 y + 4) of the item that begins in the share and ends in a later one.  The kernel is a few
+// Block (share, y): rows 4 y + [0, 4), and so on, of the item that begins in the share and ends in a later one.  The kernel is a few
 // dependent loads long, so its launch overlaps the kernel before it, everything it has to know about the item is in the
 // description, and the loads of kJoinParts parts' O wait for nothing else: with the parts one after the other a row of 37
 // parts took 29 us.  16 at a time for small items (up to as many parts as shares), 4 for large ones (two or three, and
@@ -303,54 +322,55 @@ __global__ void __launch_bounds__(kJoinRows * 32) cache_attn_join_kernel(const _
   const int kv_head = a.desc[kDescInts * share + 4];
   if (a.c.status && *reinterpret_cast<volatile int*>(a.c.status) != 0) return;
   const int lane = threadIdx.x & 31;
-  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
   const int n_parts = d.x, n_rows = d.y, r0 = d.z;
-  if (n_parts <= 0 || r >= n_rows) return;
+  if (n_parts <= 0) return;
   // parts of the row: the tail slot of this share, then the head slots of the next ones
   const long long slot = 2ll * a.item_rows * (kCacheDim + 2);
   const float* first = part_slot(a, share, true);
   const float* next = part_slot(a, share, false);  // + i slots for part i > 0
-  float m = kNoMax, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n_parts; i0 += kJoinParts) {
-    const int n = min(kJoinParts, n_parts - i0);
-    float4 v[kJoinParts];
+  for (int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5); r < n_rows; r += kJoinRows * gridDim.y) {
+    float m = kNoMax, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n_parts; i0 += kJoinParts) {
+      const int n = min(kJoinParts, n_parts - i0);
+      float4 v[kJoinParts];
 #pragma unroll
-    for (int i = 0; i < kJoinParts; ++i)
-      if (i < n) v[i] = *reinterpret_cast<const float4*>((i0 + i == 0 ? first : next + (i0 + i) * slot) + r * kCacheDim + 4 * lane);
-    float mi = kNoMax, li = 0.f;
-    if (lane < n) {
-      const float* st = (i0 + lane == 0 ? first : next + (i0 + lane) * slot) + a.item_rows * kCacheDim + r;
-      mi = st[0];
-      li = st[a.item_rows];
-    }
-    float top = mi;
-#pragma unroll
-    for (int o = kJoinParts / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    top = __shfl_sync(0xFFFFFFFFu, top, 0);
-    const float m_new = fmaxf(m, top), f = ex2_approx(m - m_new), wi = ex2_approx(mi - m_new);
-    m = m_new;
-    l *= f;
-    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-#pragma unroll
-    for (int i = 0; i < kJoinParts; ++i)
-      if (i < n) {
-        const float w = __shfl_sync(0xFFFFFFFFu, wi, i);
-        l += w * __shfl_sync(0xFFFFFFFFu, li, i);
-        acc.x += v[i].x * w;
-        acc.y += v[i].y * w;
-        acc.z += v[i].z * w;
-        acc.w += v[i].w * w;
+      for (int i = 0; i < kJoinParts; ++i)
+        if (i < n) v[i] = *reinterpret_cast<const float4*>((i0 + i == 0 ? first : next + (i0 + i) * slot) + r * kCacheDim + 4 * lane);
+      float mi = kNoMax, li = 0.f;
+      if (lane < n) {
+        const float* st = (i0 + lane == 0 ? first : next + (i0 + lane) * slot) + a.item_rows * kCacheDim + r;
+        mi = st[0];
+        li = st[a.item_rows];
       }
+      float top = mi;
+#pragma unroll
+      for (int o = kJoinParts / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      top = __shfl_sync(0xFFFFFFFFu, top, 0);
+      const float m_new = fmaxf(m, top), f = ex2_approx(m - m_new), wi = ex2_approx(mi - m_new);
+      m = m_new;
+      l *= f;
+      acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+      for (int i = 0; i < kJoinParts; ++i)
+        if (i < n) {
+          const float w = __shfl_sync(0xFFFFFFFFu, wi, i);
+          l += w * __shfl_sync(0xFFFFFFFFu, li, i);
+          acc.x += v[i].x * w;
+          acc.y += v[i].y * w;
+          acc.z += v[i].z * w;
+          acc.w += v[i].w * w;
+        }
+    }
+    const int row = r0 + r, i = a.by_group(row), token = d.w + i, head = kv_head * a.group + row - i * a.group;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint2 w;
+    w.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+    w.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(a.o + token * a.o_stride_l + head * a.o_stride_h + 4 * lane) = w;
+    if (a.lse && lane == 0)
+      a.lse[static_cast<long long>(head) * a.c.rows + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
-  const int row = r0 + r, i = a.by_group(row), token = d.w + i, head = kv_head * a.group + row - i * a.group;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  uint2 w;
-  w.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-  w.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(a.o + token * a.o_stride_l + head * a.o_stride_h + 4 * lane) = w;
-  if (a.lse && lane == 0)
-    a.lse[static_cast<long long>(head) * a.c.rows + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 }  // namespace h3a

@@ -56,22 +56,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// the e4m3 codes in bytes 0 and 1 of w as fp16
-__device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
-  return r;
-}
-__device__ __forceinline__ uint32_t e4m3_high_to_f16x2(uint32_t w) {  // bytes 2 and 3
-  uint32_t r;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 // transposes an 8 x 8 matrix of 16-bit values held as an MMA fragment
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
   uint32_t r;
@@ -79,7 +63,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
   return r;
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-__device__ __forceinline__ float pow2_float(int e) { return __uint_as_float(static_cast<uint32_t>(max(-126, min(e, 127)) + 127) << 23); }
 
 template <bool kFp8, int kNT>
 __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cache_attn_few_kernel(const __grid_constant__ CacheAttnArgs a) {

@@ -9,11 +9,18 @@
 //   warp 11          cuts the share into pieces and hands them to the others through a small ring: the bookkeeping would
 //                    cost every role some 40 registers (with each role walking the share on its own the softmax warps
 //                    spilled 1.4 KB and the kernel ran at half the speed)
-//   warps 12-15      helpers, one cache row per thread.  e4m3: widen a staged tile to bf16 (exact, the row's power of two
-//                    included) into the ring.  bf16: let tiles through, except the V tiles that not every row sees whole:
-//                    P is 0 for a key a row does not see, and 0 x NaN is NaN, so rows behind the last key become zeros
-//                    and values that are not finite become zeros until the epilogue puts them back for the rows that
-//                    do see them.
+//   warps 12-15      helpers, one cache row per thread.  e4m3: widen a staged tile into the ring (below).  bf16: let tiles
+//                    through, except the V tiles that not every row sees whole: P is 0 for a key a row does not see, and
+//                    0 x NaN is NaN, so rows behind the last key become zeros and values that are not finite become zeros
+//                    until the epilogue puts them back for the rows that do see them.
+// e4m3 tiles become fp16, two instructions per pair: a code is exact in fp16 (one conversion), and so is its product with
+// 2^(k - kref), kref being the tile's largest exponent, down to k - kref = -15 (below that a row's logits are off by less
+// than 2^-30 of the tile's largest).  2^kref goes into the tile's softmax scale, and Q into fp16 by a power of two per row
+// that joins that scale too.  V is kept relative to the running maximum of the tiles' exponents, in whose units O
+// accumulates (a rise rescales O like a rise of the row maximum), and P is held as 2^7 p: terms down to 2^-31 of the
+// row's largest count.  A V tile with rows more than 2^14 below that maximum is widened to bf16 instead, and its P
+// rounded to bf16, so that no row's own precision is lost.  (Everything through bf16 took five instructions per pair: the
+// helpers then set the pace at 500 TFLOP/s.)
 // Each 128-key tile is processed as two 64-key halves with S buffers of their own, so that a stream has two S / P buffers
 // in flight, as in the dense kernels.  TMEM: stream t: S/P buffer h at columns [128 t + 64 h, +64), O at [256 + 128 t, +128).
 //
@@ -46,9 +53,11 @@ struct TileBars {
   uint64_t staged[4];      // e4m3: copies have landed
   uint64_t unstaged[4];    // e4m3: widened
   uint64_t q_full, q_empty;
+  uint64_t q_ready[2];     // e4m3: the stream's Q is in fp16
   uint64_t s_full[2][2], p_full[2][2], o_full[2][2];  // [stream][half]
   uint64_t o_free[2];
   uint64_t piece_full[4], piece_empty[4];
+  uint64_t tops[2];        // e4m3: the helper warps' exponents of a tile are there
   uint32_t tmem_base;
   uint32_t early_exit;
   volatile uint32_t abort_flag;
@@ -58,7 +67,7 @@ constexpr int kTileSmemBytes = 2 * kTileBytes + TileRing<false>::kBytes + 1024 +
 static_assert(TileRing<true>::kBytes <= TileRing<false>::kBytes && sizeof(TileBars) <= 512, "shared memory layout");
 enum : int {  // status codes of waits that ran out (low byte of the status word)
   kTileWaitEmpty = 33, kTileWaitFull, kTileWaitReady, kTileWaitUnstaged, kTileWaitStaged, kTileWaitQFull, kTileWaitQEmpty,
-  kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitPiece
+  kTileWaitQReady, kTileWaitTops, kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitPiece
 };
 
 struct TileWait {
@@ -121,6 +130,28 @@ __device__ __forceinline__ void reg_fence16(uint32_t (&r)[16]) {
                : "memory");
 }
 
+// 8 x 8 transpose of 16-byte pieces among 8 neighbouring lanes: in, lane s has pieces 0 .. 7 of row s; out, lane s has piece
+// s of rows 0 .. 7.  A thread owns a row of O, and written as it is a warp's store would be 32 pieces of 16 bytes, 256 bytes
+// apart: 5 us per 256 rows, as long as two and a half key tiles.  Transposed, an instruction writes 4 runs of 128 bytes.
+__device__ __forceinline__ void transpose_pieces(uint32_t* r) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int b = 1; b < 8; b <<= 1) {
+    const bool up = (lane & b) != 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if ((k & b) == 0) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t &lo = r[4 * k + w], &hi = r[4 * (k | b) + w];
+          const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, up ? lo : hi, b);
+          if (up) lo = got;
+          else hi = got;
+        }
+      }
+  }
+}
+
 // A piece as the roles see it.
 struct TilePiece {
   int n_tiles;       // key tiles [t0, t0 + n_tiles)
@@ -133,6 +164,23 @@ struct TilePiece {
   int whole;         // the piece is the whole item; otherwise its results are partial
   int tail;          // ... and go to the share's tail slot (the item begins here)
 };
+// e4m3: what a tile's rows were widened with
+struct TileInfo {
+  float k_unit;   // 2^(kref - 127): the tile's logits are in these units
+  int vref;       // its V is in units of 2^(vref - 127)
+  int wide;       // V is bf16, and P is to be
+};
+constexpr int kInfoRing = 8;  // the helpers are at most two tiles ahead of the softmax warps
+// 2^-d as an fp16 pair
+__device__ __forceinline__ uint32_t f16x2_pow2_neg(int d) {
+  const uint32_t h = d <= 14 ? static_cast<uint32_t>(15 - d) << 10 : d <= 24 ? 1u << (24 - d) : 0u;
+  return h * 0x10001u;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 constexpr int kPieceRing = 4;
 constexpr int kPieceReaders = 15;  // warps
 
@@ -172,7 +220,9 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   extern __shared__ uint8_t smem_raw[];
   __shared__ ShareStart start;
   __shared__ TilePiece pieces[kPieceRing];  // n_tiles < 0: no more
-  static_assert(kTileSmemBytes + sizeof(ShareStart) + sizeof(TilePiece) * kPieceRing <= 232448, "shared memory budget");
+  __shared__ TileInfo info[kInfoRing];
+  __shared__ uint32_t tops[2][4];           // e4m3: exponents' maxima and minimum of a tile, per helper warp, by tile parity
+  static_assert(kTileSmemBytes + sizeof(ShareStart) + sizeof(TilePiece) * kPieceRing + sizeof(TileInfo) * kInfoRing + 32 <= 232448, "shared memory budget");
   using R = TileRing<kFp8>;
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -193,7 +243,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     }
     mbar_init(smem_u32(&bars->q_full), 1);
     mbar_init(smem_u32(&bars->q_empty), 2);
+    mbar_init(smem_u32(&bars->tops[0]), 4);
+    mbar_init(smem_u32(&bars->tops[1]), 4);
     for (int t = 0; t < 2; ++t) {
+      mbar_init(smem_u32(&bars->q_ready[t]), 4);
       for (int hf = 0; hf < 2; ++hf) {
         mbar_init(smem_u32(&bars->s_full[t][hf]), 1);
         mbar_init(smem_u32(&bars->p_full[t][hf]), 128);
@@ -249,27 +302,89 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int row = threadIdx.x - 384;
     const uint32_t swz = row & 7;
     int cnt = 0;
+    uint32_t n_done = 0;  // tiles so far, all pieces
     bool ok = true;
     const TilePiece* q;
     for (; ok && (q = piece()) != nullptr; piece_done()) {
       const int n_tiles = q->n_tiles, t0 = q->t0, b = q->b, h = q->h, lim_min = q->lim_min, lim_max = q->lim_max;
       if (n_tiles == 0) continue;
-      uint32_t ex[2] = {0, 0};  // e4m3: exponent bytes of this thread's row of the tile to come
+      // e4m3: the exponent bytes of this thread's row are fetched a tile ahead, their page number two tiles ahead
+      uint32_t ex[2] = {0, 0};
+      int id_next = 0;
+      uint32_t vref = 0;
+      auto fetch_id = [&](int tile) {
+        const int key = tile * kKeyTile + row;
+        if (kFp8 && key < lim_max) id_next = __ldg(a.c.pages + b * a.c.pages_stride + a.c.by_page(key));
+      };
       auto fetch_ex = [&](int tile) {
         const int key = tile * kKeyTile + row;
         if (kFp8 && key < lim_max) {
-          const int slot = a.c.by_page(key), at = key - slot * a.c.page_size;
-          const long long id = checked_page(a, b, slot);
+          const int at = key - a.c.by_page(key) * a.c.page_size;
+          long long id = id_next;
+          if (static_cast<unsigned>(id_next) >= static_cast<unsigned>(a.c.n_pages)) {
+            report_cache(a.c, b);
+            id = 0;
+          }
 #pragma unroll
           for (int x = 0; x < 2; ++x) ex[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + h * a.c.exp_head[x]);
         }
       };
+      fetch_id(t0);
       fetch_ex(t0);
+      fetch_id(t0 + 1);
       for (int it = 0; ok && it < n_tiles; ++it) {
         const int tile = t0 + it, key = tile * kKeyTile + row;
         const bool special = (tile + 1) * kKeyTile > lim_min;
-        const uint32_t e_now[2] = {ex[0], ex[1]};
-        if (it + 1 < n_tiles) fetch_ex(tile + 1);
+        const bool gone = key >= lim_max;
+        uint32_t factor[2] = {0, 0};  // e4m3: of this thread's row of K and V
+        bool blank[2] = {gone, gone}; // e4m3: ... which may hold anything, codes for NaN included, and counts as zeros
+        bool wide = false;
+        if constexpr (kFp8) {
+          // the tile's largest exponents, and V's smallest; rows of nothing (7) and rows that are not finite (255) aside
+          const uint32_t ek = ex[0], ev = ex[1];
+          if (it + 1 < n_tiles) fetch_ex(tile + 1);
+          fetch_id(tile + 2);
+          const uint32_t k_top = __reduce_max_sync(0xFFFFFFFFu, !gone && ek != 255u ? ek : 0u);
+          const uint32_t v_top = __reduce_max_sync(0xFFFFFFFFu, !gone && ev != 255u ? ev : 0u);
+          const uint32_t v_low = __reduce_min_sync(0xFFFFFFFFu, !gone && ev != 255u && ev > 7u ? ev : 255u);
+          const uint32_t par = n_done & 1;
+          if (lane == 0) {
+            tops[par][warp - 12] = k_top | (v_top << 8) | (v_low << 16);
+            mbar_arrive(smem_u32(&bars->tops[par]));
+          }
+          ok = wait(bars->tops[par], (n_done >> 1) & 1, kTileWaitTops);  // a bounded meeting: a named barrier would not be
+          if (!ok) break;
+          uint32_t kt = 0, vt = 0, vl = 255;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t x = tops[par][w];
+            kt = max(kt, x & 255u);
+            vt = max(vt, (x >> 8) & 255u);
+            vl = min(vl, x >> 16);
+          }
+          vref = max(vref, vt);
+          wide = vl + 14u < vref;
+          if (row == 0) {
+            TileInfo& to = info[n_done % kInfoRing];
+            to.k_unit = __uint_as_float(kt << 23);
+            to.vref = static_cast<int>(vref);
+            to.wide = wide;
+          }
+          factor[0] = ek == 255u ? 0x7FFF7FFFu : f16x2_pow2_neg(static_cast<int>(kt) - static_cast<int>(ek));
+          if (ev == 255u) {
+            factor[1] = 0x7FFF7FFFu;
+            if (special && !gone) {  // put back at the end
+              blank[1] = true;
+              bars->poison = 1u;
+            }
+          } else {
+            factor[1] = wide ? static_cast<uint32_t>(247 + static_cast<int>(ev) - static_cast<int>(vref)) * 0x800080u
+                             : f16x2_pow2_neg(static_cast<int>(vref) - static_cast<int>(ev));
+          }
+          if (blank[0]) factor[0] = 0;
+          if (blank[1]) factor[1] = 0;
+          ++n_done;
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x, ++cnt) {  // K, then V
           const int s = cnt % R::kRing;
@@ -280,33 +395,31 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             ok = wait(bars->staged[g], (cnt / R::kStaged) & 1, kTileWaitStaged) && wait(bars->empty[s], ph ^ 1u, kTileWaitEmpty);
             if (!ok) break;
             const uint32_t src = staging + g * kCodeBytes + row * 128;
-            uint32_t f = e4m3_factor(e_now[x]) * 0x10001u;
-            const uint32_t f2 = e4m3_factor2(e_now[x]) * 0x10001u;
-            if (key >= lim_max) {
-              f = 0;
-            } else if (x == 1 && special && e_now[x] == 255u) {
-              f = 0;
-              bars->poison = 1u;
-            }
-            const bool two = __any_sync(0xFFFFFFFFu, e_now[x] > kOneStepExp);
+            const uint32_t f = factor[x];
+            if (x == 1 && wide) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              uint4 w;
-              ld_shared_v4(src + ((c ^ swz) << 4), w);
-              const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-              uint32_t o[8];
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                o[2 * y] = mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x1404)), f);
-                o[2 * y + 1] = mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x3424)), f);
+              for (int c = 0; c < 8; ++c) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (!blank[x]) ld_shared_v4(src + ((c ^ swz) << 4), w);
+                const uint32_t at = dst + (c >> 2) * kTileHalf;
+                st_shared_v4(at + (((2 * (c & 3)) ^ swz) << 4), mul_bf16x2(e4m3_pattern(__byte_perm(w.x, 0, 0x1404)), f),
+                             mul_bf16x2(e4m3_pattern(__byte_perm(w.x, 0, 0x3424)), f), mul_bf16x2(e4m3_pattern(__byte_perm(w.y, 0, 0x1404)), f),
+                             mul_bf16x2(e4m3_pattern(__byte_perm(w.y, 0, 0x3424)), f));
+                st_shared_v4(at + (((2 * (c & 3) + 1) ^ swz) << 4), mul_bf16x2(e4m3_pattern(__byte_perm(w.z, 0, 0x1404)), f),
+                             mul_bf16x2(e4m3_pattern(__byte_perm(w.z, 0, 0x3424)), f), mul_bf16x2(e4m3_pattern(__byte_perm(w.w, 0, 0x1404)), f),
+                             mul_bf16x2(e4m3_pattern(__byte_perm(w.w, 0, 0x3424)), f));
               }
-              if (two) {
+            } else {
 #pragma unroll
-                for (int y = 0; y < 8; ++y) o[y] = mul_bf16x2(o[y], f2);
+              for (int c = 0; c < 8; ++c) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (!blank[x]) ld_shared_v4(src + ((c ^ swz) << 4), w);
+                const uint32_t at = dst + (c >> 2) * kTileHalf;
+                st_shared_v4(at + (((2 * (c & 3)) ^ swz) << 4), mul_f16x2(e4m3_to_f16x2(w.x), f), mul_f16x2(e4m3_high_to_f16x2(w.x), f),
+                             mul_f16x2(e4m3_to_f16x2(w.y), f), mul_f16x2(e4m3_high_to_f16x2(w.y), f));
+                st_shared_v4(at + (((2 * (c & 3) + 1) ^ swz) << 4), mul_f16x2(e4m3_to_f16x2(w.z), f), mul_f16x2(e4m3_high_to_f16x2(w.z), f),
+                             mul_f16x2(e4m3_to_f16x2(w.w), f), mul_f16x2(e4m3_high_to_f16x2(w.w), f));
               }
-              const uint32_t at = dst + (c >> 2) * kTileHalf;
-              st_shared_v4(at + (((2 * (c & 3)) ^ swz) << 4), o[0], o[1], o[2], o[3]);
-              st_shared_v4(at + (((2 * (c & 3) + 1) ^ swz) << 4), o[4], o[5], o[6], o[7]);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -318,7 +431,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             ok = wait(bars->full[s], ph, kTileWaitFull);
             if (!ok) break;
             if (x == 1 && special) {
-              const bool gone = key >= lim_max;
               bool bad = false;
 #pragma unroll 4
               for (int c = 0; c < 16; ++c) {
@@ -422,8 +534,9 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       // ========================================================= issuers, one warp per stream
       const int t = warp - 9;
       const uint32_t leader = elect_one();
-      constexpr uint32_t idesc_s = umma_idesc(UMMA_FMT_BF16, UMMA_FMT_BF16, 0, 0, 128, 64);
-      constexpr uint32_t idesc_pv = umma_idesc(UMMA_FMT_BF16, UMMA_FMT_BF16, 0, 1, 128, 128);
+      constexpr uint32_t kFmt = kFp8 ? UMMA_FMT_F16 : UMMA_FMT_BF16;
+      constexpr uint32_t idesc_s = umma_idesc(kFmt, kFmt, 0, 0, 128, 64);
+      constexpr uint32_t idesc_pv = umma_idesc(kFmt, kFmt, 0, 1, 128, 128), idesc_pv_wide = umma_idesc(UMMA_FMT_BF16, UMMA_FMT_BF16, 0, 1, 128, 128);
       const uint64_t q_desc = umma_desc_sw128(q_smem + t * kTileBytes, 16, 1024);
       const uint64_t k_desc0 = umma_desc_sw128(ring, 16, 1024);
       const uint64_t v_desc0 = umma_desc_sw128(ring, kTileHalf, 1024);
@@ -443,11 +556,11 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         umma_commit_if(leader, smem_u32(&bars->s_full[t][hf]));
       };
-      auto issue_pv = [&](int hf, int s) {
+      auto issue_pv = [&](int hf, int s, uint32_t idesc) {
         const uint64_t vd = v_desc0 + static_cast<uint64_t>((s * kTileBytes + hf * 8192) >> 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_bf16_ts_if(leader, o_tmem, s_tmem + hf * 64 + k * 8, vd + (k * 2048 >> 4), idesc_pv, (pv_cnt > 0 || k > 0) ? 1u : 0u);
+          umma_bf16_ts_if(leader, o_tmem, s_tmem + hf * 64 + k * 8, vd + (k * 2048 >> 4), idesc, (pv_cnt > 0 || k > 0) ? 1u : 0u);
         ++pv_cnt;
         umma_commit_if(leader, smem_u32(&bars->o_full[t][hf]));
       };
@@ -460,7 +573,9 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       for (; ok && (q = piece()) != nullptr; piece_done()) {
         const int n_tiles = q->n_tiles, n_mine = q->end[t];
         if (n_tiles == 0) continue;
-        ok = wait(bars->q_full, g & 1, kTileWaitQFull) && ready(c0);
+        if (!kFp8) ok = wait(bars->q_full, g & 1, kTileWaitQFull);
+        else if (n_mine > 0) ok = wait(bars->q_ready[t], own & 1, kTileWaitQReady);
+        ok = ok && ready(c0);
         if (!ok) break;
         pv_cnt = 0;
         if (n_mine > 0) {
@@ -484,7 +599,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               if (ok) {
                 ++p_cnt[hf];
                 tc_fence_after_sync();
-                issue_pv(hf, cv % R::kRing);
+                issue_pv(hf, cv % R::kRing, kFp8 && info[((c0 >> 1) + it) % kInfoRing].wide ? idesc_pv_wide : idesc_pv);
               }
             }
             if (ok && has_next && !k_ready) {
@@ -523,6 +638,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lane_base + t * 128, o_addr = tmem + lane_base + 256 + t * 128;
     uint32_t j = 0;  // key tiles the stream has processed: the phase of s_full / o_full
+    uint32_t g = 0;  // e4m3: pieces with work so far, the phase of q_full; their tiles
+    uint32_t n_before = 0;
     bool ok = true;
     uint32_t ra[64], rb[64];
     auto load_s = [&](uint32_t (&r)[64], int hf) {
@@ -554,6 +671,47 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const int lim = (have_row ? piece_limit(a, *q, q->tok0 + row_token) : 0) - q->t0 * kKeyTile;  // counted from tile t0
       const int lim_first = piece_limit(a, *q, q->tok0 + t * T) - q->t0 * kKeyTile;  // the stream's first row sees fewest keys
       float m_ref = kNoMax, l_sum = 0.f;
+      float row_unit = a.scale_log2;  // from S to logits in log2
+      float c = row_unit;             // ... of the current tile
+      int vref = 0;                   // e4m3: O is in units of 2^(vref - 127)
+      bool wide = false;
+      const uint32_t tile0 = n_before;
+      if constexpr (kFp8) {
+        n_before += q->n_tiles;
+        if (q->n_tiles > 0) {
+          ok = wait(bars->q_full, g & 1, kTileWaitQFull);  // every piece's: a phase must not be skipped
+          if (!ok) break;
+          if (n_mine > 0) {
+            // the thread's row of Q into fp16, in place: the row's largest becomes 2^4 .. 2^5
+            const uint32_t src = q_smem + t * kTileBytes + row * 128, swz = row & 7;
+            uint32_t m = 0;
+#pragma unroll 4
+            for (int x = 0; x < 16; ++x) {
+              uint4 w;
+              ld_shared_v4(src + (x >> 3) * kTileHalf + (((x & 7) ^ swz) << 4), w);
+              m = __vmaxu2(m, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+            }
+            const int e = max(static_cast<int>(max(m >> 16, m & 0xFFFFu) >> 7) - 127 - 4, -120);
+            const float f = pow2_float(-e);
+            row_unit *= pow2_float(e);
+#pragma unroll 4
+            for (int x = 0; x < 16; ++x) {
+              const uint32_t at = src + (x >> 3) * kTileHalf + (((x & 7) ^ swz) << 4);
+              uint4 w;
+              ld_shared_v4(at, w);
+              const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+              uint32_t o[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) o[z] = pack_f16x2(__uint_as_float(in[z] << 16) * f, __uint_as_float(in[z] & 0xFFFF0000u) * f);
+              st_shared_v4(at, o[0], o[1], o[2], o[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars->q_ready[t]));
+          }
+          ++g;
+        }
+      }
 
       auto softmax_half = [&](uint32_t (&s)[64], int hf, int it) -> bool {
         const int key0 = it * kKeyTile + hf * 64;
@@ -576,14 +734,24 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         mx0 = fmax3(mx0, __uint_as_float(s[60]), __uint_as_float(s[61]));
         mx1 = fmax3(mx1, __uint_as_float(s[62]), __uint_as_float(s[63]));
-        const float m_tile = fmax3(fmaxf(mx0, mx1), mx2, mx3) * a.scale_log2;
+        // the largest term is 2^kLift at first, and 2^(kLift + 8) before the reference moves
+        constexpr float kLift = kFp8 ? 7.f : 0.f;
+        const float m_tile = fmax3(fmaxf(mx0, mx1), mx2, mx3) * c - kLift;
+        int v_shift = 0;
+        if (kFp8 && hf == 0) {
+          const TileInfo& in = info[(tile0 + it) % kInfoRing];
+          wide = in.wide != 0;
+          v_shift = it == 0 ? 0 : vref - in.vref;
+          vref = in.vref;
+        }
         if (it == 0 && hf == 0) {
           m_ref = fmaxf(m_tile, kNoMax);
-        } else if (__any_sync(0xFFFFFFFFu, m_tile - m_ref > 8.0f)) {
+        } else if (__any_sync(0xFFFFFFFFu, m_tile - m_ref > 8.0f) || v_shift != 0) {
           const float m_new = fmaxf(m_ref, m_tile);
-          const float alpha = ex2_approx(m_ref - m_new);
+          float alpha = ex2_approx(m_ref - m_new);
           m_ref = m_new;
           l_sum *= alpha;
+          if constexpr (kFp8) alpha *= pow2_float(v_shift);
           // the stream's previous P V must be complete; MMAs complete in issue order, so it is the only one that can run
           if (!wait(bars->o_full[t][hf ^ 1], (hf ? j : j - 1) & 1, kTileWaitO)) return false;
           tc_fence_after_sync();
@@ -598,9 +766,9 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             tmem_st16(o_addr + 16 * i, o);
           }
         }
-        // P = 2^(s c - m), rounded to bf16 once; the row sum keeps the unrounded terms
+        // P = 2^(s c - m), rounded once; the row sum keeps the unrounded terms
         uint64_t acc0 = 0, acc1 = 0;
-        const uint64_t c2 = pack2(a.scale_log2, a.scale_log2), nm2 = pack2(-m_ref, -m_ref);
+        const uint64_t c2 = pack2(c, c), nm2 = pack2(-m_ref, -m_ref);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           float x0, x1;
@@ -608,7 +776,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
           if (i & 1) acc1 = add2(acc1, pack2(p0, p1));
           else acc0 = add2(acc0, pack2(p0, p1));
-          s[i] = pack_bf16x2(p0, p1);
+          s[i] = kFp8 && !wide ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
         }
         float a0, a1, a2, a3;
         unpack2(acc0, a0, a1);
@@ -622,6 +790,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         tmem_wait_ld();
         reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[0]));
         reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[32]));
+        if constexpr (kFp8) c = fminf(row_unit * info[(tile0 + it) % kInfoRing].k_unit, 3.0e38f);
         ok = softmax_half(ra, 0, it);
         if (!ok) break;
         const bool early1 = try_fetch_s(rb, 1, j);
@@ -674,36 +843,54 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           }
       };
       const bool poisoned = bars->poison != 0u;
-      if (q->whole) {
-        if (have_row) {
-          const float inv = l_sum == 0.f ? 0.f : 1.0f / l_sum;
-          __nv_bfloat16* dst = a.o + out_row * a.o_stride_l + head * a.o_stride_h;
+      // where this thread's row goes (null: nowhere), as bytes; 8 lanes write a row together
+      uint8_t* dst = nullptr;
+      if (have_row)
+        dst = q->whole ? reinterpret_cast<uint8_t*>(a.o + out_row * a.o_stride_l + head * a.o_stride_h)
+                       : reinterpret_cast<uint8_t*>(part_slot(a, blockIdx.x, q->tail != 0) + (t * T * a.group + row) * kCacheDim);
+      auto store_pieces = [&](uint32_t* r, int offset) {
+        transpose_pieces(r);
 #pragma unroll
-          for (int x = 0; x < 128; x += 8) {
-            const uint32_t* o = x < 64 ? &ra[x] : &rb[x - 64];
-            uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(o[0]) * inv, __uint_as_float(o[1]) * inv);
-            w.y = pack_bf16x2(__uint_as_float(o[2]) * inv, __uint_as_float(o[3]) * inv);
-            w.z = pack_bf16x2(__uint_as_float(o[4]) * inv, __uint_as_float(o[5]) * inv);
-            w.w = pack_bf16x2(__uint_as_float(o[6]) * inv, __uint_as_float(o[7]) * inv);
-            *reinterpret_cast<uint4*>(dst + x) = w;
-          }
-          if (poisoned) put_back(dst);
-          if (a.lse)
-            a.lse[static_cast<long long>(head) * a.c.rows + out_row] = l_sum == 0.f ? -INFINITY : (m_ref + log2f(l_sum)) * 0.6931471805599453f;
+        for (int k = 0; k < 8; ++k) {
+          uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(dst), (lane & 24) + k));
+          if (to != nullptr) *reinterpret_cast<uint4*>(to + offset + 16 * (lane & 7)) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
         }
-      } else {
-        if (have_row) {
-          float* part = part_slot(a, blockIdx.x, q->tail != 0);
-          const int r = t * T * a.group + row;
+      };
+      const float v_unit = kFp8 ? __uint_as_float(static_cast<uint32_t>(vref) << 23) : 1.0f;
+      if (q->whole) {
+        const float inv = (l_sum == 0.f ? 0.f : 1.0f / l_sum) * v_unit;
 #pragma unroll
-          for (int x = 0; x < 128; x += 4) {
-            const uint32_t* o = x < 64 ? &ra[x] : &rb[x - 64];
-            *reinterpret_cast<uint4*>(part + r * kCacheDim + x) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int i = 0; i < 32; ++i) {
+          ra[i] = pack_bf16x2(__uint_as_float(ra[2 * i]) * inv, __uint_as_float(ra[2 * i + 1]) * inv);
+          rb[i] = pack_bf16x2(__uint_as_float(rb[2 * i]) * inv, __uint_as_float(rb[2 * i + 1]) * inv);
+        }
+        store_pieces(ra, 0);
+        store_pieces(rb, 128);
+        if (have_row && a.lse)
+          a.lse[static_cast<long long>(head) * a.c.rows + out_row] = l_sum == 0.f ? -INFINITY : (m_ref + log2f(l_sum)) * 0.6931471805599453f;
+      } else {
+        if constexpr (kFp8) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            ra[i] = __float_as_uint(__uint_as_float(ra[i]) * v_unit);
+            rb[i] = __float_as_uint(__uint_as_float(rb[i]) * v_unit);
           }
-          if (poisoned) put_back(part + r * kCacheDim);
-          part[kTileRows * kCacheDim + r] = m_ref;
-          part[kTileRows * kCacheDim + kTileRows + r] = l_sum;
+        }
+        store_pieces(ra, 0);
+        store_pieces(ra + 32, 128);
+        store_pieces(rb, 256);
+        store_pieces(rb + 32, 384);
+        if (have_row) {
+          float* stat = part_slot(a, blockIdx.x, q->tail != 0) + kTileRows * kCacheDim + t * T * a.group + row;
+          stat[0] = m_ref;
+          stat[kTileRows] = l_sum;
+        }
+      }
+      if (poisoned) {
+        __syncwarp();  // the row was stored by its neighbours
+        if (have_row) {
+          if (q->whole) put_back(reinterpret_cast<__nv_bfloat16*>(dst));
+          else put_back(reinterpret_cast<float*>(dst));
         }
       }
     }

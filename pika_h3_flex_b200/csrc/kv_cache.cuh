@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kRowThreads) cache_rows_kernel(const __grid_co
               lo = fminf(fmaxf(lo, -240.f), 240.f);
               hi = fminf(fmaxf(hi, -240.f), 240.f);
             }
-            c[z] = cvt_e4m3x2(lo, hi);
+            c[z] = e[i] == 255u ? 0u : cvt_e4m3x2(lo, hi);  // a row that is not finite has no codes, only its byte
           }
           *reinterpret_cast<uint2*>(cached_row(y)) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
           if (lane == 0) {

@@ -227,7 +227,8 @@ int32_t launch_tile(const h3a_cache_attn_params* p, const h3a::CacheAttnArgs& a,
 
 int32_t launch_join(const h3a::CacheAttnArgs& a, int shares, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(shares, (a.item_rows + h3a::kJoinRows - 1) / h3a::kJoinRows);
+  // a warp per row where rows are few; larger items loop, or blocks with nothing to do would take longer to launch than to run
+  cfg.gridDim = dim3(shares, std::min(8, a.item_rows / h3a::kJoinRows));
   cfg.blockDim = dim3(h3a::kJoinRows * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr;

@@ -171,6 +171,7 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr, uint32_t lbo
 // Instruction descriptor for kind::f16 / kind::f8f6f4, fp32 accumulate, dense.
 //   [4,6) D format (1 = f32)  [7,10) A format  [10,13) B format  [15] A major  [16] B major (1 = MN-major)
 //   [17,23) N >> 3            [24,29) M >> 4
+constexpr uint32_t UMMA_FMT_F16 = 0;   // kind::f16
 constexpr uint32_t UMMA_FMT_BF16 = 1;  // kind::f16
 constexpr uint32_t UMMA_FMT_E4M3 = 0;  // kind::f8f6f4
 __host__ __device__ constexpr uint32_t umma_idesc(uint32_t afmt, uint32_t bfmt, uint32_t a_mn, uint32_t b_mn, uint32_t M, uint32_t N) {
