@@ -181,6 +181,36 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// A row of 128 codes (at `src`, 16-byte pieces swizzled by the row like the copies that brought them) as 128 bf16 or fp16
+// values times `f`, in the two half boxes at `dst`.  The pieces are read four at a time: one by one, a piece waited for the
+// one before it, and the helpers for them all (1,100 cycles for 16 KB).
+template <bool kBf16>
+__device__ __forceinline__ void widen_row(uint32_t src, uint32_t dst, uint32_t swz, uint32_t f, bool blank) {
+#pragma unroll
+  for (int c0 = 0; c0 < 8; c0 += 4) {
+    uint4 w[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) ld_shared_v4(src + (((c0 + c) ^ swz) << 4), w[c]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t in[4] = {blank ? 0u : w[c].x, blank ? 0u : w[c].y, blank ? 0u : w[c].z, blank ? 0u : w[c].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        if constexpr (kBf16) {
+          o[2 * y] = mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x1404)), f);
+          o[2 * y + 1] = mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x3424)), f);
+        } else {
+          o[2 * y] = mul_f16x2(e4m3_to_f16x2(in[y]), f);
+          o[2 * y + 1] = mul_f16x2(e4m3_high_to_f16x2(in[y]), f);
+        }
+      }
+      const uint32_t at = dst + ((c0 + c) >> 2) * kTileHalf;
+      st_shared_v4(at + (((2 * c) ^ swz) << 4), o[0], o[1], o[2], o[3]);
+      st_shared_v4(at + (((2 * c + 1) ^ swz) << 4), o[4], o[5], o[6], o[7]);
+    }
+  }
+}
 constexpr int kPieceRing = 4;
 constexpr int kPieceReaders = 15;  // warps
 
@@ -302,7 +332,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int row = threadIdx.x - 384;
     const uint32_t swz = row & 7;
     int cnt = 0;
-    uint32_t n_done = 0;  // tiles so far, all pieces
+    uint32_t n_done = 0, n_left = 0;  // tiles so far, all pieces
     bool ok = true;
     const TilePiece* q;
     for (; ok && (q = piece()) != nullptr; piece_done()) {
@@ -329,9 +359,25 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           for (int x = 0; x < 2; ++x) ex[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + h * a.c.exp_head[x]);
         }
       };
-      fetch_id(t0);
-      fetch_ex(t0);
-      fetch_id(t0 + 1);
+      // The tile's largest exponents, and V's smallest; rows of nothing (7) and rows that are not finite (255) aside.  Each
+      // warp leaves its own, a tile ahead; they meet at a barrier with a bounded wait.
+      auto leave_tops = [&](int tile) {
+        const bool there = tile * kKeyTile + row < lim_max;
+        const uint32_t k_top = __reduce_max_sync(0xFFFFFFFFu, there && ex[0] != 255u ? ex[0] : 0u);
+        const uint32_t v_top = __reduce_max_sync(0xFFFFFFFFu, there && ex[1] != 255u ? ex[1] : 0u);
+        const uint32_t v_low = __reduce_min_sync(0xFFFFFFFFu, there && ex[1] != 255u && ex[1] > 7u ? ex[1] : 255u);
+        if (lane == 0) {
+          tops[n_left & 1][warp - 12] = k_top | (v_top << 8) | (v_low << 16);
+          mbar_arrive(smem_u32(&bars->tops[n_left & 1]));
+        }
+        ++n_left;
+      };
+      if constexpr (kFp8) {
+        fetch_id(t0);
+        fetch_ex(t0);
+        fetch_id(t0 + 1);
+        leave_tops(t0);
+      }
       for (int it = 0; ok && it < n_tiles; ++it) {
         const int tile = t0 + it, key = tile * kKeyTile + row;
         const bool special = (tile + 1) * kKeyTile > lim_min;
@@ -340,19 +386,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         bool blank[2] = {gone, gone}; // e4m3: ... which may hold anything, codes for NaN included, and counts as zeros
         bool wide = false;
         if constexpr (kFp8) {
-          // the tile's largest exponents, and V's smallest; rows of nothing (7) and rows that are not finite (255) aside
-          const uint32_t ek = ex[0], ev = ex[1];
+          const uint32_t ek = ex[0], ev = ex[1], par = n_done & 1;
           if (it + 1 < n_tiles) fetch_ex(tile + 1);
           fetch_id(tile + 2);
-          const uint32_t k_top = __reduce_max_sync(0xFFFFFFFFu, !gone && ek != 255u ? ek : 0u);
-          const uint32_t v_top = __reduce_max_sync(0xFFFFFFFFu, !gone && ev != 255u ? ev : 0u);
-          const uint32_t v_low = __reduce_min_sync(0xFFFFFFFFu, !gone && ev != 255u && ev > 7u ? ev : 255u);
-          const uint32_t par = n_done & 1;
-          if (lane == 0) {
-            tops[par][warp - 12] = k_top | (v_top << 8) | (v_low << 16);
-            mbar_arrive(smem_u32(&bars->tops[par]));
-          }
-          ok = wait(bars->tops[par], (n_done >> 1) & 1, kTileWaitTops);  // a bounded meeting: a named barrier would not be
+          ok = wait(bars->tops[par], (n_done >> 1) & 1, kTileWaitTops);
           if (!ok) break;
           uint32_t kt = 0, vt = 0, vl = 255;
 #pragma unroll
@@ -396,37 +433,15 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (!ok) break;
             const uint32_t src = staging + g * kCodeBytes + row * 128;
             const uint32_t f = factor[x];
-            if (x == 1 && wide) {
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (!blank[x]) ld_shared_v4(src + ((c ^ swz) << 4), w);
-                const uint32_t at = dst + (c >> 2) * kTileHalf;
-                st_shared_v4(at + (((2 * (c & 3)) ^ swz) << 4), mul_bf16x2(e4m3_pattern(__byte_perm(w.x, 0, 0x1404)), f),
-                             mul_bf16x2(e4m3_pattern(__byte_perm(w.x, 0, 0x3424)), f), mul_bf16x2(e4m3_pattern(__byte_perm(w.y, 0, 0x1404)), f),
-                             mul_bf16x2(e4m3_pattern(__byte_perm(w.y, 0, 0x3424)), f));
-                st_shared_v4(at + (((2 * (c & 3) + 1) ^ swz) << 4), mul_bf16x2(e4m3_pattern(__byte_perm(w.z, 0, 0x1404)), f),
-                             mul_bf16x2(e4m3_pattern(__byte_perm(w.z, 0, 0x3424)), f), mul_bf16x2(e4m3_pattern(__byte_perm(w.w, 0, 0x1404)), f),
-                             mul_bf16x2(e4m3_pattern(__byte_perm(w.w, 0, 0x3424)), f));
-              }
-            } else {
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (!blank[x]) ld_shared_v4(src + ((c ^ swz) << 4), w);
-                const uint32_t at = dst + (c >> 2) * kTileHalf;
-                st_shared_v4(at + (((2 * (c & 3)) ^ swz) << 4), mul_f16x2(e4m3_to_f16x2(w.x), f), mul_f16x2(e4m3_high_to_f16x2(w.x), f),
-                             mul_f16x2(e4m3_to_f16x2(w.y), f), mul_f16x2(e4m3_high_to_f16x2(w.y), f));
-                st_shared_v4(at + (((2 * (c & 3) + 1) ^ swz) << 4), mul_f16x2(e4m3_to_f16x2(w.z), f), mul_f16x2(e4m3_high_to_f16x2(w.z), f),
-                             mul_f16x2(e4m3_to_f16x2(w.w), f), mul_f16x2(e4m3_high_to_f16x2(w.w), f));
-              }
-            }
+            if (x == 1 && wide) widen_row<true>(src, dst, swz, f, blank[x]);
+            else widen_row<false>(src, dst, swz, f, blank[x]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
               mbar_arrive(smem_u32(&bars->ready[s]));
               mbar_arrive(smem_u32(&bars->unstaged[g]));
             }
+            if (x == 1 && it + 1 < n_tiles) leave_tops(tile + 1);
           } else {
             ok = wait(bars->full[s], ph, kTileWaitFull);
             if (!ok) break;
@@ -471,11 +486,11 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         // Q is free late in the previous piece, ring slots earlier: the first two key tiles go ahead of Q
         const int q_at = g > 0 ? min(2, n_tiles - 1) : 0;
         bool q_loaded = false;
-        // page and place of this lane's sub-box of a tile; none behind the last key
-        int id = -1;
+        // page of this lane's sub-box of a tile, fetched a tile ahead; none behind the last key
+        int id = 0;
+        auto has_box = [&](int tile) { return lane < n_boxes && tile * kKeyTile + lane * box_rows < lim_max; };
         auto fetch_page = [&](int tile) {
-          const int key = tile * kKeyTile + lane * box_rows;
-          id = lane < n_boxes && key < lim_max ? checked_page(a, b, a.c.by_page(key)) : -1;
+          if (has_box(tile)) id = __ldg(a.c.pages + b * a.c.pages_stride + a.c.by_page(tile * kKeyTile + lane * box_rows));
         };
         fetch_page(t0);
         for (int it = 0; ok && it < n_tiles; ++it) {
@@ -500,9 +515,15 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
           }
           const int tile = t0 + it;
-          const int now = id, key = tile * kKeyTile + lane * box_rows, at = key - a.c.by_page(key) * a.c.page_size;
-          const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, now >= 0)) * box_bytes;
-          if (it + 1 < n_tiles) fetch_page(tile + 1);
+          const int key = tile * kKeyTile + lane * box_rows, at = key - a.c.by_page(key) * a.c.page_size;
+          const bool mine = has_box(tile);
+          const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, mine)) * box_bytes;
+          int now = id;
+          if (mine && static_cast<unsigned>(id) >= static_cast<unsigned>(a.c.n_pages)) {  // reported, and some other page read
+            report_cache(a.c, b);
+            now = 0;
+          }
+          fetch_page(tile + 1);
 #pragma unroll
           for (int x = 0; x < 2; ++x, ++cnt) {
             const CUtensorMap* tm = x ? &tm_v : &tm_k;
@@ -521,7 +542,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
             __syncwarp();
-            if (now >= 0) {
+            if (mine) {
               tma_load_4d(dst, tm, bar, 0, at, h, now);
               if constexpr (!kFp8) tma_load_4d(dst + kTileHalf, tm, bar, 64, at, h, now);
             }
