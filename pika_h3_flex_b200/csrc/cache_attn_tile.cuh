@@ -2,47 +2,54 @@
 //
 // One CTA per SM walks its share of the units piece by piece.  A piece is up to 2 x 128 query rows (two "streams", each
 // floor(128 / group) tokens x the group's heads, so that shared K/V heads fill the rows) against a run of 128-key tiles.
-//   warps 0-3 / 4-7  softmax of stream 0 / 1, one row per thread (TMEM lane == row): running maximum, exp2, row sum,
-//                    P written back over S as packed bf16, lazy rescale of O (when the maximum grows by more than 2^8)
-//   warp 8           producer: TMA loads of Q and of the K and V tiles, page by page, into a ring
-//   warps 9, 10      issuers, one per stream: S = Q K^T (N = 64 keys), O += P V (P from TMEM), tcgen05.commit
-//   warp 11          cuts the share into pieces and hands them to the others through a small ring: the bookkeeping would
-//                    cost every role some 40 registers (with each role walking the share on its own the softmax warps
-//                    spilled 1.4 KB and the kernel ran at half the speed)
-//   warps 12-15      helpers, one cache row per thread.  e4m3: widen a staged tile into the ring (below).  bf16: let tiles
+//   warps 0-15       softmax, a warpgroup per stream and 64-key half of every tile, one row per thread (TMEM lane == row)
+//   warp 16          producer: TMA loads of Q and of the K and V tiles, page by page, into a ring
+//   warps 17, 18     issuers, one per stream: S = Q K^T (N = 64 keys), O += P V (P from TMEM), tcgen05.commit
+//   warp 19          cuts the share into pieces and hands them to the others through a small ring: the bookkeeping would
+//                    cost every role some 40 registers
+//   warps 20-23      helpers, one cache row per thread.  e4m3: widen a staged tile into the ring (below).  bf16: let tiles
 //                    through, except the V tiles that not every row sees whole: P is 0 for a key a row does not see, and
 //                    0 x NaN is NaN, so rows behind the last key become zeros and values that are not finite become zeros
 //                    until the epilogue puts them back for the rows that do see them.
+// TMEM: stream t: S/P buffer of half h at columns [128 t + 64 h, +64), O at [256 + 128 t, +128).  Four chains of S -> P -> O
+// run per CTA; the two warpgroups of a stream share the accumulator and so have to agree on each row's reference.
+//
+// Softmax reference.  Softmax is exact for any reference while the terms stay in range.  A row's is the maximum of its
+// logits over the piece's FIRST key tile (the warpgroups exchange it once), which later logits rarely exceed by much: terms
+// may grow to 2^60 (bf16 P), 2^14 (fp16 P).  A piece in which some row outgrows that is done again after the others: one
+// pass that only looks for the rows' maxima, then one with those as references.  Against a running maximum per warp, with O
+// rescaled when it moves (two warpgroups, both halves each, two register images of S): that loop was 1.4 K instructions and
+// the SM's instruction cache missed on every second request, with helpers and issuers running other code beside it
+// (5.5 warps stalled on instruction fetch per issue); the loop here is a quarter of it.
+//
 // e4m3 tiles become fp16, two instructions per pair: a code is exact in fp16 (one conversion), and so is its product with
 // 2^(k - kref), kref being the tile's largest exponent, down to k - kref = -15 (below that a row's logits are off by less
 // than 2^-30 of the tile's largest).  2^kref goes into the tile's softmax scale, and Q into fp16 by a power of two per row
-// that joins that scale too.  V is kept relative to the running maximum of the tiles' exponents, in whose units O
-// accumulates (a rise rescales O like a rise of the row maximum), and P is held as 2^7 p: terms down to 2^-31 of the
-// row's largest count.  A V tile with rows more than 2^14 below that maximum is widened to bf16 instead, and its P
-// rounded to bf16, so that no row's own precision is lost.  (Everything through bf16 took five instructions per pair: the
-// helpers then set the pace at 500 TFLOP/s.)
-// Each 128-key tile is processed as two 64-key halves with S buffers of their own, so that a stream has two S / P buffers
-// in flight, as in the dense kernels.  TMEM: stream t: S/P buffer h at columns [128 t + 64 h, +64), O at [256 + 128 t, +128).
+// that joins that scale too.  V and O are in units of the largest exponent of the piece's first tile; fp16 holds codes up
+// to 2^7 above that, and rows 2^14 below it with all their bits.  A V tile with rows outside that is widened to bf16
+// instead, and its P rounded to bf16.  (Everything through bf16 took five instructions per pair.)
 //
 // Every wait is bounded: when the limit runs out the CTA records a code in the status word, raises a CTA-wide flag that the
-// other waits poll, lets copies in flight land, frees TMEM and returns.
+// other waits poll, lets copies in flight land, frees TMEM and returns.  Warps meet at mbarriers, never at named barriers,
+// so that one that gave up keeps nobody waiting for ever.
 #pragma once
 #include "cache_attn.cuh"
 
 namespace h3a {
 
-constexpr int kTileThreads = 512;
+constexpr int kTileThreads = 768;
 constexpr int kKeyTile = 128, kTileKeyShift = 7;
-constexpr int kTileSoftmaxRegs = 200, kTileOtherRegs = 56, kTileLaunchRegs = 128;
-static_assert(256 * kTileSoftmaxRegs + 256 * kTileOtherRegs <= kTileLaunchRegs * kTileThreads, "setmaxnreg budget exceeds the launch allocation");
+constexpr int kTileSoftmaxRegs = 96, kTileOtherRegs = 48, kTileLaunchRegs = 80;
+static_assert(512 * kTileSoftmaxRegs + 256 * kTileOtherRegs <= kTileLaunchRegs * kTileThreads, "setmaxnreg budget exceeds the launch allocation");
+constexpr int kProducerWarp = 16, kIssuerWarp = 17, kPieceWarp = 19, kHelperWarp = 20;
 constexpr int kTileRows = 256;         // rows of an item
 constexpr int kTileBytes = 32768;      // 128 rows of 128 bf16
 constexpr int kTileHalf = 16384;       // one [128 rows][128 bytes] swizzled box
 constexpr int kCodeBytes = 16384;      // 128 rows of 128 codes
 template <bool kFp8>
 struct TileRing {
-  static constexpr int kRing = kFp8 ? 3 : 5;     // bf16 tiles
-  static constexpr int kStaged = kFp8 ? 4 : 0;   // e4m3 tiles as loaded
+  static constexpr int kRing = kFp8 ? 3 : 4;     // tiles as the MMAs read them
+  static constexpr int kStaged = kFp8 ? 3 : 0;   // e4m3 tiles as loaded
   static constexpr int kBytes = kRing * kTileBytes + kStaged * kCodeBytes;
 };
 
@@ -54,20 +61,25 @@ struct TileBars {
   uint64_t unstaged[4];    // e4m3: widened
   uint64_t q_full, q_empty;
   uint64_t q_ready[2];     // e4m3: the stream's Q is in fp16
-  uint64_t s_full[2][2], p_full[2][2], o_full[2][2];  // [stream][half]
-  uint64_t o_free[2];
+  uint64_t s_full[2][2], p_full[2][2];  // [stream][half]
+  uint64_t o_full[2];      // every P V of the stream's piece has completed
+  uint64_t o_free[2];      // the stream's warps have read O
+  uint64_t meet[2];        // the stream's eight warps have left what the other half is to see
   uint64_t piece_full[4], piece_empty[4];
   uint64_t tops[2];        // e4m3: the helper warps' exponents of a tile are there
   uint32_t tmem_base;
   uint32_t early_exit;
   volatile uint32_t abort_flag;
   volatile uint32_t poison;  // some V value counted as zero: from then on every epilogue looks for such values
+  uint32_t redo;             // pieces of the current batch that outgrew their reference, a bit each
+  float left[2][2][2][128];  // [turn][stream][half][row]: what the halves of a stream leave for each other
 };
-constexpr int kTileSmemBytes = 2 * kTileBytes + TileRing<false>::kBytes + 1024 + 512;
-static_assert(TileRing<true>::kBytes <= TileRing<false>::kBytes && sizeof(TileBars) <= 512, "shared memory layout");
+constexpr int kTileBarBytes = 4608;
+constexpr int kTileSmemBytes = 2 * kTileBytes + (TileRing<true>::kBytes > TileRing<false>::kBytes ? TileRing<true>::kBytes : TileRing<false>::kBytes) + 1024 + kTileBarBytes;
+static_assert(sizeof(TileBars) <= kTileBarBytes, "shared memory layout");
 enum : int {  // status codes of waits that ran out (low byte of the status word)
   kTileWaitEmpty = 33, kTileWaitFull, kTileWaitReady, kTileWaitUnstaged, kTileWaitStaged, kTileWaitQFull, kTileWaitQEmpty,
-  kTileWaitQReady, kTileWaitTops, kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitPiece
+  kTileWaitQReady, kTileWaitTops, kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitMeet, kTileWaitPiece
 };
 
 struct TileWait {
@@ -106,28 +118,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, 
       : "memory");
 }
 
-// 16 columns at a time: for the rescale path, which runs with both register images of S alive
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-__device__ __forceinline__ void reg_fence16(uint32_t (&r)[16]) {
-  asm volatile(""
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
 }
 
 // 8 x 8 transpose of 16-byte pieces among 8 neighbouring lanes: in, lane s has pieces 0 .. 7 of row s; out, lane s has piece
@@ -163,15 +159,17 @@ struct TilePiece {
   int tok0, n, len;  // its number in the sequence; new rows and length of the sequence
   int whole;         // the piece is the whole item; otherwise its results are partial
   int tail;          // ... and go to the share's tail slot (the item begins here)
+  int mode;          // how the rows' references come about
+  int bit;           // its bit in `redo`
 };
 // e4m3: what a tile's rows were widened with
 struct TileInfo {
   float k_unit;   // 2^(kref - 127): the tile's logits are in these units
-  int vref;       // its V is in units of 2^(vref - 127)
+  int vref;       // V, and so O, is in units of 2^(vref - 127): the same for a piece's tiles
   int wide;       // V is bf16, and P is to be
 };
 constexpr int kInfoRing = 8;  // the helpers are at most two tiles ahead of the softmax warps
-// 2^-d as an fp16 pair
+// 2^-d as an fp16 pair, d >= -15
 __device__ __forceinline__ uint32_t f16x2_pow2_neg(int d) {
   const uint32_t h = d <= 14 ? static_cast<uint32_t>(15 - d) << 10 : d <= 24 ? 1u << (24 - d) : 0u;
   return h * 0x10001u;
@@ -212,7 +210,9 @@ __device__ __forceinline__ void widen_row(uint32_t src, uint32_t dst, uint32_t s
   }
 }
 constexpr int kPieceRing = 4;
-constexpr int kPieceReaders = 15;  // warps
+constexpr int kPieceReaders = 23;  // warps
+constexpr int kPieceBatch = 32;    // pieces between two looks at `redo`
+enum : int { kFirstTile = 0, kFindMaxima = 1, kUseMaxima = 2 };
 
 __device__ __forceinline__ int piece_limit(const CacheAttnArgs& a, const TilePiece& q, int token) {
   return a.causal ? max(0, min(q.len, q.len - q.n + token + 1)) : q.len;
@@ -258,7 +258,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw_addr);
   const uint32_t q_smem = base, ring = base + 2 * kTileBytes, staging = ring + R::kRing * kTileBytes;
-  TileBars* bars = reinterpret_cast<TileBars*>(smem + 2 * kTileBytes + TileRing<false>::kBytes);
+  TileBars* bars = reinterpret_cast<TileBars*>(smem + kTileSmemBytes - 1024 - kTileBarBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -276,13 +276,14 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     mbar_init(smem_u32(&bars->tops[0]), 4);
     mbar_init(smem_u32(&bars->tops[1]), 4);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(smem_u32(&bars->q_ready[t]), 4);
+      mbar_init(smem_u32(&bars->q_ready[t]), 8);
       for (int hf = 0; hf < 2; ++hf) {
         mbar_init(smem_u32(&bars->s_full[t][hf]), 1);
-        mbar_init(smem_u32(&bars->p_full[t][hf]), 128);
-        mbar_init(smem_u32(&bars->o_full[t][hf]), 1);
+        mbar_init(smem_u32(&bars->p_full[t][hf]), 4);
       }
-      mbar_init(smem_u32(&bars->o_free[t]), 4);
+      mbar_init(smem_u32(&bars->o_full[t]), 1);
+      mbar_init(smem_u32(&bars->o_free[t]), 8);
+      mbar_init(smem_u32(&bars->meet[t]), 8);
     }
     for (int i = 0; i < kPieceRing; ++i) {
       mbar_init(smem_u32(&bars->piece_full[i]), 1);
@@ -290,11 +291,12 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     }
     bars->abort_flag = 0;
     bars->poison = 0;
+    bars->redo = 0;
     bars->early_exit = (a.c.status != nullptr && *reinterpret_cast<volatile int*>(a.c.status) != 0) ? 1u : 0u;
     fence_mbar_init();
     a.desc[kDescInts * blockIdx.x] = 0;
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == kProducerWarp && lane == 0) {
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
@@ -303,7 +305,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   ShareIter iter = share_begin(a, &start);
   __syncthreads();  // barriers and flags are set up
   if (bars->early_exit) return;
-  if (warp == 9) {
+  if (warp == kIssuerWarp) {
     tmem_alloc(smem_u32(&bars->tmem_base), 512);
     tmem_relinquish();
   }
@@ -326,13 +328,14 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     ++n_pieces;
   };
 
-  if (warp >= 12) {
+  if (warp >= kHelperWarp) {
     // =========================================================== helpers: thread r owns row r of every tile
     setmaxnreg_dec<kTileOtherRegs>();
-    const int row = threadIdx.x - 384;
+    const int row = threadIdx.x - kHelperWarp * 32;
     const uint32_t swz = row & 7;
     int cnt = 0;
     uint32_t n_done = 0, n_left = 0;  // tiles so far, all pieces
+    uint32_t vref = 0;
     bool ok = true;
     const TilePiece* q;
     for (; ok && (q = piece()) != nullptr; piece_done()) {
@@ -341,7 +344,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       // e4m3: the exponent bytes of this thread's row are fetched a tile ahead, their page number two tiles ahead
       uint32_t ex[2] = {0, 0};
       int id_next = 0;
-      uint32_t vref = 0;
+      uint32_t v_most = 0;  // largest exponent of V in the piece
+      if (q->mode != kUseMaxima) vref = 0;  // otherwise what the pass before it found
       auto fetch_id = [&](int tile) {
         const int key = tile * kKeyTile + row;
         if (kFp8 && key < lim_max) id_next = __ldg(a.c.pages + b * a.c.pages_stride + a.c.by_page(key));
@@ -364,10 +368,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       auto leave_tops = [&](int tile) {
         const bool there = tile * kKeyTile + row < lim_max;
         const uint32_t k_top = __reduce_max_sync(0xFFFFFFFFu, there && ex[0] != 255u ? ex[0] : 0u);
-        const uint32_t v_top = __reduce_max_sync(0xFFFFFFFFu, there && ex[1] != 255u ? ex[1] : 0u);
+        const uint32_t v_top = __reduce_max_sync(0xFFFFFFFFu, there && ex[1] != 255u && ex[1] > 7u ? ex[1] : 0u);
         const uint32_t v_low = __reduce_min_sync(0xFFFFFFFFu, there && ex[1] != 255u && ex[1] > 7u ? ex[1] : 255u);
         if (lane == 0) {
-          tops[n_left & 1][warp - 12] = k_top | (v_top << 8) | (v_low << 16);
+          tops[n_left & 1][warp - kHelperWarp] = k_top | (v_top << 8) | (v_low << 16);
           mbar_arrive(smem_u32(&bars->tops[n_left & 1]));
         }
         ++n_left;
@@ -382,8 +386,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const int tile = t0 + it, key = tile * kKeyTile + row;
         const bool special = (tile + 1) * kKeyTile > lim_min;
         const bool gone = key >= lim_max;
-        uint32_t factor[2] = {0, 0};  // e4m3: of this thread's row of K and V
-        bool blank[2] = {gone, gone}; // e4m3: ... which may hold anything, codes for NaN included, and counts as zeros
+        uint32_t factor[2] = {0, 0};   // e4m3: of this thread's row of K and V
+        bool blank[2] = {gone, gone};  // e4m3: ... which may hold anything, codes for NaN included, and counts as zeros
         bool wide = false;
         if constexpr (kFp8) {
           const uint32_t ek = ex[0], ev = ex[1], par = n_done & 1;
@@ -399,8 +403,11 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             vt = max(vt, (x >> 8) & 255u);
             vl = min(vl, x >> 16);
           }
-          vref = max(vref, vt);
-          wide = vl + 14u < vref;
+          v_most = max(v_most, vt);
+          if (vref == 0u) vref = vt != 0u ? vt : 127u;
+          wide = vl + 14u < vref || vt > vref + 7u;
+          // O itself could leave fp32 (the first tile's V next to nothing): with the piece's largest exponent as the unit it cannot
+          if (vt > vref + 40u && row == 0) atomicOr(&bars->redo, 1u << q->bit);
           if (row == 0) {
             TileInfo& to = info[n_done % kInfoRing];
             to.k_unit = __uint_as_float(kt << 23);
@@ -415,14 +422,14 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               bars->poison = 1u;
             }
           } else {
-            factor[1] = wide ? static_cast<uint32_t>(247 + static_cast<int>(ev) - static_cast<int>(vref)) * 0x800080u
+            factor[1] = wide ? static_cast<uint32_t>(max(0, min(254, 247 + static_cast<int>(ev) - static_cast<int>(vref)))) * 0x800080u
                              : f16x2_pow2_neg(static_cast<int>(vref) - static_cast<int>(ev));
           }
           if (blank[0]) factor[0] = 0;
           if (blank[1]) factor[1] = 0;
           ++n_done;
         }
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < 2; ++x, ++cnt) {  // K, then V
           const int s = cnt % R::kRing;
           const uint32_t ph = (cnt / R::kRing) & 1;
@@ -432,16 +439,20 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             ok = wait(bars->staged[g], (cnt / R::kStaged) & 1, kTileWaitStaged) && wait(bars->empty[s], ph ^ 1u, kTileWaitEmpty);
             if (!ok) break;
             const uint32_t src = staging + g * kCodeBytes + row * 128;
-            const uint32_t f = factor[x];
-            if (x == 1 && wide) widen_row<true>(src, dst, swz, f, blank[x]);
-            else widen_row<false>(src, dst, swz, f, blank[x]);
+            const uint32_t f = x ? factor[1] : factor[0];
+            const bool none = x ? blank[1] : blank[0];
+            if (x == 1 && wide) widen_row<true>(src, dst, swz, f, none);
+            else widen_row<false>(src, dst, swz, f, none);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
               mbar_arrive(smem_u32(&bars->ready[s]));
               mbar_arrive(smem_u32(&bars->unstaged[g]));
             }
-            if (x == 1 && it + 1 < n_tiles) leave_tops(tile + 1);
+            if (x == 1) {
+              if (it + 1 < n_tiles) leave_tops(tile + 1);
+              else if (q->mode == kFindMaxima) vref = v_most != 0u ? v_most : 127u;
+            }
           } else {
             ok = wait(bars->full[s], ph, kTileWaitFull);
             if (!ok) break;
@@ -469,9 +480,9 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= kProducerWarp) {
     setmaxnreg_dec<kTileOtherRegs>();
-    if (warp == 8) {
+    if (warp == kProducerWarp) {
       // ========================================================= producer: lane x copies sub-box x of a tile
       const int n_boxes = kKeyTile / box_rows;
       const int box_bytes = box_rows * (kFp8 ? kCacheDim : 2 * kCacheDim);
@@ -551,9 +562,9 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         ++g;
       }
-    } else if (warp < 11) {
+    } else if (warp < kPieceWarp) {
       // ========================================================= issuers, one warp per stream
-      const int t = warp - 9;
+      const int t = warp - kIssuerWarp;
       const uint32_t leader = elect_one();
       constexpr uint32_t kFmt = kFp8 ? UMMA_FMT_F16 : UMMA_FMT_BF16;
       constexpr uint32_t idesc_s = umma_idesc(kFmt, kFmt, 0, 0, 128, 64);
@@ -583,7 +594,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         for (int k = 0; k < 4; ++k)
           umma_bf16_ts_if(leader, o_tmem, s_tmem + hf * 64 + k * 8, vd + (k * 2048 >> 4), idesc, (pv_cnt > 0 || k > 0) ? 1u : 0u);
         ++pv_cnt;
-        umma_commit_if(leader, smem_u32(&bars->o_full[t][hf]));
       };
       auto ready = [&](int c) {
         const bool got = wait(bars->ready[c % R::kRing], (c / R::kRing) & 1, kTileWaitReady);
@@ -633,77 +643,107 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           umma_commit_if(leader, smem_u32(&bars->empty[cv % R::kRing]));
           if (has_next) umma_commit_if(leader, smem_u32(&bars->empty[ck % R::kRing]));
         }
+        if (!ok) break;
         c0 += 2 * n_tiles;
         ++g;
-        if (n_mine > 0) ++own;
+        if (n_mine > 0) {
+          umma_commit_if(leader, smem_u32(&bars->o_full[t]));
+          ++own;
+        }
       }
     } else if (lane == 0) {
       // ========================================================= the share's pieces, one after the other
       Piece p;
-      for (uint32_t n = 0;; ++n) {
+      uint32_t n = 0;  // pieces handed out
+      bool ok = true;
+      auto hand_out = [&](const ShareIter& at, int mode, int bit) {
         const uint32_t i = n % kPieceRing;
-        const bool more = iter.next(a, p);
-        if (!wait.one(bars->piece_empty[i], ((n / kPieceRing) & 1) ^ 1u, kTileWaitPiece)) break;
-        if (more) describe_piece(a, iter, p, pieces[i]);
-        else pieces[i].n_tiles = -1;
+        ok = wait.one(bars->piece_empty[i], ((n / kPieceRing) & 1) ^ 1u, kTileWaitPiece);
+        if (!ok) return;
+        describe_piece(a, at, p, pieces[i]);
+        pieces[i].mode = mode;
+        pieces[i].bit = bit;
         mbar_arrive(smem_u32(&bars->piece_full[i]));
-        if (!more) break;
+        ++n;
+      };
+      auto all_done = [&]() {  // everybody has finished every piece handed out
+        for (uint32_t k = n < kPieceRing ? 0 : n - kPieceRing; ok && k < n; ++k)
+          ok = wait.one(bars->piece_empty[k % kPieceRing], (k / kPieceRing) & 1, kTileWaitPiece);
+      };
+      bool more = true;
+      while (ok && more) {
+        ShareIter again = iter;
+        int in_batch = 0;
+        while (ok && in_batch < kPieceBatch && (more = iter.next(a, p))) hand_out(iter, kFirstTile, in_batch++);
+        if (ok) all_done();
+        if (!ok) break;
+        const uint32_t redo = bars->redo;
+        bars->redo = 0;
+        for (int k = 0; ok && redo != 0u && k < in_batch; ++k) {
+          again.next(a, p);
+          if ((redo >> k) & 1u) {
+            hand_out(again, kFindMaxima, 31);
+            if (ok) hand_out(again, kUseMaxima, 31);
+          }
+        }
+        if (redo != 0u && ok) all_done();
+        bars->redo = 0;
+      }
+      if (ok) {
+        const uint32_t i = n % kPieceRing;
+        if (wait.one(bars->piece_empty[i], ((n / kPieceRing) & 1) ^ 1u, kTileWaitPiece)) {
+          pieces[i].n_tiles = -1;
+          mbar_arrive(smem_u32(&bars->piece_full[i]));
+        }
       }
     }
     __syncwarp();
   } else {
-    // =========================================================== softmax, rescaling, results
+    // =========================================================== softmax and results
     setmaxnreg_inc<kTileSoftmaxRegs>();
-    const int t = warp >> 2, quarter = warp & 3;
+    const int t = (warp >> 2) & 1, hf = warp >> 3, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lane_base + t * 128, o_addr = tmem + lane_base + 256 + t * 128;
-    uint32_t j = 0;  // key tiles the stream has processed: the phase of s_full / o_full
-    uint32_t g = 0;  // e4m3: pieces with work so far, the phase of q_full; their tiles
-    uint32_t n_before = 0;
+    const uint32_t s_addr = tmem + lane_base + t * 128 + hf * 64;
+    const uint32_t o_addr = tmem + lane_base + 256 + t * 128 + hf * 64;  // epilogue: this warpgroup's 64 columns of O
+    constexpr float kLift = kFp8 ? 2.f : 0.f;            // the reference's own term is 2^kLift
+    constexpr float kMostTerms = kFp8 ? 6.0e4f : 1.0e18f;  // 64 terms of a row: more than that has outgrown the reference
+    uint32_t j = 0;         // key tiles the stream has processed: the phase of s_full
+    uint32_t own = 0;       // pieces in which the stream had work: the phase of o_full
+    uint32_t g = 0;         // e4m3: pieces with work, the phase of q_full
+    uint32_t n_before = 0;  // tiles of the pieces before
+    uint32_t turn = 0;      // meetings of the stream's two halves so far
     bool ok = true;
-    uint32_t ra[64], rb[64];
-    auto load_s = [&](uint32_t (&r)[64], int hf) {
-      tc_fence_after_sync();
-      tmem_ld32(s_addr + hf * 64, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-      tmem_ld32(s_addr + hf * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+    // Leaves x for the same row's thread of the other half and returns what that one left.  Each side's values are in a
+    // slot by turn: nobody can be two meetings ahead of a reader.
+    auto exchange = [&](float x) -> float {
+      bars->left[turn & 1][t][hf][row] = x;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars->meet[t]));
+      ok = wait(bars->meet[t], turn & 1, kTileWaitMeet);
+      const float y = bars->left[turn & 1][t][hf ^ 1][row];
+      ++turn;
+      return y;
     };
-    auto fetch_s = [&](uint32_t (&r)[64], int hf, uint32_t jt) {
-      const bool got = wait(bars->s_full[t][hf], jt & 1, kTileWaitS);
-      if (got) load_s(r, hf);
-      return got;
-    };
-    auto try_fetch_s = [&](uint32_t (&r)[64], int hf, uint32_t jt) {
-      const bool there = __all_sync(0xFFFFFFFFu, mbar_test_wait(smem_u32(&bars->s_full[t][hf]), jt & 1));
-      if (there) load_s(r, hf);
-      return there;
-    };
-    auto publish_p = [&](uint32_t (&s)[64], int hf) {
-      tmem_st32(s_addr + hf * 64, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-      tmem_wait_st();
-      tc_fence_before_sync();
-      mbar_arrive(smem_u32(&bars->p_full[t][hf]));
-    };
-    const int row_token = t * T + row / a.group, row_head = row % a.group;  // row r: token r / group, head r % group
     const TilePiece* q;
     for (; ok && (q = piece()) != nullptr; piece_done()) {
-      const int n_mine = q->end[t];
+      const int n_mine = q->end[t], mode = q->mode;
+      const int row_i = a.by_group(row);                  // row r: token r / group, head r % group
+      const int row_token = t * T + row_i;
       const bool have_row = row < T * a.group && q->tok0 + row_token < q->n;
-      const int lim = (have_row ? piece_limit(a, *q, q->tok0 + row_token) : 0) - q->t0 * kKeyTile;  // counted from tile t0
-      const int lim_first = piece_limit(a, *q, q->tok0 + t * T) - q->t0 * kKeyTile;  // the stream's first row sees fewest keys
-      float m_ref = kNoMax, l_sum = 0.f;
+      const int lim = (have_row ? piece_limit(a, *q, q->tok0 + row_token) : 0) - q->t0 * kKeyTile - hf * 64;  // keys of this half, counted from tile t0
+      const int lim_first = piece_limit(a, *q, q->tok0 + t * T) - q->t0 * kKeyTile - hf * 64;  // the stream's first row sees fewest keys
       float row_unit = a.scale_log2;  // from S to logits in log2
-      float c = row_unit;             // ... of the current tile
-      int vref = 0;                   // e4m3: O is in units of 2^(vref - 127)
-      bool wide = false;
-      const uint32_t tile0 = n_before;
+      float m_ref = kNoMax;
+      if (mode == kUseMaxima && n_mine > 0)  // what the pass before this one left
+        m_ref = fmaxf(bars->left[(turn & 1) ^ 1][t][0][row], bars->left[(turn & 1) ^ 1][t][1][row]) - kLift;
       if constexpr (kFp8) {
-        n_before += q->n_tiles;
         if (q->n_tiles > 0) {
           ok = wait(bars->q_full, g & 1, kTileWaitQFull);  // every piece's: a phase must not be skipped
           if (!ok) break;
           if (n_mine > 0) {
-            // the thread's row of Q into fp16, in place: the row's largest becomes 2^4 .. 2^5
+            // The thread's row of Q into fp16, in place: the row's largest becomes 2^4 .. 2^5.  Both halves look at the whole
+            // row, meet (everything has been read), and convert half of it each.
             const uint32_t src = q_smem + t * kTileBytes + row * 128, swz = row & 7;
             uint32_t m = 0;
 #pragma unroll 4
@@ -715,9 +755,11 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const int e = max(static_cast<int>(max(m >> 16, m & 0xFFFFu) >> 7) - 127 - 4, -120);
             const float f = pow2_float(-e);
             row_unit *= pow2_float(e);
+            exchange(0.f);
+            if (!ok) break;
 #pragma unroll 4
-            for (int x = 0; x < 16; ++x) {
-              const uint32_t at = src + (x >> 3) * kTileHalf + (((x & 7) ^ swz) << 4);
+            for (int x = 0; x < 8; ++x) {
+              const uint32_t at = src + hf * kTileHalf + ((x ^ swz) << 4);
               uint4 w;
               ld_shared_v4(at, w);
               const uint32_t in[4] = {w.x, w.y, w.z, w.w};
@@ -733,142 +775,129 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           ++g;
         }
       }
-
-      auto softmax_half = [&](uint32_t (&s)[64], int hf, int it) -> bool {
-        const int key0 = it * kKeyTile + hf * 64;
-        if (key0 + 64 > lim_first) {
-          const int valid = lim - key0;
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i >= valid) s[i] = 0xFF800000u;  // -inf
-        }
-        float mx0 = fmax3(__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]));
-        float mx1 = fmax3(__uint_as_float(s[3]), __uint_as_float(s[4]), __uint_as_float(s[5]));
-        float mx2 = fmax3(__uint_as_float(s[6]), __uint_as_float(s[7]), __uint_as_float(s[8]));
-        float mx3 = fmax3(__uint_as_float(s[9]), __uint_as_float(s[10]), __uint_as_float(s[11]));
-#pragma unroll
-        for (int i = 12; i < 60; i += 8) {
-          mx0 = fmax3(mx0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-          mx1 = fmax3(mx1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-          mx2 = fmax3(mx2, __uint_as_float(s[i + 4]), __uint_as_float(s[i + 5]));
-          mx3 = fmax3(mx3, __uint_as_float(s[i + 6]), __uint_as_float(s[i + 7]));
-        }
-        mx0 = fmax3(mx0, __uint_as_float(s[60]), __uint_as_float(s[61]));
-        mx1 = fmax3(mx1, __uint_as_float(s[62]), __uint_as_float(s[63]));
-        // the largest term is 2^kLift at first, and 2^(kLift + 8) before the reference moves
-        constexpr float kLift = kFp8 ? 7.f : 0.f;
-        const float m_tile = fmax3(fmaxf(mx0, mx1), mx2, mx3) * c - kLift;
-        int v_shift = 0;
-        if (kFp8 && hf == 0) {
-          const TileInfo& in = info[(tile0 + it) % kInfoRing];
+      float l_sum = 0.f;
+      bool over = false;
+      for (int it = 0; it < n_mine; ++it) {
+        ok = wait(bars->s_full[t][hf], j & 1, kTileWaitS);
+        if (!ok) break;
+        tc_fence_after_sync();
+        float c = row_unit;
+        bool wide = false;
+        if constexpr (kFp8) {
+          const TileInfo& in = info[(n_before + it) % kInfoRing];
+          c = fminf(row_unit * in.k_unit, 3.0e38f);
           wide = in.wide != 0;
-          v_shift = it == 0 ? 0 : vref - in.vref;
-          vref = in.vref;
         }
-        if (it == 0 && hf == 0) {
-          m_ref = fmaxf(m_tile, kNoMax);
-        } else if (__any_sync(0xFFFFFFFFu, m_tile - m_ref > 8.0f) || v_shift != 0) {
-          const float m_new = fmaxf(m_ref, m_tile);
-          float alpha = ex2_approx(m_ref - m_new);
-          m_ref = m_new;
-          l_sum *= alpha;
-          if constexpr (kFp8) alpha *= pow2_float(v_shift);
-          // the stream's previous P V must be complete; MMAs complete in issue order, so it is the only one that can run
-          if (!wait(bars->o_full[t][hf ^ 1], (hf ? j : j - 1) & 1, kTileWaitO)) return false;
-          tc_fence_after_sync();
+        const bool partly = (it + 1) * kKeyTile - 64 > lim_first;
+        const int valid = lim - it * kKeyTile;
+        // 32 of the half's 64 keys at a time
+        auto load = [&](uint32_t (&r)[32], int x) {
+          tmem_ld32(s_addr + 32 * x, r);
+          tmem_wait_ld();
+          reg_fence32(r);
+          if (partly) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t o[16];
-            tmem_ld16(o_addr + 16 * i, o);
-            tmem_wait_ld();
-            reg_fence16(o);
+            for (int i = 0; i < 32; ++i)
+              if (i >= valid - 32 * x) r[i] = 0xFF800000u;  // -inf
+          }
+        };
+        if (mode == kFindMaxima || (it == 0 && mode == kFirstTile)) {
+#pragma unroll 1
+          for (int x = 0; x < 2; ++x) {
+            uint32_t r[32];
+            load(r, x);
+            float mx0 = fmax3(__uint_as_float(r[0]), __uint_as_float(r[1]), __uint_as_float(r[2]));
+            float mx1 = fmax3(__uint_as_float(r[3]), __uint_as_float(r[4]), __uint_as_float(r[5]));
 #pragma unroll
-            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-            tmem_st16(o_addr + 16 * i, o);
+            for (int i = 6; i < 30; i += 4) {
+              mx0 = fmax3(mx0, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+              mx1 = fmax3(mx1, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+            }
+            mx0 = fmax3(mx0, __uint_as_float(r[30]), __uint_as_float(r[31]));
+            m_ref = fmaxf(m_ref, fmaxf(mx0, mx1) * c);  // a maximum of nothing but NaN: the reference stays finite
+          }
+          if (mode == kFirstTile) {
+            m_ref = fmaxf(m_ref, exchange(m_ref)) - kLift;
+            if (!ok) break;
           }
         }
         // P = 2^(s c - m), rounded once; the row sum keeps the unrounded terms
-        uint64_t acc0 = 0, acc1 = 0;
+        float l_half = 0.f;
         const uint64_t c2 = pack2(c, c), nm2 = pack2(-m_ref, -m_ref);
+        auto half = [&](auto pack) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float x0, x1;
-          unpack2(fma2(pack2u(s[2 * i], s[2 * i + 1]), c2, nm2), x0, x1);
-          const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-          if (i & 1) acc1 = add2(acc1, pack2(p0, p1));
-          else acc0 = add2(acc0, pack2(p0, p1));
-          s[i] = kFp8 && !wide ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+          for (int x = 0; x < 2; ++x) {
+            uint32_t r[32], o[16];
+            load(r, x);
+            uint64_t acc0 = 0, acc1 = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x0, x1;
+              unpack2(fma2(pack2u(r[2 * i], r[2 * i + 1]), c2, nm2), x0, x1);
+              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              if (i & 1) acc1 = add2(acc1, pack2(p0, p1));
+              else acc0 = add2(acc0, pack2(p0, p1));
+              o[i] = pack(p0, p1);
+            }
+            float a0, a1, a2, a3;
+            unpack2(acc0, a0, a1);
+            unpack2(acc1, a2, a3);
+            l_half += (a0 + a1) + (a2 + a3);
+            tmem_st16(s_addr + 16 * x, o);
+          }
+        };
+        if (mode == kFindMaxima) {
+          uint32_t o[16] = {};  // P = 0
+          tmem_st16(s_addr, o);
+          tmem_st16(s_addr + 16, o);
+        } else if (kFp8 && !wide) {
+          half([](float x, float y) { return pack_f16x2(x, y); });
+        } else {
+          half([](float x, float y) { return pack_bf16x2(x, y); });
         }
-        float a0, a1, a2, a3;
-        unpack2(acc0, a0, a1);
-        unpack2(acc1, a2, a3);
-        l_sum += (a0 + a1) + (a2 + a3);
-        return true;
-      };
-
-      if (n_mine > 0) ok = fetch_s(ra, 0, j);
-      for (int it = 0; ok && it < n_mine; ++it) {
-        tmem_wait_ld();
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[0]));
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[32]));
-        if constexpr (kFp8) c = fminf(row_unit * info[(tile0 + it) % kInfoRing].k_unit, 3.0e38f);
-        ok = softmax_half(ra, 0, it);
-        if (!ok) break;
-        const bool early1 = try_fetch_s(rb, 1, j);
-        publish_p(ra, 0);
-        if (!early1) ok = fetch_s(rb, 1, j);
-        if (!ok) break;
-        tmem_wait_ld();
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&rb[0]));
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&rb[32]));
-        ok = softmax_half(rb, 1, it);
-        if (!ok) break;
-        const bool more = it + 1 < n_mine;
-        const bool early0 = more && try_fetch_s(ra, 0, j + 1);
-        publish_p(rb, 1);
+        l_sum += l_half;
+        over |= !(l_half < kMostTerms);  // also infinities and NaN
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->p_full[t][hf]));
         ++j;
-        if (more && !early0) ok = fetch_s(ra, 0, j);
       }
       if (!ok) break;
+      if constexpr (kFp8) n_before += q->n_tiles;
 
       // ---- O leaves TMEM first: the next piece's first P V may overwrite it while the rows are stored
+      uint32_t s[64];
       if (n_mine > 0) {
-        ok = wait(bars->o_full[t][1], (j - 1) & 1, kTileWaitO);
+        ok = wait(bars->o_full[t], own & 1, kTileWaitO);
         if (!ok) break;
+        ++own;
         tc_fence_after_sync();
-        tmem_ld32(o_addr, *reinterpret_cast<uint32_t(*)[32]>(&ra[0]));
-        tmem_ld32(o_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&ra[32]));
-        tmem_ld32(o_addr + 64, *reinterpret_cast<uint32_t(*)[32]>(&rb[0]));
-        tmem_ld32(o_addr + 96, *reinterpret_cast<uint32_t(*)[32]>(&rb[32]));
+        tmem_ld32(o_addr, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        tmem_ld32(o_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
         tmem_wait_ld();
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[0]));
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&ra[32]));
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&rb[0]));
-        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&rb[32]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(&s[32]));
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bars->o_free[t]));
       } else {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) ra[i] = rb[i] = 0u;
+        for (int i = 0; i < 64; ++i) s[i] = 0u;
       }
-      const int head = q->h * a.group + row_head;
+      // the two halves' row sums; after a pass for the maxima, those, which then stay where they were left
+      const float other = exchange(mode == kFindMaxima ? m_ref : l_sum);
+      if (!ok) break;
+      if (mode == kFindMaxima) continue;
+      if (mode == kFirstTile && over && have_row) atomicOr(&bars->redo, 1u << q->bit);
+      l_sum += other;
+      const int head = q->h * a.group + row - row_i * a.group;
       const long long out_row = q->row0 + row_token;
-      // rare: values that the helpers left out are added to the stored row, for the rows that see them
-      auto put_back = [&](auto* dst) {
-        const int end = q->t0 * kKeyTile + min(lim, q->n_tiles * kKeyTile);
-        for (int key = max(q->lim_min & ~(kKeyTile - 1), q->t0 * kKeyTile); key < end; ++key)
-          for (int d = 0; d < kCacheDim; ++d) {
-            const float v = v_value<kFp8>(a, q->b, q->h, key, d);
-            if (!isfinite(v)) dst[d] = static_cast<float>(dst[d]) + v;
-          }
-      };
-      const bool poisoned = bars->poison != 0u;
-      // where this thread's row goes (null: nowhere), as bytes; 8 lanes write a row together
+      // where this thread's half row goes (null: nowhere), as bytes; 8 lanes write a row together
       uint8_t* dst = nullptr;
       if (have_row)
-        dst = q->whole ? reinterpret_cast<uint8_t*>(a.o + out_row * a.o_stride_l + head * a.o_stride_h)
-                       : reinterpret_cast<uint8_t*>(part_slot(a, blockIdx.x, q->tail != 0) + (t * T * a.group + row) * kCacheDim);
+        dst = q->whole ? reinterpret_cast<uint8_t*>(a.o + out_row * a.o_stride_l + head * a.o_stride_h + 64 * hf)
+                       : reinterpret_cast<uint8_t*>(part_slot(a, blockIdx.x, q->tail != 0) + (t * T * a.group + row) * kCacheDim + 64 * hf);
       auto store_pieces = [&](uint32_t* r, int offset) {
         transpose_pieces(r);
 #pragma unroll
@@ -877,41 +906,43 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (to != nullptr) *reinterpret_cast<uint4*>(to + offset + 16 * (lane & 7)) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
         }
       };
-      const float v_unit = kFp8 ? __uint_as_float(static_cast<uint32_t>(vref) << 23) : 1.0f;
+      float unit = 1.0f;
+      if constexpr (kFp8)
+        if (n_mine > 0) unit = __uint_as_float(static_cast<uint32_t>(info[(n_before - 1) % kInfoRing].vref) << 23);
       if (q->whole) {
-        const float inv = (l_sum == 0.f ? 0.f : 1.0f / l_sum) * v_unit;
+        const float inv = (l_sum == 0.f ? 0.f : 1.0f / l_sum) * unit;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          ra[i] = pack_bf16x2(__uint_as_float(ra[2 * i]) * inv, __uint_as_float(ra[2 * i + 1]) * inv);
-          rb[i] = pack_bf16x2(__uint_as_float(rb[2 * i]) * inv, __uint_as_float(rb[2 * i + 1]) * inv);
-        }
-        store_pieces(ra, 0);
-        store_pieces(rb, 128);
-        if (have_row && a.lse)
+        for (int i = 0; i < 32; ++i) s[i] = pack_bf16x2(__uint_as_float(s[2 * i]) * inv, __uint_as_float(s[2 * i + 1]) * inv);
+        store_pieces(s, 0);
+        if (have_row && a.lse && hf == 0)
           a.lse[static_cast<long long>(head) * a.c.rows + out_row] = l_sum == 0.f ? -INFINITY : (m_ref + log2f(l_sum)) * 0.6931471805599453f;
       } else {
-        if constexpr (kFp8) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            ra[i] = __float_as_uint(__uint_as_float(ra[i]) * v_unit);
-            rb[i] = __float_as_uint(__uint_as_float(rb[i]) * v_unit);
-          }
-        }
-        store_pieces(ra, 0);
-        store_pieces(ra + 32, 128);
-        store_pieces(rb, 256);
-        store_pieces(rb + 32, 384);
-        if (have_row) {
+        for (int i = 0; i < 64; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * unit);
+        store_pieces(s, 0);
+        store_pieces(s + 32, 128);
+        if (have_row && hf == 0) {
           float* stat = part_slot(a, blockIdx.x, q->tail != 0) + kTileRows * kCacheDim + t * T * a.group + row;
           stat[0] = m_ref;
           stat[kTileRows] = l_sum;
         }
       }
-      if (poisoned) {
-        __syncwarp();  // the row was stored by its neighbours
+      if (bars->poison != 0u) {  // rare: values that the helpers left out are added to the stored row, for the rows that see them
+        __syncwarp();            // the row was stored by its neighbours
         if (have_row) {
-          if (q->whole) put_back(reinterpret_cast<__nv_bfloat16*>(dst));
-          else put_back(reinterpret_cast<float*>(dst));
+          const int begin = max(q->lim_min & ~(kKeyTile - 1), q->t0 * kKeyTile);
+          const int end = min(lim + hf * 64, q->n_tiles * kKeyTile) + q->t0 * kKeyTile;
+          for (int key = begin; key < end; ++key)
+            for (int d = 0; d < 64; ++d) {
+              const float v = v_value<kFp8>(a, q->b, q->h, key, 64 * hf + d);
+              if (isfinite(v)) continue;
+              if (q->whole) {
+                __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(dst) + d;
+                *o = static_cast<__nv_bfloat16>(static_cast<float>(*o) + v);
+              } else {
+                reinterpret_cast<float*>(dst)[d] += v;
+              }
+            }
         }
       }
     }
@@ -925,7 +956,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
     __syncthreads();
   }
-  if (warp == 9) {
+  if (warp == kIssuerWarp) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
