@@ -242,6 +242,10 @@ __device__ __forceinline__ void describe_piece(const CacheAttnArgs& a, const Sha
   }
 }
 
+// The same value in every lane, in a form that lets the compiler know it: what is computed from it, descriptors of MMAs
+// above all, then lives in uniform registers (moved there from ordinary ones before each, an MMA took 90 cycles to issue).
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xFFFFFFFFu, x); }
+
 // rows [0, box_rows) of a 4-D page box are whole keys of one page: box_rows divides the page size and the tile
 template <bool kFp8>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -259,7 +263,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   uint8_t* smem = smem_raw + (base - raw_addr);
   const uint32_t q_smem = base, ring = base + 2 * kTileBytes, staging = ring + R::kRing * kTileBytes;
   TileBars* bars = reinterpret_cast<TileBars*>(smem + kTileSmemBytes - 1024 - kTileBarBytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < R::kRing; ++i) {
@@ -312,7 +316,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(bars->tmem_base)));
   const TileWait wait{a, bars};
   const int T = a.item_tokens >> 1;
   // the readers' side of the ring of pieces
@@ -339,10 +343,11 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     bool ok = true;
     const TilePiece* q;
     for (; ok && (q = piece()) != nullptr; piece_done()) {
-      const int n_tiles = q->n_tiles, t0 = q->t0, b = q->b, h = q->h, lim_min = q->lim_min, lim_max = q->lim_max;
+      const int n_tiles = uniform(q->n_tiles), t0 = uniform(q->t0), b = uniform(q->b), h = uniform(q->h);
+      const int lim_min = uniform(q->lim_min), lim_max = uniform(q->lim_max);
       if (n_tiles == 0) continue;
-      // e4m3: the exponent bytes of this thread's row are fetched a tile ahead, their page number two tiles ahead
-      uint32_t ex[2] = {0, 0};
+      // e4m3: the exponent bytes of this thread's row are fetched two tiles ahead, their page number three tiles ahead
+      uint32_t ex[2] = {0, 0}, ex_next[2] = {0, 0};  // of the current tile; of the next one
       int id_next = 0;
       uint32_t v_most = 0;  // largest exponent of V in the piece
       if (q->mode != kUseMaxima) vref = 0;  // otherwise what the pass before it found
@@ -350,7 +355,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const int key = tile * kKeyTile + row;
         if (kFp8 && key < lim_max) id_next = __ldg(a.c.pages + b * a.c.pages_stride + a.c.by_page(key));
       };
-      auto fetch_ex = [&](int tile) {
+      auto fetch_ex = [&](uint32_t (&to)[2], int tile) {
         const int key = tile * kKeyTile + row;
         if (kFp8 && key < lim_max) {
           const int at = key - a.c.by_page(key) * a.c.page_size;
@@ -360,16 +365,17 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             id = 0;
           }
 #pragma unroll
-          for (int x = 0; x < 2; ++x) ex[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + h * a.c.exp_head[x]);
+          for (int x = 0; x < 2; ++x) to[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + h * a.c.exp_head[x]);
         }
       };
       // The tile's largest exponents, and V's smallest; rows of nothing (7) and rows that are not finite (255) aside.  Each
       // warp leaves its own, a tile ahead; they meet at a barrier with a bounded wait.
       auto leave_tops = [&](int tile) {
         const bool there = tile * kKeyTile + row < lim_max;
+        const bool v_counts = there && ex[1] != 255u && ex[1] > 7u;
         const uint32_t k_top = __reduce_max_sync(0xFFFFFFFFu, there && ex[0] != 255u ? ex[0] : 0u);
-        const uint32_t v_top = __reduce_max_sync(0xFFFFFFFFu, there && ex[1] != 255u && ex[1] > 7u ? ex[1] : 0u);
-        const uint32_t v_low = __reduce_min_sync(0xFFFFFFFFu, there && ex[1] != 255u && ex[1] > 7u ? ex[1] : 255u);
+        const uint32_t v_top = __reduce_max_sync(0xFFFFFFFFu, v_counts ? ex[1] : 0u);
+        const uint32_t v_low = __reduce_min_sync(0xFFFFFFFFu, v_counts ? ex[1] : 255u);
         if (lane == 0) {
           tops[n_left & 1][warp - kHelperWarp] = k_top | (v_top << 8) | (v_low << 16);
           mbar_arrive(smem_u32(&bars->tops[n_left & 1]));
@@ -378,8 +384,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       };
       if constexpr (kFp8) {
         fetch_id(t0);
-        fetch_ex(t0);
+        fetch_ex(ex, t0);
         fetch_id(t0 + 1);
+        fetch_ex(ex_next, t0 + 1);
+        fetch_id(t0 + 2);
         leave_tops(t0);
       }
       for (int it = 0; ok && it < n_tiles; ++it) {
@@ -391,8 +399,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         bool wide = false;
         if constexpr (kFp8) {
           const uint32_t ek = ex[0], ev = ex[1], par = n_done & 1;
-          if (it + 1 < n_tiles) fetch_ex(tile + 1);
-          fetch_id(tile + 2);
+          ex[0] = ex_next[0];
+          ex[1] = ex_next[1];
+          fetch_ex(ex_next, tile + 2);
+          fetch_id(tile + 3);
           ok = wait(bars->tops[par], (n_done >> 1) & 1, kTileWaitTops);
           if (!ok) break;
           uint32_t kt = 0, vt = 0, vl = 255;
@@ -492,7 +502,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       bool ok = true;
       const TilePiece* q;
       for (; ok && (q = piece()) != nullptr; piece_done()) {
-        const int n_tiles = q->n_tiles, t0 = q->t0, b = q->b, h = q->h, lim_max = q->lim_max;
+        const int n_tiles = uniform(q->n_tiles), t0 = uniform(q->t0), b = uniform(q->b), h = uniform(q->h), lim_max = uniform(q->lim_max);
         if (n_tiles == 0) continue;
         // Q is free late in the previous piece, ring slots earlier: the first two key tiles go ahead of Q
         const int q_at = g > 0 ? min(2, n_tiles - 1) : 0;
@@ -602,7 +612,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       };
       const TilePiece* q;
       for (; ok && (q = piece()) != nullptr; piece_done()) {
-        const int n_tiles = q->n_tiles, n_mine = q->end[t];
+        const int n_tiles = uniform(q->n_tiles), n_mine = uniform(q->end[t]);
         if (n_tiles == 0) continue;
         if (!kFp8) ok = wait(bars->q_full, g & 1, kTileWaitQFull);
         else if (n_mine > 0) ok = wait(bars->q_ready[t], own & 1, kTileWaitQReady);
@@ -727,7 +737,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     };
     const TilePiece* q;
     for (; ok && (q = piece()) != nullptr; piece_done()) {
-      const int n_mine = q->end[t], mode = q->mode;
+      const int n_mine = uniform(q->end[t]), mode = uniform(q->mode);
       const int row_i = a.by_group(row);                  // row r: token r / group, head r % group
       const int row_token = t * T + row_i;
       const bool have_row = row < T * a.group && q->tok0 + row_token < q->n;
