@@ -66,7 +66,6 @@ struct TileBars {
   uint64_t o_free[2];      // the stream's warps have read O
   uint64_t meet[2];        // the stream's eight warps have left what the other half is to see
   uint64_t piece_full[4], piece_empty[4];
-  uint64_t tops[2];        // e4m3: the helper warps' exponents of a tile are there
   uint32_t tmem_base;
   uint32_t early_exit;
   volatile uint32_t abort_flag;
@@ -79,7 +78,7 @@ constexpr int kTileSmemBytes = 2 * kTileBytes + (TileRing<true>::kBytes > TileRi
 static_assert(sizeof(TileBars) <= kTileBarBytes, "shared memory layout");
 enum : int {  // status codes of waits that ran out (low byte of the status word)
   kTileWaitEmpty = 33, kTileWaitFull, kTileWaitReady, kTileWaitUnstaged, kTileWaitStaged, kTileWaitQFull, kTileWaitQEmpty,
-  kTileWaitQReady, kTileWaitTops, kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitMeet, kTileWaitPiece
+  kTileWaitQReady, kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitMeet, kTileWaitPiece
 };
 
 struct TileWait {
@@ -164,11 +163,11 @@ struct TilePiece {
 };
 // e4m3: what a tile's rows were widened with
 struct TileInfo {
-  float k_unit;   // 2^(kref - 127): the tile's logits are in these units
+  int kref;       // the tile's logits are in units of 2^(kref - 127)
   int vref;       // V, and so O, is in units of 2^(vref - 127): the same for a piece's tiles
   int wide;       // V is bf16, and P is to be
 };
-constexpr int kInfoRing = 8;  // the helpers are at most two tiles ahead of the softmax warps
+constexpr int kInfoRing = 8;  // the producer is at most four tiles ahead of the softmax warps
 // 2^-d as an fp16 pair, d >= -15
 __device__ __forceinline__ uint32_t f16x2_pow2_neg(int d) {
   const uint32_t h = d <= 14 ? static_cast<uint32_t>(15 - d) << 10 : d <= 24 ? 1u << (24 - d) : 0u;
@@ -255,8 +254,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   __shared__ ShareStart start;
   __shared__ TilePiece pieces[kPieceRing];  // n_tiles < 0: no more
   __shared__ TileInfo info[kInfoRing];
-  __shared__ uint32_t tops[2][4];           // e4m3: exponents' maxima and minimum of a tile, per helper warp, by tile parity
-  static_assert(kTileSmemBytes + sizeof(ShareStart) + sizeof(TilePiece) * kPieceRing + sizeof(TileInfo) * kInfoRing + 32 <= 232448, "shared memory budget");
+  __shared__ alignas(4) uint8_t exps[kInfoRing][2][kKeyTile];  // e4m3: the exponent bytes of a tile's rows of K and V
+  static_assert(kTileSmemBytes + sizeof(ShareStart) + sizeof(TilePiece) * kPieceRing + (sizeof(TileInfo) + 2 * kKeyTile) * kInfoRing <= 232448, "shared memory budget");
   using R = TileRing<kFp8>;
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -277,8 +276,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     }
     mbar_init(smem_u32(&bars->q_full), 1);
     mbar_init(smem_u32(&bars->q_empty), 2);
-    mbar_init(smem_u32(&bars->tops[0]), 4);
-    mbar_init(smem_u32(&bars->tops[1]), 4);
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&bars->q_ready[t]), 8);
       for (int hf = 0; hf < 2; ++hf) {
@@ -338,107 +335,16 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int row = threadIdx.x - kHelperWarp * 32;
     const uint32_t swz = row & 7;
     int cnt = 0;
-    uint32_t n_done = 0, n_left = 0;  // tiles so far, all pieces
-    uint32_t vref = 0;
+    uint32_t n_done = 0;  // tiles so far, all pieces
     bool ok = true;
     const TilePiece* q;
     for (; ok && (q = piece()) != nullptr; piece_done()) {
-      const int n_tiles = uniform(q->n_tiles), t0 = uniform(q->t0), b = uniform(q->b), h = uniform(q->h);
-      const int lim_min = uniform(q->lim_min), lim_max = uniform(q->lim_max);
+      const int n_tiles = uniform(q->n_tiles), t0 = uniform(q->t0), lim_min = uniform(q->lim_min), lim_max = uniform(q->lim_max);
       if (n_tiles == 0) continue;
-      // e4m3: the exponent bytes of this thread's row are fetched two tiles ahead, their page number three tiles ahead
-      uint32_t ex[2] = {0, 0}, ex_next[2] = {0, 0};  // of the current tile; of the next one
-      int id_next = 0;
-      uint32_t v_most = 0;  // largest exponent of V in the piece
-      if (q->mode != kUseMaxima) vref = 0;  // otherwise what the pass before it found
-      auto fetch_id = [&](int tile) {
-        const int key = tile * kKeyTile + row;
-        if (kFp8 && key < lim_max) id_next = __ldg(a.c.pages + b * a.c.pages_stride + a.c.by_page(key));
-      };
-      auto fetch_ex = [&](uint32_t (&to)[2], int tile) {
-        const int key = tile * kKeyTile + row;
-        if (kFp8 && key < lim_max) {
-          const int at = key - a.c.by_page(key) * a.c.page_size;
-          long long id = id_next;
-          if (static_cast<unsigned>(id_next) >= static_cast<unsigned>(a.c.n_pages)) {
-            report_cache(a.c, b);
-            id = 0;
-          }
-#pragma unroll
-          for (int x = 0; x < 2; ++x) to[x] = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + at * a.c.exp_token[x] + h * a.c.exp_head[x]);
-        }
-      };
-      // The tile's largest exponents, and V's smallest; rows of nothing (7) and rows that are not finite (255) aside.  Each
-      // warp leaves its own, a tile ahead; they meet at a barrier with a bounded wait.
-      auto leave_tops = [&](int tile) {
-        const bool there = tile * kKeyTile + row < lim_max;
-        const bool v_counts = there && ex[1] != 255u && ex[1] > 7u;
-        const uint32_t k_top = __reduce_max_sync(0xFFFFFFFFu, there && ex[0] != 255u ? ex[0] : 0u);
-        const uint32_t v_top = __reduce_max_sync(0xFFFFFFFFu, v_counts ? ex[1] : 0u);
-        const uint32_t v_low = __reduce_min_sync(0xFFFFFFFFu, v_counts ? ex[1] : 255u);
-        if (lane == 0) {
-          tops[n_left & 1][warp - kHelperWarp] = k_top | (v_top << 8) | (v_low << 16);
-          mbar_arrive(smem_u32(&bars->tops[n_left & 1]));
-        }
-        ++n_left;
-      };
-      if constexpr (kFp8) {
-        fetch_id(t0);
-        fetch_ex(ex, t0);
-        fetch_id(t0 + 1);
-        fetch_ex(ex_next, t0 + 1);
-        fetch_id(t0 + 2);
-        leave_tops(t0);
-      }
-      for (int it = 0; ok && it < n_tiles; ++it) {
+      for (int it = 0; ok && it < n_tiles; ++it, ++n_done) {
         const int tile = t0 + it, key = tile * kKeyTile + row;
         const bool special = (tile + 1) * kKeyTile > lim_min;
         const bool gone = key >= lim_max;
-        uint32_t factor[2] = {0, 0};   // e4m3: of this thread's row of K and V
-        bool blank[2] = {gone, gone};  // e4m3: ... which may hold anything, codes for NaN included, and counts as zeros
-        bool wide = false;
-        if constexpr (kFp8) {
-          const uint32_t ek = ex[0], ev = ex[1], par = n_done & 1;
-          ex[0] = ex_next[0];
-          ex[1] = ex_next[1];
-          fetch_ex(ex_next, tile + 2);
-          fetch_id(tile + 3);
-          ok = wait(bars->tops[par], (n_done >> 1) & 1, kTileWaitTops);
-          if (!ok) break;
-          uint32_t kt = 0, vt = 0, vl = 255;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t x = tops[par][w];
-            kt = max(kt, x & 255u);
-            vt = max(vt, (x >> 8) & 255u);
-            vl = min(vl, x >> 16);
-          }
-          v_most = max(v_most, vt);
-          if (vref == 0u) vref = vt != 0u ? vt : 127u;
-          wide = vl + 14u < vref || vt > vref + 7u;
-          // O itself could leave fp32 (the first tile's V next to nothing): with the piece's largest exponent as the unit it cannot
-          if (vt > vref + 40u && row == 0) atomicOr(&bars->redo, 1u << q->bit);
-          if (row == 0) {
-            TileInfo& to = info[n_done % kInfoRing];
-            to.k_unit = __uint_as_float(kt << 23);
-            to.vref = static_cast<int>(vref);
-            to.wide = wide;
-          }
-          factor[0] = ek == 255u ? 0x7FFF7FFFu : f16x2_pow2_neg(static_cast<int>(kt) - static_cast<int>(ek));
-          if (ev == 255u) {
-            factor[1] = 0x7FFF7FFFu;
-            if (special && !gone) {  // put back at the end
-              blank[1] = true;
-              bars->poison = 1u;
-            }
-          } else {
-            factor[1] = wide ? static_cast<uint32_t>(max(0, min(254, 247 + static_cast<int>(ev) - static_cast<int>(vref)))) * 0x800080u
-                             : f16x2_pow2_neg(static_cast<int>(vref) - static_cast<int>(ev));
-          }
-          if (blank[0]) factor[0] = 0;
-          if (blank[1]) factor[1] = 0;
-          ++n_done;
-        }
 #pragma unroll 1
         for (int x = 0; x < 2; ++x, ++cnt) {  // K, then V
           const int s = cnt % R::kRing;
@@ -449,19 +355,25 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             ok = wait(bars->staged[g], (cnt / R::kStaged) & 1, kTileWaitStaged) && wait(bars->empty[s], ph ^ 1u, kTileWaitEmpty);
             if (!ok) break;
             const uint32_t src = staging + g * kCodeBytes + row * 128;
-            const uint32_t f = x ? factor[1] : factor[0];
-            const bool none = x ? blank[1] : blank[0];
-            if (x == 1 && wide) widen_row<true>(src, dst, swz, f, none);
-            else widen_row<false>(src, dst, swz, f, none);
+            // what the producer has found out about the tile; a row that is not there may hold anything, codes for NaN
+            // included, and counts as zeros, as does for now a row that is not finite and that not every query row sees
+            const TileInfo in = info[n_done % kInfoRing];
+            const int e = exps[n_done % kInfoRing][x][row];
+            const bool put_back = x == 1 && special && !gone && e == 255;
+            if (put_back) bars->poison = 1u;
+            const bool none = gone || put_back;
+            const int d = (x ? in.vref : in.kref) - e;  // the row's power of two against the unit's
+            if (x == 1 && in.wide) {
+              const uint32_t f = none ? 0u : e == 255 ? 0x7FFF7FFFu : static_cast<uint32_t>(max(0, min(254, 247 - d))) * 0x800080u;
+              widen_row<true>(src, dst, swz, f, none);
+            } else {
+              widen_row<false>(src, dst, swz, none ? 0u : e == 255 ? 0x7FFF7FFFu : f16x2_pow2_neg(d), none);
+            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
               mbar_arrive(smem_u32(&bars->ready[s]));
               mbar_arrive(smem_u32(&bars->unstaged[g]));
-            }
-            if (x == 1) {
-              if (it + 1 < n_tiles) leave_tops(tile + 1);
-              else if (q->mode == kFindMaxima) vref = v_most != 0u ? v_most : 127u;
             }
           } else {
             ok = wait(bars->full[s], ph, kTileWaitFull);
@@ -498,23 +410,47 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const int box_bytes = box_rows * (kFp8 ? kCacheDim : 2 * kCacheDim);
       const uint32_t q_bytes = T * a.group * 256;
       int cnt = 0;
-      uint32_t g = 0;  // pieces with work so far: the phase of q_full / q_empty
+      uint32_t n_done = 0;  // tiles so far, all pieces
+      int vref = 0;         // e4m3: V's unit in the piece
+      uint32_t g = 0;       // pieces with work so far: the phase of q_full / q_empty
       bool ok = true;
       const TilePiece* q;
       for (; ok && (q = piece()) != nullptr; piece_done()) {
         const int n_tiles = uniform(q->n_tiles), t0 = uniform(q->t0), b = uniform(q->b), h = uniform(q->h), lim_max = uniform(q->lim_max);
+        const int mode = uniform(q->mode);
         if (n_tiles == 0) continue;
         // Q is free late in the previous piece, ring slots earlier: the first two key tiles go ahead of Q
         const int q_at = g > 0 ? min(2, n_tiles - 1) : 0;
         bool q_loaded = false;
-        // page of this lane's sub-box of a tile, fetched a tile ahead; none behind the last key
-        int id = 0;
-        auto has_box = [&](int tile) { return lane < n_boxes && tile * kKeyTile + lane * box_rows < lim_max; };
-        auto fetch_page = [&](int tile) {
-          if (has_box(tile)) id = __ldg(a.c.pages + b * a.c.pages_stride + a.c.by_page(tile * kKeyTile + lane * box_rows));
+        // A lane looks after 4 rows of every tile, which are in one page.  Its page number is fetched two tiles ahead, the rows'
+        // exponent bytes (e4m3) one tile ahead; nothing looks at either before it is needed, or the loads would be waited for.
+        int id = 0, id_next = 0;
+        uint32_t raw_k[4] = {}, raw_v[4] = {};
+        auto fetch_id = [&](int tile) {
+          const int key = tile * kKeyTile + lane * 4;
+          return key < lim_max ? __ldg(a.c.pages + b * a.c.pages_stride + a.c.by_page(key)) : 0;
         };
-        fetch_page(t0);
-        for (int it = 0; ok && it < n_tiles; ++it) {
+        auto checked = [&](int raw) {  // a page that does not exist is reported, and some other page read
+          if (static_cast<unsigned>(raw) < static_cast<unsigned>(a.c.n_pages)) return raw;
+          report_cache(a.c, b);
+          return 0;
+        };
+        auto fetch_ex = [&](int tile, int page) {
+          const int key = tile * kKeyTile + lane * 4, at = key - a.c.by_page(key) * a.c.page_size;
+          const uint8_t* from_k = a.c.exps[0] + page * a.c.exp_page[0] + at * a.c.exp_token[0] + h * a.c.exp_head[0];
+          const uint8_t* from_v = a.c.exps[1] + page * a.c.exp_page[1] + at * a.c.exp_token[1] + h * a.c.exp_head[1];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            raw_k[i] = key + i < lim_max ? __ldg(from_k + i * a.c.exp_token[0]) : 0u;
+            raw_v[i] = key + i < lim_max ? __ldg(from_v + i * a.c.exp_token[1]) : 0u;
+          }
+        };
+        id = checked(fetch_id(t0));
+        id_next = fetch_id(t0 + 1);
+        if constexpr (kFp8) fetch_ex(t0, id);
+        int v_most = 0;                       // largest exponent of V in the piece
+        if (mode != kUseMaxima) vref = 0;     // otherwise what the pass before found
+        for (int it = 0; ok && it < n_tiles; ++it, ++n_done) {
           if (!q_loaded) {
             bool q_free = g == 0 || __all_sync(0xFFFFFFFFu, mbar_test_wait(smem_u32(&bars->q_empty), (g - 1) & 1));
             if (!q_free && it >= q_at) {
@@ -536,16 +472,44 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
           }
           const int tile = t0 + it;
+          // sub-box x of the tile: lane x copies it; none behind the last key
           const int key = tile * kKeyTile + lane * box_rows, at = key - a.c.by_page(key) * a.c.page_size;
-          const bool mine = has_box(tile);
+          const bool mine = lane < n_boxes && key < lim_max;
           const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, mine)) * box_bytes;
-          int now = id;
-          if (mine && static_cast<unsigned>(id) >= static_cast<unsigned>(a.c.n_pages)) {  // reported, and some other page read
-            report_cache(a.c, b);
-            now = 0;
-          }
-          fetch_page(tile + 1);
+          const int page = __shfl_sync(0xFFFFFFFFu, id, (lane * box_rows / 4) & 31);
+          if constexpr (kFp8) {
+            // the tile's largest exponents, and V's smallest; rows of nothing (7) and rows that are not finite (255) aside
+            uint32_t k_top = 0, v_top = 0, v_low = 255;
 #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x = raw_k[i], y = raw_v[i];
+              if (x != 255u) k_top = max(k_top, x);
+              if (y > 7u && y != 255u) {
+                v_top = max(v_top, y);
+                v_low = min(v_low, y);
+              }
+            }
+            k_top = __reduce_max_sync(0xFFFFFFFFu, k_top);
+            v_top = __reduce_max_sync(0xFFFFFFFFu, v_top);
+            v_low = __reduce_min_sync(0xFFFFFFFFu, v_low);
+            const int vt = static_cast<int>(v_top), vl = static_cast<int>(v_low);
+            v_most = max(v_most, vt);
+            if (vref == 0) vref = vt != 0 ? vt : 127;
+            const uint32_t slot = n_done % kInfoRing;
+            *reinterpret_cast<uint32_t*>(&exps[slot][0][4 * lane]) = raw_k[0] | (raw_k[1] << 8) | (raw_k[2] << 16) | (raw_k[3] << 24);
+            *reinterpret_cast<uint32_t*>(&exps[slot][1][4 * lane]) = raw_v[0] | (raw_v[1] << 8) | (raw_v[2] << 16) | (raw_v[3] << 24);
+            if (lane == 0) {
+              info[slot].kref = static_cast<int>(k_top);
+              info[slot].vref = vref;
+              info[slot].wide = vl + 14 < vref || vt > vref + 7;
+              // O itself could leave fp32 (the first tile's V next to nothing): with the piece's largest exponent as the unit it cannot
+              if (vt > vref + 40) atomicOr(&bars->redo, 1u << q->bit);
+            }
+          }
+          id = checked(id_next);
+          id_next = fetch_id(tile + 2);
+          if constexpr (kFp8) fetch_ex(tile + 1, id);
+#pragma unroll 1
           for (int x = 0; x < 2; ++x, ++cnt) {
             const CUtensorMap* tm = x ? &tm_v : &tm_k;
             uint32_t dst, bar;
@@ -561,15 +525,17 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               bar = smem_u32(&bars->full[s]);
             }
             if (!ok) break;
+            __syncwarp();  // with what was left about the tile
             if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
             __syncwarp();
             if (mine) {
-              tma_load_4d(dst, tm, bar, 0, at, h, now);
-              if constexpr (!kFp8) tma_load_4d(dst + kTileHalf, tm, bar, 64, at, h, now);
+              tma_load_4d(dst, tm, bar, 0, at, h, page);
+              if constexpr (!kFp8) tma_load_4d(dst + kTileHalf, tm, bar, 64, at, h, page);
             }
             __syncwarp();
           }
         }
+        if (mode == kFindMaxima) vref = v_most != 0 ? v_most : 127;
         ++g;
       }
     } else if (warp < kPieceWarp) {
@@ -795,7 +761,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         bool wide = false;
         if constexpr (kFp8) {
           const TileInfo& in = info[(n_before + it) % kInfoRing];
-          c = fminf(row_unit * in.k_unit, 3.0e38f);
+          c = fminf(row_unit * __uint_as_float(static_cast<uint32_t>(in.kref) << 23), 3.0e38f);
           wide = in.wide != 0;
         }
         const bool partly = (it + 1) * kKeyTile - 64 > lim_first;
