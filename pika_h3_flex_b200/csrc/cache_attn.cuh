@@ -9,6 +9,11 @@
 // an SM.  An item that crosses a cut leaves fp32 partial results (O, running maximum, sum) in the workspace; a second small
 // launch joins them in order of the keys, so results do not depend on timing.  A CTA has at most two such pieces (its
 // first and its last), which bounds the workspace by the number of SMs, not by the batch.
+//
+// Laid end to end, neighbouring CTAs are at different keys of different heads at any moment, and where K and V do not fit
+// L2 every CTA fetches them from HBM for itself (40 heads of 49,384 keys: 18 of the 19 GB that the items read).  So where
+// all items cost the same and there are more of them than CTAs (one sequence without a causal mask), whole items are dealt
+// out in rounds, the CTAs of a round walking the same few heads' keys in step, and only the last, partial round is cut.
 #pragma once
 #include "kv_cache.cuh"
 
@@ -85,11 +90,24 @@ struct ShareIter {
   int n_shares;
   int b, h, it;
   AttnSeq s;
+  int whole, whole_item;  // whole items dealt to this CTA and not yet begun; number of the next one
 
   __device__ __forceinline__ void skip_empty(const CacheAttnArgs& a) {
     while (s.n_items == 0 && b + 1 < a.c.n_seqs) s = attn_seq(a, ++b);
   }
   __device__ __forceinline__ bool next(const CacheAttnArgs& a, Piece& p) {
+    if (whole > 0) {
+      p.b = b;
+      p.h = whole_item / s.n_items;
+      p.it = whole_item - p.h * s.n_items;
+      p.s = s;
+      p.t0 = 0;
+      p.t1 = item_tiles(a, s, p.it);
+      p.first = p.last = true;
+      whole_item += gridDim.x;
+      --whole;
+      return true;
+    }
     if (pos >= end) return false;
     const int units = 1 + item_tiles(a, s, it);
     const int u0 = static_cast<int>(pos - item_base);
@@ -160,6 +178,22 @@ __device__ __forceinline__ void share_item(const CacheAttnArgs& a, ShareIter& s,
 __device__ __forceinline__ ShareIter share_begin(const CacheAttnArgs& a, ShareStart* sh) {
   const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   ShareIter s;
+  s.whole = s.whole_item = 0;
+  if (a.c.n_seqs == 1 && !a.causal && a.item_tokens > 0) {
+    s.b = 0;
+    s.s = attn_seq(a, 0);
+    const int n_items = s.s.n_items * a.c.kv_heads, units = 1 + item_tiles(a, s.s, 0);
+    s.whole = n_items / gridDim.x;
+    s.whole_item = blockIdx.x;
+    const int dealt = s.whole * gridDim.x;
+    s.total = static_cast<long long>(n_items - dealt) * units;
+    share_range(a, s);
+    const int ahead = static_cast<int>(div_units(s.pos, units));  // items of the last round before this share's first
+    s.item_base = static_cast<long long>(ahead) * units;
+    s.h = s.s.n_items > 0 ? (dealt + ahead) / s.s.n_items : 0;
+    s.it = dealt + ahead - s.h * s.s.n_items;
+    return s;
+  }
   if (a.c.n_seqs <= 32) {
     AttnSeq q{0, 0, 0, 0};
     long long head_total = 0;

@@ -253,9 +253,11 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   extern __shared__ uint8_t smem_raw[];
   __shared__ ShareStart start;
   __shared__ TilePiece pieces[kPieceRing];  // n_tiles < 0: no more
+  __shared__ ShareIter walk, again;         // the piece warp's: where it is in the share, where its batch began
+  __shared__ Piece p;
   __shared__ TileInfo info[kInfoRing];
   __shared__ alignas(4) uint8_t exps[kInfoRing][2][kKeyTile];  // e4m3: the exponent bytes of a tile's rows of K and V
-  static_assert(kTileSmemBytes + sizeof(ShareStart) + sizeof(TilePiece) * kPieceRing + (sizeof(TileInfo) + 2 * kKeyTile) * kInfoRing <= 232448, "shared memory budget");
+  static_assert(kTileSmemBytes + sizeof(ShareStart) + sizeof(TilePiece) * kPieceRing + 2 * sizeof(ShareIter) + sizeof(Piece) + (sizeof(TileInfo) + 2 * kKeyTile) * kInfoRing <= 232448, "shared memory budget");
   using R = TileRing<kFp8>;
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -303,7 +305,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     prefetch_tmap(&tm_v);
   }
   allow_next_launch();
-  ShareIter iter = share_begin(a, &start);
+  {
+    const ShareIter begin = share_begin(a, &start);
+    if (threadIdx.x == kPieceWarp * 32) walk = begin;
+  }
   __syncthreads();  // barriers and flags are set up
   if (bars->early_exit) return;
   if (warp == kIssuerWarp) {
@@ -629,7 +634,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
     } else if (lane == 0) {
       // ========================================================= the share's pieces, one after the other
-      Piece p;
       uint32_t n = 0;  // pieces handed out
       bool ok = true;
       auto hand_out = [&](const ShareIter& at, int mode, int bit) {
@@ -648,9 +652,9 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       };
       bool more = true;
       while (ok && more) {
-        ShareIter again = iter;
+        again = walk;
         int in_batch = 0;
-        while (ok && in_batch < kPieceBatch && (more = iter.next(a, p))) hand_out(iter, kFirstTile, in_batch++);
+        while (ok && in_batch < kPieceBatch && (more = walk.next(a, p))) hand_out(walk, kFirstTile, in_batch++);
         if (ok) all_done();
         if (!ok) break;
         const uint32_t redo = bars->redo;
