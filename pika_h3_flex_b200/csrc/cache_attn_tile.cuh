@@ -66,8 +66,10 @@ struct TileBars {
   uint64_t o_free[2];      // the stream's warps have read O
   uint64_t meet[2];        // the stream's eight warps have left what the other half is to see
   uint64_t piece_full[4], piece_empty[4];
+  uint64_t tmem_ready;
   uint32_t tmem_base;
   uint32_t early_exit;
+  uint32_t more;             // the share has a piece at all
   volatile uint32_t abort_flag;
   volatile uint32_t poison;  // some V value counted as zero: from then on every epilogue looks for such values
   uint32_t redo;             // pieces of the current batch that outgrew their reference, a bit each
@@ -78,7 +80,7 @@ constexpr int kTileSmemBytes = 2 * kTileBytes + (TileRing<true>::kBytes > TileRi
 static_assert(sizeof(TileBars) <= kTileBarBytes, "shared memory layout");
 enum : int {  // status codes of waits that ran out (low byte of the status word)
   kTileWaitEmpty = 33, kTileWaitFull, kTileWaitReady, kTileWaitUnstaged, kTileWaitStaged, kTileWaitQFull, kTileWaitQEmpty,
-  kTileWaitQReady, kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitMeet, kTileWaitPiece
+  kTileWaitQReady, kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitMeet, kTileWaitPiece, kTileWaitTmem
 };
 
 struct TileWait {
@@ -183,7 +185,7 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 // one before it, and the helpers for them all (1,100 cycles for 16 KB).
 template <bool kBf16>
 __device__ __forceinline__ void widen_row(uint32_t src, uint32_t dst, uint32_t swz, uint32_t f, bool blank) {
-#pragma unroll
+#pragma unroll 1
   for (int c0 = 0; c0 < 8; c0 += 4) {
     uint4 w[4];
 #pragma unroll
@@ -202,7 +204,7 @@ __device__ __forceinline__ void widen_row(uint32_t src, uint32_t dst, uint32_t s
           o[2 * y + 1] = mul_f16x2(e4m3_high_to_f16x2(in[y]), f);
         }
       }
-      const uint32_t at = dst + ((c0 + c) >> 2) * kTileHalf;
+      const uint32_t at = dst + (c0 >> 2) * kTileHalf;
       st_shared_v4(at + (((2 * c) ^ swz) << 4), o[0], o[1], o[2], o[3]);
       st_shared_v4(at + (((2 * c + 1) ^ swz) << 4), o[4], o[5], o[6], o[7]);
     }
@@ -278,6 +280,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     }
     mbar_init(smem_u32(&bars->q_full), 1);
     mbar_init(smem_u32(&bars->q_empty), 2);
+    mbar_init(smem_u32(&bars->tmem_ready), 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&bars->q_ready[t]), 8);
       for (int hf = 0; hf < 2; ++hf) {
@@ -306,19 +309,16 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   }
   allow_next_launch();
   {
-    const ShareIter begin = share_begin(a, &start);
-    if (threadIdx.x == kPieceWarp * 32) walk = begin;
+    ShareIter begin = share_begin(a, &start);
+    if (threadIdx.x == kPieceWarp * 32) {  // the first piece is found here, in registers: everybody waits for it
+      again = begin;
+      bars->more = begin.next(a, p);
+      if (bars->more) describe_piece(a, begin, p, pieces[0]);
+      walk = begin;
+    }
   }
   __syncthreads();  // barriers and flags are set up
   if (bars->early_exit) return;
-  if (warp == kIssuerWarp) {
-    tmem_alloc(smem_u32(&bars->tmem_base), 512);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(bars->tmem_base)));
   const TileWait wait{a, bars};
   const int T = a.item_tokens >> 1;
   // the readers' side of the ring of pieces
@@ -332,6 +332,13 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&bars->piece_empty[n_pieces % kPieceRing]));
     ++n_pieces;
+  };
+
+  // Tensor memory is allocated by the first issuer while the first tiles are on their way; who uses it waits for that.
+  auto tensor_memory = [&](bool& ok) -> uint32_t {
+    ok = wait(bars->tmem_ready, 0, kTileWaitTmem);
+    tc_fence_after_sync();
+    return static_cast<uint32_t>(uniform(static_cast<int>(bars->tmem_base)));
   };
 
   if (warp >= kHelperWarp) {
@@ -553,13 +560,21 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const uint64_t q_desc = umma_desc_sw128(q_smem + t * kTileBytes, 16, 1024);
       const uint64_t k_desc0 = umma_desc_sw128(ring, 16, 1024);
       const uint64_t v_desc0 = umma_desc_sw128(ring, kTileHalf, 1024);
+      if (t == 0) {
+        tmem_alloc(smem_u32(&bars->tmem_base), 512);
+        tmem_relinquish();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars->tmem_ready));
+      }
+      bool ok = true;
+      const uint32_t tmem = tensor_memory(ok);
       const uint32_t s_tmem = tmem + t * 128, o_tmem = tmem + 256 + t * 128;
       uint32_t p_cnt[2] = {0, 0};  // P halves consumed so far: the phase of p_full
       uint32_t pv_cnt = 0;         // P V groups of the current piece: the first one overwrites O
       uint32_t g = 0;              // pieces with work so far
       uint32_t own = 0;            // pieces in which this stream had work: the phase of o_free
       int c0 = 0;                  // ring tiles before the current piece
-      bool ok = true;
       auto issue_s = [&](int hf, int s) {
         const uint64_t kd = k_desc0 + static_cast<uint64_t>((s * kTileBytes + hf * 8192) >> 4);
 #pragma unroll
@@ -650,10 +665,15 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         for (uint32_t k = n < kPieceRing ? 0 : n - kPieceRing; ok && k < n; ++k)
           ok = wait.one(bars->piece_empty[k % kPieceRing], (k / kPieceRing) & 1, kTileWaitPiece);
       };
-      bool more = true;
+      bool more = bars->more != 0u;
+      int in_batch = 0;
+      if (more) {  // the first piece has been described already
+        pieces[0].mode = kFirstTile;
+        pieces[0].bit = in_batch++;
+        mbar_arrive(smem_u32(&bars->piece_full[0]));
+        n = 1;
+      }
       while (ok && more) {
-        again = walk;
-        int in_batch = 0;
         while (ok && in_batch < kPieceBatch && (more = walk.next(a, p))) hand_out(walk, kFirstTile, in_batch++);
         if (ok) all_done();
         if (!ok) break;
@@ -668,6 +688,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         if (redo != 0u && ok) all_done();
         bars->redo = 0;
+        again = walk;
+        in_batch = 0;
       }
       if (ok) {
         const uint32_t i = n % kPieceRing;
@@ -684,6 +706,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int t = (warp >> 2) & 1, hf = warp >> 3, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    bool ok = true;
+    const uint32_t tmem = tensor_memory(ok);
     const uint32_t s_addr = tmem + lane_base + t * 128 + hf * 64;
     const uint32_t o_addr = tmem + lane_base + 256 + t * 128 + hf * 64;  // epilogue: this warpgroup's 64 columns of O
     constexpr float kLift = kFp8 ? 2.f : 0.f;            // the reference's own term is 2^kLift
@@ -693,7 +717,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     uint32_t g = 0;         // e4m3: pieces with work, the phase of q_full
     uint32_t n_before = 0;  // tiles of the pieces before
     uint32_t turn = 0;      // meetings of the stream's two halves so far
-    bool ok = true;
     // Leaves x for the same row's thread of the other half and returns what that one left.  Each side's values are in a
     // slot by turn: nobody can be two meetings ahead of a reader.
     auto exchange = [&](float x) -> float {
@@ -805,7 +828,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         float l_half = 0.f;
         const uint64_t c2 = pack2(c, c), nm2 = pack2(-m_ref, -m_ref);
         auto half = [&](auto pack) {
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < 2; ++x) {
             uint32_t r[32], o[16];
             load(r, x);
@@ -938,7 +961,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   }
   if (warp == kIssuerWarp) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(bars->tmem_base, 512);
   }
 }
 

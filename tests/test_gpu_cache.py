@@ -6,6 +6,11 @@ read back is a bf16 number.  Attention tolerance, element by element, with u = 2
   u A            the rounding of each probability before P V, where A = sum_j softmax_j |v_j|,
   2 (ds + r) A   errors of the logits and of the exponentials: ds = scale (max_j sum_d |q_d k_jd|) 128 2^-23 (fp32 sums of 128
                  exact products, truncating adders allowed for), r = 2^-20 (exponential, scaling, 8-bit lazy rescale, sums),
+and for a quantised cache, whose probabilities are fp16 numbers with a last place of 2^-24, so that terms far below the row's
+largest vanish however large the relative error of one that stands alone would be: at most half of that place a term, against
+a largest term of at least 2^2 (many rows) or 2^6 (few rows; each relative to V's unit, which is at most 2^8 above the row's
+own), divided by a sum that is at least the largest term:
+  2^-25 2^-2 S  or  2^-25 2^-6 2^8 S,  S = sum_j |v_j| over the keys the row sees,
 and for the log-sum-exp ds + (keys) 2^-24 + 2^-21 (1 + |lse| + max logit)."""
 import math
 
@@ -121,6 +126,8 @@ class Case:
         """(out, lse, tolerance of out, tolerance of lse) in 64 bits, on the GPU."""
         dev, group = "cuda", self.heads // self.kv_heads
         q = (self.q if q is None else q).to(dev).double()
+        few = -(-self.rows // len(self.n)) * group <= 16  # which kernel runs: the average sequence's rows per K/V head
+        absolute = (2.0 ** -23 if few else 2.0 ** -27) if self.quantised else 0.0
         out = torch.zeros(self.rows, self.heads, D, dtype=torch.float64, device=dev)
         tol = torch.zeros_like(out)
         lse = torch.full((self.heads, self.rows), -math.inf, dtype=torch.float64, device=dev)
@@ -152,7 +159,7 @@ class Case:
             a = w @ vz.abs()
             r = slice(self.starts[b], self.starts[b] + n)
             out[r] = o.transpose(0, 1)
-            tol[r] = (U * o.abs() + (U + 2 * (ds + 2.0 ** -20))[..., None] * a).transpose(0, 1)
+            tol[r] = (U * o.abs() + (U + 2 * (ds + 2.0 ** -20))[..., None] * a + absolute * (seen.double() @ vz.abs())).transpose(0, 1)
             lse[:, r] = torch.where(l == 0, torch.full_like(l, -math.inf), l.log() + m0)
             ltol[:, r] = ds + length * 2.0 ** -24 + 2.0 ** -21 * (1 + m0.abs() + (l.clamp(min=1e-300).log() + m0).abs())
         return out, lse, tol, ltol
@@ -331,15 +338,33 @@ def test_hidden_values_that_are_not_finite(h, n, length, quantised):
     assert torch.isfinite(out[: n // 2].float()).all()
 
 
+@pytest.mark.parametrize("quantised", [False, True])
 @pytest.mark.parametrize("n,length", [(1, 5000), (2, 200), (64, 3000), (300, 2000)])
-def test_large_logits_and_growing_maxima(h, n, length):
+def test_large_logits_and_growing_maxima(h, n, length, quantised):
     """Keys whose logits grow along the sequence far past the range of the exponential: every tile moves the maximum."""
-    c = Case(h, [n], [length], 2, 1, 16, False, seed=n)
+    c = Case(h, [n], [length], 2, 1, 16, quantised, seed=n)
     c.k[0] = (c.k[0].float() * torch.linspace(0.1, 30, length)[:, None, None]).bfloat16()
     c.q = (c.q.float() * 4).bfloat16()
     c.fill().check(True)
     c.k[0] = c.k[0].flip(0)
     c.fill().check(False)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_many_short_pieces_some_done_twice(h, quantised):
+    """More pieces per SM than are handed out at a time, of more sequences than a warp looks over, in some of which late
+    keys outgrow the first ones."""
+    c = Case(h, [20 + b % 5 for b in range(200)], [150 + b for b in range(200)], 32, 32, 16, quantised, seed=1)
+    for b in range(0, 200, 7):
+        c.k[b][140:] *= 30
+    c.fill().check(True)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("n,length,heads,kv_heads", [(2000, 300, 40, 40), (2100, 129, 40, 8), (9600, 77, 4, 4)])
+def test_whole_items_in_rounds(h, n, length, heads, kv_heads, quantised):
+    """One sequence without a mask and with more items than SMs: whole items are dealt out, the rest is cut."""
+    Case(h, [n], [length], heads, kv_heads, 32, quantised, seed=n).fill().check(False)
 
 
 def test_quantised_rows_of_very_different_sizes(h):
