@@ -435,6 +435,9 @@ typedef struct h3a_cache_attn_params {
   int32_t heads;          /* query heads, a multiple of cache.heads */
   int32_t causal;
   float softmax_scale;    /* <= 0 selects 1/sqrt(d) */
+  int32_t max_new;        /* optional: the most rows any one sequence has (0: unknown).  It only chooses the kernel - up to 16
+                             query rows per K/V head, or more - which otherwise goes by the average; say it for batches that
+                             mix single tokens with long chunks. */
   void* workspace;        /* h3a_cache_attn_workspace_bytes() bytes, 16-byte aligned; used by this call alone until it is done */
   size_t workspace_bytes;
   int32_t* status_word;   /* as in h3a_attn_params */

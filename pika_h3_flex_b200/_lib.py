@@ -138,7 +138,7 @@ class CacheAttnParams(C.Structure):
         ("cache", Cache), ("batch", CacheBatch),
         ("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
         ("q_stride_l", C.c_int64), ("q_stride_h", C.c_int64), ("o_stride_l", C.c_int64), ("o_stride_h", C.c_int64),
-        ("heads", C.c_int32), ("causal", C.c_int32), ("softmax_scale", C.c_float),
+        ("heads", C.c_int32), ("causal", C.c_int32), ("softmax_scale", C.c_float), ("max_new", C.c_int32),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status_word", C.c_void_p), ("wait_limit_ns", C.c_int64),
     ]
 

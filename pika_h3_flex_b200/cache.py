@@ -193,29 +193,31 @@ def cache_read(cache: KVCache, batch: CacheBatch, rows: Optional[int] = None, ou
 
 
 @lru_cache(maxsize=256)
-def _workspace_bytes(device_index: int, rows: int, n_seqs: int, heads: int, kv_heads: int, quantised: bool) -> int:
+def _workspace_bytes(device_index: int, rows: int, n_seqs: int, heads: int, kv_heads: int, quantised: bool, max_new: int) -> int:
     p = _lib.CacheAttnParams()
-    p.cache.heads, p.cache.quantised, p.batch.rows, p.batch.n_seqs, p.heads = kv_heads, int(quantised), rows, n_seqs, heads
+    p.cache.heads, p.cache.quantised, p.batch.rows, p.batch.n_seqs, p.heads, p.max_new = kv_heads, int(quantised), rows, n_seqs, heads, max_new
     need = C.c_size_t(0)
     with torch.cuda.device(device_index):
         check(_lib.load().h3a_cache_attn_workspace_bytes(C.byref(p), C.byref(need)), "h3a_cache_attn_workspace_bytes")
     return int(need.value)
 
 
-def cache_attn_workspace_bytes(cache: KVCache, batch: CacheBatch, rows: int, heads: int) -> int:
+def cache_attn_workspace_bytes(cache: KVCache, batch: CacheBatch, rows: int, heads: int, max_new: Optional[int] = None) -> int:
     """Bytes of device scratch a ``cache_attn`` call of this shape needs; callers in a loop can allocate it once (one
     per stream: calls that may run at the same time must not share it)."""
-    return _workspace_bytes(cache.device.index, int(rows), batch._c.n_seqs, int(heads), cache.heads, cache.quantised)
+    return _workspace_bytes(cache.device.index, int(rows), batch._c.n_seqs, int(heads), cache.heads, cache.quantised, int(max_new or 0))
 
 
 def cache_attn(q: torch.Tensor, cache: KVCache, batch: CacheBatch, causal: bool = True, softmax_scale: float = 0.0,
                out: Optional[torch.Tensor] = None, return_lse: bool = False, status_word: Optional[torch.Tensor] = None,
-               workspace: Optional[torch.Tensor] = None, wait_limit_ns: int = 0):
+               workspace: Optional[torch.Tensor] = None, wait_limit_ns: int = 0, max_new: Optional[int] = None):
     """Attention of the batch's rows ``q [rows, heads, 128]`` bf16 over their sequences' cached keys; ``heads`` is a
     multiple of the cache's (query head h reads K/V head ``h // (heads // cache.heads)``).  ``causal``: row i of a sequence
     is the token at position ``lengths[b] - n_b + i`` and sees the keys up to itself (write its K and V first); otherwise
     every row sees all ``lengths[b]`` keys.  A row without a key is zeros (lse -inf).  Returns ``out [rows, heads, 128]``
-    bf16 (and ``lse [heads, rows]``); rows outside every sequence are not written.  ``softmax_scale`` 0: ``1/sqrt(128)``."""
+    bf16 (and ``lse [heads, rows]``); rows outside every sequence are not written.  ``softmax_scale`` 0: ``1/sqrt(128)``.
+    ``max_new``, the most rows any one sequence has, only chooses the kernel, which otherwise goes by the average: worth
+    saying for a batch that mixes single tokens with long chunks."""
     _require_cuda(q)
     device = cache.device
     H = q.shape[1] if q.dim() == 3 else 0
@@ -236,11 +238,11 @@ def cache_attn(q: torch.Tensor, cache: KVCache, batch: CacheBatch, causal: bool 
     if L == 0:
         return (out, lse) if return_lse else out
     if workspace is None:
-        workspace = torch.empty(_workspace_bytes(device.index, L, batch._c.n_seqs, H, cache.heads, cache.quantised), dtype=torch.uint8, device=device)
+        workspace = torch.empty(_workspace_bytes(device.index, L, batch._c.n_seqs, H, cache.heads, cache.quantised, max_new or 0), dtype=torch.uint8, device=device)
     elif workspace.device != device:
         raise ValueError(f"expected everything on {device}, got the workspace on {workspace.device}")
     p = _lib.CacheAttnParams(cache._c, batch._c, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, qsl, qsh, osl, osh,
-                             H, 1 if causal else 0, softmax_scale, workspace.data_ptr(), workspace.nbytes, status, wait_limit_ns)
+                             H, 1 if causal else 0, softmax_scale, max_new or 0, workspace.data_ptr(), workspace.nbytes, status, wait_limit_ns)
     p.batch.rows = L
     with _on(device):
         check(_lib.load().h3a_cache_attn(C.byref(p), _stream(device)), "h3a_cache_attn")

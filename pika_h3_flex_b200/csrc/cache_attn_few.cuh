@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
   extern __shared__ __align__(16) uint8_t few_raw[];
   FewSmem<kNT>& sm = *reinterpret_cast<FewSmem<kNT>*>(few_raw);
   __shared__ ShareStart start;
-  if (a.c.status && *reinterpret_cast<volatile int*>(a.c.status) != 0) return;
+  if (block_stops(a.c)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
   constexpr int kRows = 8 * kNT;

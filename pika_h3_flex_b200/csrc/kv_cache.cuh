@@ -52,6 +52,13 @@ __device__ __forceinline__ void report_cache(const CacheArgs& a, int b) {
   if (a.status) atomicCAS(a.status, 0, kBadCacheIndex | ((b & 0x7FFFFF) << 8));
 }
 
+// Whether an earlier launch, or an earlier block of this one, has set the status word: one verdict for the whole block, whose
+// threads go on to share memory.
+__device__ __forceinline__ bool block_stops(const CacheArgs& a) {
+  if (a.status == nullptr) return false;
+  return __syncthreads_or(*reinterpret_cast<volatile int*>(a.status) != 0) != 0;
+}
+
 // One sequence of the batch, with every number brought into its range (what is outside is reported).
 struct CacheSeq {
   int s0, n, len;
@@ -161,7 +168,7 @@ constexpr int kUnroll = kWrite && kQuantised ? 4 : 8;  // quantising wants regis
 constexpr int kExpRows = 256;  // rows of a token between two meetings of the exponent bytes
 template <bool kWrite, bool kQuantised>
 __global__ void __launch_bounds__(kRowThreads) cache_rows_kernel(const __grid_constant__ RowsArgs a, const int per_token) {
-  if (a.c.status && *reinterpret_cast<volatile int*>(a.c.status) != 0) return;
+  if (block_stops(a.c)) return;
   constexpr int kRowUnroll = kUnroll<kWrite, kQuantised>;
   const int lane = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const uint32_t half_mask = (threadIdx.x & 16) ? 0xFFFF0000u : 0x0000FFFFu;

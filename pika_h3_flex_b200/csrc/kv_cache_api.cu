@@ -165,8 +165,10 @@ struct AttnPlan {
 AttnPlan attn_plan(const h3a_cache_attn_params* p, int sms) {
   AttnPlan n;
   const int group = p->heads / p->cache.heads;
-  // query rows per K/V head of an average sequence: the lengths themselves are known on the device only
-  const int64_t rows = (static_cast<int64_t>(p->batch.rows) + p->batch.n_seqs - 1) / p->batch.n_seqs * group;
+  // query rows per K/V head: of the longest sequence, if the caller says so, else of the average one (the numbers
+  // themselves are known on the device only); either kernel computes any batch
+  const int64_t tokens = p->max_new > 0 ? p->max_new : (static_cast<int64_t>(p->batch.rows) + p->batch.n_seqs - 1) / p->batch.n_seqs;
+  const int64_t rows = tokens * group;
   if (rows > h3a::kFewRows && group <= 128) {
     n.item_rows = h3a::kTileRows;
     n.item_tokens = 2 * (128 / group);
@@ -272,8 +274,8 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   int32_t rc = cache_args(&p->cache, &p->batch, p->status_word, &a.c);
   if (rc != H3A_OK) return rc;
   if (p->heads <= 0 || p->heads % p->cache.heads || static_cast<int64_t>(p->batch.rows) * p->heads >= (1ll << 31)) return H3A_ERR_SHAPE;
-  if (p->causal != 0 && p->causal != 1) return H3A_ERR_ARG;
-  if (!aligned16(p->q) || !aligned16(p->o) || !rows16(p->q_stride_l, 2, true) || !rows16(p->q_stride_h, 2, true) || !rows16(p->o_stride_l, 2) ||
+  if ((p->causal != 0 && p->causal != 1) || p->max_new < 0) return H3A_ERR_ARG;
+  if (!aligned16(p->q) || !aligned16(p->o) || !rows16(p->q_stride_l, 2) || !rows16(p->q_stride_h, 2) || !rows16(p->o_stride_l, 2) ||
       !rows16(p->o_stride_h, 2))
     return H3A_ERR_ALIGN;
   Device dev;

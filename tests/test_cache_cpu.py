@@ -45,8 +45,8 @@ BAD = [
     ("batch.rows", 0, "SHAPE"), ("batch.rows", 1 << 30, "SHAPE"),
     ("cache.k", BASE + 2, "ALIGN"), ("cache.v_stride_token", 100, "ALIGN"), ("cache.k_stride_head", 0, "ALIGN"), ("cache.v_stride_page", -128, "ALIGN"),
 ]
-BAD_ATTN = [("q", None, "ARG"), ("o", None, "ARG"), ("causal", 2, "ARG"), ("heads", 0, "SHAPE"), ("q", BASE + 8, "ALIGN"), ("o_stride_h", 0, "ALIGN"),
-            ("q_stride_l", -128, "ALIGN"), ("o_stride_l", 4, "ALIGN")]
+BAD_ATTN = [("q", None, "ARG"), ("o", None, "ARG"), ("causal", 2, "ARG"), ("max_new", -1, "ARG"), ("heads", 0, "SHAPE"), ("q", BASE + 8, "ALIGN"), ("o_stride_h", 0, "ALIGN"),
+            ("q_stride_l", -128, "ALIGN"), ("q_stride_h", 0, "ALIGN"), ("o_stride_l", 4, "ALIGN")]
 
 
 @pytest.mark.parametrize("path,value,code", BAD + BAD_ATTN)
