@@ -59,7 +59,8 @@ struct TileBars {
   uint64_t empty[5];       // ring slot: both issuers' MMAs are done with it
   uint64_t staged[4];      // e4m3: copies have landed
   uint64_t unstaged[4];    // e4m3: widened
-  uint64_t q_full, q_empty;
+  uint64_t q_full[2];      // [stream]: one phase per piece in which the stream has work, so that nobody has to watch a phase of the other's
+  uint64_t q_empty;
   uint64_t q_ready[2];     // e4m3: the stream's Q is in fp16
   uint64_t s_full[2][2], p_full[2][2];  // [stream][half]
   uint64_t o_full[2];      // every P V of the stream's piece has completed
@@ -278,10 +279,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       mbar_init(smem_u32(&bars->staged[i]), 1);
       mbar_init(smem_u32(&bars->unstaged[i]), 4);
     }
-    mbar_init(smem_u32(&bars->q_full), 1);
     mbar_init(smem_u32(&bars->q_empty), 2);
     mbar_init(smem_u32(&bars->tmem_ready), 1);
     for (int t = 0; t < 2; ++t) {
+      mbar_init(smem_u32(&bars->q_full[t]), 1);
       mbar_init(smem_u32(&bars->q_ready[t]), 8);
       for (int hf = 0; hf < 2; ++hf) {
         mbar_init(smem_u32(&bars->s_full[t][hf]), 1);
@@ -424,7 +425,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       int cnt = 0;
       uint32_t n_done = 0;  // tiles so far, all pieces
       int vref = 0;         // e4m3: V's unit in the piece
-      uint32_t g = 0;       // pieces with work so far: the phase of q_full / q_empty
+      uint32_t g = 0;       // pieces with work so far: the phase of q_empty
       bool ok = true;
       const TilePiece* q;
       for (; ok && (q = piece()) != nullptr; piece_done()) {
@@ -472,12 +473,13 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
             if (q_free) {
               if (lane == 0) {
-                const uint32_t bar = smem_u32(&bars->q_full);
-                const bool second = q->tok0 + T < q->n;
-                mbar_arrive_expect_tx(bar, second ? 2 * q_bytes : q_bytes);
-                for (int t = 0; t < (second ? 2 : 1); ++t)
+                for (int t = 0; t < 2; ++t) {
+                  if (q->end[t] == 0) continue;
+                  const uint32_t bar = smem_u32(&bars->q_full[t]);
+                  mbar_arrive_expect_tx(bar, q_bytes);
                   for (int hf = 0; hf < 2; ++hf)
                     tma_load_3d(q_smem + t * kTileBytes + hf * kTileHalf, &tm_q, bar, 64 * hf, h * a.group, q->row0 + t * T);
+                }
               }
               __syncwarp();
               q_loaded = true;
@@ -572,8 +574,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const uint32_t s_tmem = tmem + t * 128, o_tmem = tmem + 256 + t * 128;
       uint32_t p_cnt[2] = {0, 0};  // P halves consumed so far: the phase of p_full
       uint32_t pv_cnt = 0;         // P V groups of the current piece: the first one overwrites O
-      uint32_t g = 0;              // pieces with work so far
-      uint32_t own = 0;            // pieces in which this stream had work: the phase of o_free
+      uint32_t own = 0;            // pieces in which this stream had work: the phase of q_full, q_ready and o_free
       int c0 = 0;                  // ring tiles before the current piece
       auto issue_s = [&](int hf, int s) {
         const uint64_t kd = k_desc0 + static_cast<uint64_t>((s * kTileBytes + hf * 8192) >> 4);
@@ -600,8 +601,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       for (; ok && (q = piece()) != nullptr; piece_done()) {
         const int n_tiles = uniform(q->n_tiles), n_mine = uniform(q->end[t]);
         if (n_tiles == 0) continue;
-        if (!kFp8) ok = wait(bars->q_full, g & 1, kTileWaitQFull);
-        else if (n_mine > 0) ok = wait(bars->q_ready[t], own & 1, kTileWaitQReady);
+        if (n_mine > 0) ok = wait(kFp8 ? bars->q_ready[t] : bars->q_full[t], own & 1, kFp8 ? kTileWaitQReady : kTileWaitQFull);
         ok = ok && ready(c0);
         if (!ok) break;
         pv_cnt = 0;
@@ -641,7 +641,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         if (!ok) break;
         c0 += 2 * n_tiles;
-        ++g;
         if (n_mine > 0) {
           umma_commit_if(leader, smem_u32(&bars->o_full[t]));
           ++own;
@@ -713,8 +712,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     constexpr float kLift = kFp8 ? 2.f : 0.f;            // the reference's own term is 2^kLift
     constexpr float kMostTerms = kFp8 ? 6.0e4f : 1.0e18f;  // 64 terms of a row: more than that has outgrown the reference
     uint32_t j = 0;         // key tiles the stream has processed: the phase of s_full
-    uint32_t own = 0;       // pieces in which the stream had work: the phase of o_full
-    uint32_t g = 0;         // e4m3: pieces with work, the phase of q_full
+    uint32_t own = 0;       // pieces in which the stream had work: the phase of q_full and o_full
     uint32_t n_before = 0;  // tiles of the pieces before
     uint32_t turn = 0;      // meetings of the stream's two halves so far
     // Leaves x for the same row's thread of the other half and returns what that one left.  Each side's values are in a
@@ -741,44 +739,42 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       if (mode == kUseMaxima && n_mine > 0)  // what the pass before this one left
         m_ref = fmaxf(bars->left[(turn & 1) ^ 1][t][0][row], bars->left[(turn & 1) ^ 1][t][1][row]) - kLift;
       if constexpr (kFp8) {
-        if (q->n_tiles > 0) {
-          ok = wait(bars->q_full, g & 1, kTileWaitQFull);  // every piece's: a phase must not be skipped
+        if (n_mine > 0) {
+          ok = wait(bars->q_full[t], own & 1, kTileWaitQFull);
           if (!ok) break;
-          if (n_mine > 0) {
-            // The thread's row of Q into fp16, in place: the row's largest becomes 2^4 .. 2^5.  Both halves look at the whole
-            // row, meet (everything has been read), and convert half of it each.
-            const uint32_t src = q_smem + t * kTileBytes + row * 128, swz = row & 7;
-            uint32_t m = 0;
-#pragma unroll 4
-            for (int x = 0; x < 16; ++x) {
-              uint4 w;
-              ld_shared_v4(src + (x >> 3) * kTileHalf + (((x & 7) ^ swz) << 4), w);
-              m = __vmaxu2(m, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
-            }
-            const int e = max(static_cast<int>(max(m >> 16, m & 0xFFFFu) >> 7) - 127 - 4, -120);
-            const float f = pow2_float(-e);
-            row_unit *= pow2_float(e);
-            exchange(0.f);
-            if (!ok) break;
-#pragma unroll 4
-            for (int x = 0; x < 8; ++x) {
-              const uint32_t at = src + hf * kTileHalf + ((x ^ swz) << 4);
-              uint4 w;
-              ld_shared_v4(at, w);
-              const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-              uint32_t o[4];
-#pragma unroll
-              for (int z = 0; z < 4; ++z) o[z] = pack_f16x2(__uint_as_float(in[z] << 16) * f, __uint_as_float(in[z] & 0xFFFF0000u) * f);
-              st_shared_v4(at, o[0], o[1], o[2], o[3]);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars->q_ready[t]));
+          // The thread's row of Q into fp16, in place: the row's largest becomes 2^4 .. 2^5.  Both halves look at the whole
+          // row, meet (everything has been read), and convert half of it each.
+          const uint32_t src = q_smem + t * kTileBytes + row * 128, swz = row & 7;
+          uint32_t m = 0;
+  #pragma unroll 4
+          for (int x = 0; x < 16; ++x) {
+            uint4 w;
+            ld_shared_v4(src + (x >> 3) * kTileHalf + (((x & 7) ^ swz) << 4), w);
+            m = __vmaxu2(m, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
           }
-          ++g;
+          const int e = max(static_cast<int>(max(m >> 16, m & 0xFFFFu) >> 7) - 127 - 4, -120);
+          const float f = pow2_float(-e);
+          row_unit *= pow2_float(e);
+          exchange(0.f);
+          if (!ok) break;
+  #pragma unroll 4
+          for (int x = 0; x < 8; ++x) {
+            const uint32_t at = src + hf * kTileHalf + ((x ^ swz) << 4);
+            uint4 w;
+            ld_shared_v4(at, w);
+            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+            uint32_t o[4];
+  #pragma unroll
+            for (int z = 0; z < 4; ++z) o[z] = pack_f16x2(__uint_as_float(in[z] << 16) * f, __uint_as_float(in[z] & 0xFFFF0000u) * f);
+            st_shared_v4(at, o[0], o[1], o[2], o[3]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bars->q_ready[t]));
         }
       }
       float l_sum = 0.f;
+      int vref = 0;  // e4m3: O is in units of 2^(vref - 127)
       bool over = false;
       for (int it = 0; it < n_mine; ++it) {
         ok = wait(bars->s_full[t][hf], j & 1, kTileWaitS);
@@ -790,6 +786,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           const TileInfo& in = info[(n_before + it) % kInfoRing];
           c = fminf(row_unit * __uint_as_float(static_cast<uint32_t>(in.kref) << 23), 3.0e38f);
           wide = in.wide != 0;
+          vref = in.vref;
         }
         const bool partly = (it + 1) * kKeyTile - 64 > lim_first;
         const int valid = lim - it * kKeyTile;
@@ -909,9 +906,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (to != nullptr) *reinterpret_cast<uint4*>(to + offset + 16 * (lane & 7)) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
         }
       };
-      float unit = 1.0f;
-      if constexpr (kFp8)
-        if (n_mine > 0) unit = __uint_as_float(static_cast<uint32_t>(info[(n_before - 1) % kInfoRing].vref) << 23);
+      const float unit = kFp8 ? __uint_as_float(static_cast<uint32_t>(vref) << 23) : 1.0f;
       if (q->whole) {
         const float inv = (l_sum == 0.f ? 0.f : 1.0f / l_sum) * unit;
 #pragma unroll

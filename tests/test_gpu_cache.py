@@ -122,11 +122,11 @@ class Case:
             return values(*quantise(k)), values(*quantise(v))
         return k.double(), v.double()
 
-    def reference(self, causal, scale=D ** -0.5, q=None):
+    def reference(self, causal, scale=D ** -0.5, q=None, max_new=None):
         """(out, lse, tolerance of out, tolerance of lse) in 64 bits, on the GPU."""
         dev, group = "cuda", self.heads // self.kv_heads
         q = (self.q if q is None else q).to(dev).double()
-        few = -(-self.rows // len(self.n)) * group <= 16  # which kernel runs: the average sequence's rows per K/V head
+        few = (max_new or -(-self.rows // len(self.n))) * group <= 16  # which kernel runs
         absolute = (2.0 ** -23 if few else 2.0 ** -27) if self.quantised else 0.0
         out = torch.zeros(self.rows, self.heads, D, dtype=torch.float64, device=dev)
         tol = torch.zeros_like(out)
@@ -168,7 +168,7 @@ class Case:
         status = torch.zeros(1, dtype=torch.int32, device="cuda")
         out, lse = self.h.cache_attn(self.q.cuda(), self.cache, self.batch, causal=causal, return_lse=True, status_word=status, **kw)
         assert self.h.read_status(status) == 0
-        self.compare(out, lse, *self.reference(causal, kw.get("softmax_scale", 0) or D ** -0.5))
+        self.compare(out, lse, *self.reference(causal, kw.get("softmax_scale", 0) or D ** -0.5, max_new=kw.get("max_new")))
         return out, lse
 
     @staticmethod
@@ -260,6 +260,22 @@ def test_positions_before_the_cache(h):
     out, lse = c.check(True)
     assert (out[:2] == 0).all() and (lse[:, :2] == -math.inf).all()
     c.check(False)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("n,length", [(200, 150), (400, 20), (129, 0)])
+def test_more_rows_than_keys(h, n, length, quantised):
+    c = Case(h, [n, 30], [length, 40], 2, 2, 16, quantised, seed=n).fill()
+    out, lse = c.check(True)
+    assert (out[: n - length] == 0).all() and (lse[:, : n - length] == -math.inf).all()
+    c.check(False)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("max_new", [None, 1, 400])
+def test_tokens_and_a_chunk_in_one_batch(h, max_new, quantised):
+    """Either kernel computes any batch; the longest sequence's rows only choose which."""
+    Case(h, [1] * 20 + [400] + [1] * 40, [100 + 30 * b for b in range(61)], 8, 4, 32, quantised, seed=5).fill().check(True, max_new=max_new)
 
 
 # ---------------------------------------------------------------------------------------------- attention
@@ -564,5 +580,11 @@ def test_refusals(h):
         h.CacheBatch(c.batch.pages.long(), c.batch.lengths, c.batch.starts)
     with pytest.raises(ValueError):
         h.CacheBatch(c.batch.pages, c.batch.lengths, c.batch.starts[:1])
+    with pytest.raises(_lib.H3AError) as e:  # one row for all
+        h.cache_attn(q[:1].expand(2, 4, D), c.cache, c.batch)
+    assert e.value.status == _lib.H3A_ERR_ALIGN
+    with pytest.raises(_lib.H3AError) as e:
+        h.cache_attn(q, c.cache, c.batch, max_new=-1)
+    assert e.value.status == _lib.H3A_ERR_ARG
     assert h.cache_attn(q[:0], c.cache, c.batch).shape == (0, 4, D)
     assert h.cache_read(c.cache, c.batch, 0)[0].shape == (0, 2, D)
