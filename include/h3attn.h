@@ -429,7 +429,7 @@ typedef struct h3a_cache_attn_params {
   h3a_cache cache;
   h3a_cache_batch batch;  /* batch.rows = rows of q and o */
   const void* q;          /* [rows, heads, 128] bf16 */
-  void* o;                /* [rows, heads, 128] bf16 */
+  void* o;                /* [rows, heads, 128] bf16; must not overlap q */
   float* lse;             /* optional [heads, rows] fp32, natural logarithm */
   int64_t q_stride_l, q_stride_h, o_stride_l, o_stride_h;
   int32_t heads;          /* query heads, a multiple of cache.heads */

@@ -215,7 +215,7 @@ def cache_attn(q: torch.Tensor, cache: KVCache, batch: CacheBatch, causal: bool 
     multiple of the cache's (query head h reads K/V head ``h // (heads // cache.heads)``).  ``causal``: row i of a sequence
     is the token at position ``lengths[b] - n_b + i`` and sees the keys up to itself (write its K and V first); otherwise
     every row sees all ``lengths[b]`` keys.  A row without a key is zeros (lse -inf).  Returns ``out [rows, heads, 128]``
-    bf16 (and ``lse [heads, rows]``); rows outside every sequence are not written.  ``softmax_scale`` 0: ``1/sqrt(128)``.
+    bf16 (and ``lse [heads, rows]``); rows outside every sequence are not written; ``out`` must not overlap ``q``.  ``softmax_scale`` 0: ``1/sqrt(128)``.
     ``max_new``, the most rows any one sequence has, only chooses the kernel, which otherwise goes by the average: worth
     saying for a batch that mixes single tokens with long chunks."""
     _require_cuda(q)

@@ -268,7 +268,7 @@ int32_t h3a_cache_attn_workspace_bytes(const h3a_cache_attn_params* p, size_t* b
 }
 
 int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
-  if (!p || !p->q || !p->o) return H3A_ERR_ARG;
+  if (!p || !p->q || !p->o || p->o == p->q) return H3A_ERR_ARG;  // a piece that is done twice reads its q again
   h3a::CacheAttnArgs a;
   std::memset(&a, 0, sizeof(a));
   int32_t rc = cache_args(&p->cache, &p->batch, p->status_word, &a.c);

@@ -21,7 +21,7 @@ def good():
     c.n_pages, c.page_size, c.heads, c.d = 4, 16, 1, 128
     b.pages = b.lengths = b.starts = BASE
     b.pages_stride, b.n_seqs, b.max_pages, b.rows = 4, 1, 4, 1
-    p.q = p.o = BASE
+    p.q, p.o = BASE, BASE + 4096
     p.q_stride_l = p.q_stride_h = p.o_stride_l = p.o_stride_h = 128
     p.heads, p.causal = 1, 1
     p.workspace, p.workspace_bytes = BASE, 1
@@ -45,7 +45,7 @@ BAD = [
     ("batch.rows", 0, "SHAPE"), ("batch.rows", 1 << 30, "SHAPE"),
     ("cache.k", BASE + 2, "ALIGN"), ("cache.v_stride_token", 100, "ALIGN"), ("cache.k_stride_head", 0, "ALIGN"), ("cache.v_stride_page", -128, "ALIGN"),
 ]
-BAD_ATTN = [("q", None, "ARG"), ("o", None, "ARG"), ("causal", 2, "ARG"), ("max_new", -1, "ARG"), ("heads", 0, "SHAPE"), ("q", BASE + 8, "ALIGN"), ("o_stride_h", 0, "ALIGN"),
+BAD_ATTN = [("q", None, "ARG"), ("o", None, "ARG"), ("o", BASE, "ARG"), ("causal", 2, "ARG"), ("max_new", -1, "ARG"), ("heads", 0, "SHAPE"), ("q", BASE + 8, "ALIGN"), ("o_stride_h", 0, "ALIGN"),
             ("q_stride_l", -128, "ALIGN"), ("q_stride_h", 0, "ALIGN"), ("o_stride_l", 4, "ALIGN")]
 
 

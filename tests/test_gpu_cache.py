@@ -586,5 +586,8 @@ def test_refusals(h):
     with pytest.raises(_lib.H3AError) as e:
         h.cache_attn(q, c.cache, c.batch, max_new=-1)
     assert e.value.status == _lib.H3A_ERR_ARG
+    with pytest.raises(_lib.H3AError) as e:
+        h.cache_attn(q, c.cache, c.batch, out=q)
+    assert e.value.status == _lib.H3A_ERR_ARG
     assert h.cache_attn(q[:0], c.cache, c.batch).shape == (0, 4, D)
     assert h.cache_read(c.cache, c.batch, 0)[0].shape == (0, 2, D)
