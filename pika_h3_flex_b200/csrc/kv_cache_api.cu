@@ -229,8 +229,9 @@ int32_t launch_tile(const h3a_cache_attn_params* p, const h3a::CacheAttnArgs& a,
 
 int32_t launch_join(const h3a::CacheAttnArgs& a, int shares, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  // a warp per row where rows are few; larger items loop, or blocks with nothing to do would take longer to launch than to run
-  cfg.gridDim = dim3(shares, std::min(8, a.item_rows / h3a::kJoinRows));
+  // a warp per row where rows are few, and per two rows of larger items: 8 blocks per item instead of 32 left 20 items of
+  // 252 rows in 18 parts to too few warps (chunks of 3 to 301 tokens: 53 against 39 us in all), 64 are not faster
+  cfg.gridDim = dim3(shares, std::min(32, a.item_rows / h3a::kJoinRows));
   cfg.blockDim = dim3(h3a::kJoinRows * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr;
