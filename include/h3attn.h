@@ -438,7 +438,7 @@ typedef struct h3a_cache_attn_params {
   int32_t max_new;        /* optional: the most rows any one sequence has (0: unknown).  It only chooses the kernel - up to 16
                              query rows per K/V head, or more - which otherwise goes by the average; say it for batches that
                              mix single tokens with long chunks. */
-  void* workspace;        /* h3a_cache_attn_workspace_bytes() bytes, 16-byte aligned; used by this call alone until it is done */
+  void* workspace;        /* h3a_cache_attn_workspace_bytes() bytes, 32-byte aligned; used by this call alone until it is done */
   size_t workspace_bytes;
   int32_t* status_word;   /* as in h3a_attn_params */
   int64_t wait_limit_ns;  /* as in h3a_attn_params */

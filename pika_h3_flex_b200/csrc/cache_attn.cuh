@@ -25,6 +25,7 @@ struct CacheAttnArgs {
   long long q_row_bytes, q_head_bytes;
   __nv_bfloat16* o;
   long long o_stride_l, o_stride_h;
+  int o_sectors;                     // rows of o begin at multiples of 32 bytes
   float* lse;                        // [heads, rows] or null
   int heads, group;                  // group = heads / kv_heads
   FastDiv by_group, by_item_tokens, by_item_rows;

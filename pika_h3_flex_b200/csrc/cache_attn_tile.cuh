@@ -128,26 +128,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-// 8 x 8 transpose of 16-byte pieces among 8 neighbouring lanes: in, lane s has pieces 0 .. 7 of row s; out, lane s has piece
-// s of rows 0 .. 7.  A thread owns a row of O, and written as it is a warp's store would be 32 pieces of 16 bytes, 256 bytes
-// apart: 5 us per 256 rows, as long as two and a half key tiles.  Transposed, an instruction writes 4 runs of 128 bytes.
-__device__ __forceinline__ void transpose_pieces(uint32_t* r) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int b = 1; b < 8; b <<= 1) {
-    const bool up = (lane & b) != 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if ((k & b) == 0) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t &lo = r[4 * k + w], &hi = r[4 * (k | b) + w];
-          const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, up ? lo : hi, b);
-          if (up) lo = got;
-          else hi = got;
-        }
-      }
-  }
+// 32 bytes of one row: a thread owns a row of O, and a warp's store is 32 pieces 256 bytes apart, so that pieces as long as
+// a sector count (16 bytes at a time, 256 rows took 5 us, as long as two and a half key tiles).
+__device__ __forceinline__ void stg_v8(void* to, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // A piece as the roles see it.
@@ -893,32 +879,34 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       l_sum += other;
       const int head = q->h * a.group + row - row_i * a.group;
       const long long out_row = q->row0 + row_token;
-      // where this thread's half row goes (null: nowhere), as bytes; 8 lanes write a row together
+      // where this thread's half row goes (null: nowhere)
       uint8_t* dst = nullptr;
       if (have_row)
         dst = q->whole ? reinterpret_cast<uint8_t*>(a.o + out_row * a.o_stride_l + head * a.o_stride_h + 64 * hf)
                        : reinterpret_cast<uint8_t*>(part_slot(a, blockIdx.x, q->tail != 0) + (t * T * a.group + row) * kCacheDim + 64 * hf);
-      auto store_pieces = [&](uint32_t* r, int offset) {
-        transpose_pieces(r);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(dst), (lane & 24) + k));
-          if (to != nullptr) *reinterpret_cast<uint4*>(to + offset + 16 * (lane & 7)) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
-        }
-      };
       const float unit = kFp8 ? __uint_as_float(static_cast<uint32_t>(vref) << 23) : 1.0f;
       if (q->whole) {
         const float inv = (l_sum == 0.f ? 0.f : 1.0f / l_sum) * unit;
 #pragma unroll
         for (int i = 0; i < 32; ++i) s[i] = pack_bf16x2(__uint_as_float(s[2 * i]) * inv, __uint_as_float(s[2 * i + 1]) * inv);
-        store_pieces(s, 0);
+        if (have_row) {
+          if (a.o_sectors) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) stg_v8(dst + 32 * i, s + 8 * i);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(dst + 16 * i) = make_uint4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+          }
+        }
         if (have_row && a.lse && hf == 0)
           a.lse[static_cast<long long>(head) * a.c.rows + out_row] = l_sum == 0.f ? -INFINITY : (m_ref + log2f(l_sum)) * 0.6931471805599453f;
       } else {
 #pragma unroll
         for (int i = 0; i < 64; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * unit);
-        store_pieces(s, 0);
-        store_pieces(s + 32, 128);
+        if (have_row) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) stg_v8(dst + 32 * i, s + 8 * i);
+        }
         if (have_row && hf == 0) {
           float* stat = part_slot(a, blockIdx.x, q->tail != 0) + kTileRows * kCacheDim + t * T * a.group + row;
           stat[0] = m_ref;
@@ -926,7 +914,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       }
       if (bars->poison != 0u) {  // rare: values that the helpers left out are added to the stored row, for the rows that see them
-        __syncwarp();            // the row was stored by its neighbours
         if (have_row) {
           const int begin = max(q->lim_min & ~(kKeyTile - 1), q->t0 * kKeyTile);
           const int end = min(lim + hf * 64, q->n_tiles * kKeyTile) + q->t0 * kKeyTile;

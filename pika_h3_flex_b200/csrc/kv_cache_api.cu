@@ -283,13 +283,14 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   if ((rc = current_device(&dev)) != H3A_OK) return rc;
   const AttnPlan n = attn_plan(p, dev.sms);
   if (!p->workspace || p->workspace_bytes < n.bytes) return H3A_ERR_WORKSPACE;
-  if (!aligned16(p->workspace)) return H3A_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(p->workspace) % 32) return H3A_ERR_ALIGN;
   a.q = static_cast<const uint8_t*>(p->q);
   a.q_row_bytes = p->q_stride_l * 2;
   a.q_head_bytes = p->q_stride_h * 2;
   a.o = static_cast<__nv_bfloat16*>(p->o);
   a.o_stride_l = p->o_stride_l;
   a.o_stride_h = p->o_stride_h;
+  a.o_sectors = (reinterpret_cast<uintptr_t>(p->o) | static_cast<uintptr_t>(2 * p->o_stride_l) | static_cast<uintptr_t>(2 * p->o_stride_h)) % 32 == 0;
   a.lse = p->lse;
   a.heads = p->heads;
   a.group = p->heads / p->cache.heads;
