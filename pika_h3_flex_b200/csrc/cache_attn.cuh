@@ -4,7 +4,7 @@
 //   o_i = sum_j softmax_j(scale q_i . k_j) v_j,  j < lengths[b], and with the causal mask j <= position of row i.
 //
 // Work.  An ITEM is a run of query rows of one sequence that share a K/V head (row r = token i * group + head in the
-// group); it costs one unit per tile of keys plus one for its own set-up.  All items' units are laid end to end and cut
+// group); it costs one unit per tile of keys plus `set_up`.  All items' units are laid end to end and cut
 // into equal SHARES, one per CTA, whatever the lengths: a long sequence is spread over many SMs and many short ones share
 // an SM.  An item that crosses a cut leaves fp32 partial results (O, running maximum, sum) in the workspace; a second small
 // launch joins them in order of the keys, so results do not depend on timing.  A CTA has at most two such pieces (its
@@ -36,8 +36,9 @@ struct CacheAttnArgs {
   float scale_log2;
   float* part;                       // [share][2][item_rows] x (128 + 2) fp32
   int* desc;                         // [share][kDescInts]: the item that a share begins and does not finish
+  int set_up;                        // units that an item costs beside one per tile
   int share_shift;                   // a share has at least 2^this units
-  long long wait_ns;
+  uint32_t wait_units;               // longest wait, in 1,024 ns
 };
 
 struct AttnSeq {
@@ -64,9 +65,9 @@ __device__ __forceinline__ int item_tiles(const CacheAttnArgs& a, const AttnSeq&
 }
 // units of all the sequence's items of one K/V head
 __device__ __forceinline__ long long head_units(const CacheAttnArgs& a, const AttnSeq& s) {
-  if (!a.causal) return static_cast<long long>(s.n_items) * (1 + ((s.len + (1 << a.key_shift) - 1) >> a.key_shift));
+  if (!a.causal) return static_cast<long long>(s.n_items) * (a.set_up + ((s.len + (1 << a.key_shift) - 1) >> a.key_shift));
   long long w = 0;
-  for (int it = 0; it < s.n_items; ++it) w += 1 + item_tiles(a, s, it);
+  for (int it = 0; it < s.n_items; ++it) w += a.set_up + item_tiles(a, s, it);
   return w;
 }
 
@@ -77,7 +78,7 @@ struct ShareStart {     // in shared memory
   int b;
 };
 
-// A piece of an item: key tiles [t0, t1); `first` / `last`: it holds the item's first / last unit.
+// A piece of an item: key tiles [t0, t1); `first` / `last`: it holds the item's first / last tile.
 struct Piece {
   int b, h, it, t0, t1;
   bool first, last;
@@ -110,18 +111,19 @@ struct ShareIter {
       return true;
     }
     if (pos >= end) return false;
-    const int units = 1 + item_tiles(a, s, it);
+    const int units = a.set_up + item_tiles(a, s, it);
     const int u0 = static_cast<int>(pos - item_base);
     const int u1 = static_cast<int>(min(static_cast<long long>(units), end - item_base));
     p.b = b;
     p.h = h;
     p.it = it;
     p.s = s;
-    p.t0 = max(u0, 1) - 1;
-    p.t1 = u1 - 1;
-    p.first = u0 == 0;
-    p.last = u1 == units;
     pos = item_base + u1;
+    p.t0 = max(u0 - a.set_up, 0);
+    p.t1 = u1 - a.set_up;
+    p.first = p.t0 == 0;
+    p.last = u1 == units;
+    if (p.t1 <= 0 && !p.last) return false;  // the share ends before the item's first tile: the next one begins it
     if (p.last) {
       item_base += units;
       if (++it == s.n_items) {
@@ -159,13 +161,13 @@ __device__ __forceinline__ void share_item(const CacheAttnArgs& a, ShareIter& s,
   s.item_base += s.h * head_total;
   s.it = 0;
   if (!a.causal) {  // items of equal length
-    const int units = 1 + item_tiles(a, s.s, 0);
+    const int units = a.set_up + item_tiles(a, s.s, 0);
     s.it = static_cast<int>(div_units(s.pos - s.item_base, units));
     s.item_base += static_cast<long long>(s.it) * units;
     return;
   }
   for (;;) {
-    const int units = 1 + item_tiles(a, s.s, s.it);
+    const int units = a.set_up + item_tiles(a, s.s, s.it);
     if (s.pos < s.item_base + units) break;
     s.item_base += units;
     ++s.it;
@@ -183,7 +185,7 @@ __device__ __forceinline__ ShareIter share_begin(const CacheAttnArgs& a, ShareSt
   if (a.c.n_seqs == 1 && !a.causal && a.item_tokens > 0) {
     s.b = 0;
     s.s = attn_seq(a, 0);
-    const int n_items = s.s.n_items * a.c.kv_heads, units = 1 + item_tiles(a, s.s, 0);
+    const int n_items = s.s.n_items * a.c.kv_heads, units = a.set_up + item_tiles(a, s.s, 0);
     s.whole = n_items / gridDim.x;
     s.whole_item = blockIdx.x;
     const int dealt = s.whole * gridDim.x;

@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
       }
     }
     if (threadIdx.x == 0 && p.first && !p.last)
-      describe_join(a, sm.iter, sm.iter.item_base + 1 + item_tiles(a, p.s, p.it), n_rows, r0, p.s.s0, p.h);
+      describe_join(a, sm.iter, sm.iter.item_base + a.set_up + item_tiles(a, p.s, p.it), n_rows, r0, p.s.s0, p.h);
     __syncthreads();  // everybody is done with this piece's shared memory
     if (threadIdx.x == 0) {
       sm.poison = 0;

@@ -7,10 +7,11 @@
 //   warps 17, 18     issuers, one per stream: S = Q K^T (N = 64 keys), O += P V (P from TMEM), tcgen05.commit
 //   warp 19          cuts the share into pieces and hands them to the others through a small ring: the bookkeeping would
 //                    cost every role some 40 registers
-//   warps 20-23      helpers, one cache row per thread.  e4m3: widen a staged tile into the ring (below).  bf16: let tiles
-//                    through, except the V tiles that not every row sees whole: P is 0 for a key a row does not see, and
-//                    0 x NaN is NaN, so rows behind the last key become zeros and values that are not finite become zeros
-//                    until the epilogue puts them back for the rows that do see them.
+//   warps 20-23      helpers, one cache row per thread.  e4m3: widen a staged tile into the ring (below).  bf16: look
+//                    at V tiles that not every row sees whole: P is 0 for a key a row does not see, and 0 x NaN is NaN, so
+//                    rows behind the last key become zeros and values that are not finite become zeros until they are put
+//                    back for the rows that do see them; other tiles go to the MMAs as they are.  And they take the results out of tensor
+//                    memory, while the softmax warps are at the next piece.
 // TMEM: stream t: S/P buffer of half h at columns [128 t + 64 h, +64), O at [256 + 128 t, +128).  Four chains of S -> P -> O
 // run per CTA; the two warpgroups of a stream share the accumulator and so have to agree on each row's reference.
 //
@@ -39,8 +40,6 @@ namespace h3a {
 
 constexpr int kTileThreads = 768;
 constexpr int kKeyTile = 128, kTileKeyShift = 7;
-constexpr int kTileSoftmaxRegs = 88, kTileOtherRegs = 64, kTileLaunchRegs = 80;
-static_assert(512 * kTileSoftmaxRegs + 256 * kTileOtherRegs <= kTileLaunchRegs * kTileThreads, "setmaxnreg budget exceeds the launch allocation");
 constexpr int kProducerWarp = 16, kIssuerWarp = 17, kPieceWarp = 19, kHelperWarp = 20;
 constexpr int kTileRows = 256;         // rows of an item
 constexpr int kTileBytes = 32768;      // 128 rows of 128 bf16
@@ -54,13 +53,12 @@ struct TileRing {
 };
 
 struct TileBars {
-  uint64_t full[5];        // ring slot: copies have landed (bf16)
-  uint64_t ready[5];       // ring slot: may be read by MMAs
+  uint64_t full[5];        // ring slot: copies have landed that MMAs may read as they are (bf16)
+  uint64_t ready[5];       // ring slot: a helper has written or looked at it
   uint64_t empty[5];       // ring slot: both issuers' MMAs are done with it
-  uint64_t staged[4];      // e4m3: copies have landed
+  uint64_t staged[4];      // copies have landed that a helper is to look at: e4m3 staging slot; bf16 ring slot
   uint64_t unstaged[4];    // e4m3: widened
-  uint64_t q_full[2];      // [stream]: one phase per piece in which the stream has work, so that nobody has to watch a phase of the other's
-  uint64_t q_empty;
+  uint64_t q_full[2], q_empty[2];  // [stream]: a phase per piece in which the stream has work, so that nobody has to watch the other's
   uint64_t q_ready[2];     // e4m3: the stream's Q is in fp16
   uint64_t s_full[2][2], p_full[2][2];  // [stream][half]
   uint64_t o_full[2];      // every P V of the stream's piece has completed
@@ -72,7 +70,7 @@ struct TileBars {
   uint32_t tmem_base;
   uint32_t early_exit;
   uint32_t more;             // the share has a piece at all
-  volatile uint32_t abort_flag;
+  volatile uint32_t abort_flag;  // code of a wait that gave up: everybody else does too
   volatile uint32_t poison;  // some V value counted as zero: from then on every epilogue looks for such values
   uint32_t redo;             // pieces of the current batch that outgrew their reference, a bit each
   float left[2][2][2][128];  // [turn][stream][half][row]: what the halves of a stream leave for each other
@@ -81,37 +79,36 @@ struct TileBars {
 constexpr int kTileBarBytes = 7680;
 constexpr int kTileSmemBytes = 2 * kTileBytes + (TileRing<true>::kBytes > TileRing<false>::kBytes ? TileRing<true>::kBytes : TileRing<false>::kBytes) + 1024 + kTileBarBytes;
 static_assert(sizeof(TileBars) <= kTileBarBytes, "shared memory layout");
-enum : int {  // status codes of waits that ran out (low byte of the status word)
+enum : uint32_t {  // status codes of waits that ran out (low byte of the status word)
   kTileWaitEmpty = 33, kTileWaitFull, kTileWaitReady, kTileWaitUnstaged, kTileWaitStaged, kTileWaitQFull, kTileWaitQEmpty,
   kTileWaitQReady, kTileWaitS, kTileWaitP, kTileWaitO, kTileWaitOFree, kTileWaitMeet, kTileWaitPiece, kTileWaitTmem,
   kTileWaitFin, kTileWaitFinFree
 };
 
+// There are forty waits, and what a hot loop steps over costs instruction cache too: a wait that gives up only leaves its
+// code, which is reported at the end.
 struct TileWait {
   const CacheAttnArgs& a;
   TileBars* bars;
-  __device__ __forceinline__ bool one(uint64_t& barrier, uint32_t parity, int code) const {
+  __device__ __forceinline__ static uint32_t now() { return static_cast<uint32_t>(global_timer_ns() >> 10); }
+  __device__ __forceinline__ bool one(uint64_t& barrier, uint32_t parity, uint32_t code) const {
     const uint32_t bar = smem_u32(&barrier);
     if (mbar_try_wait(bar, parity)) return true;
-    uint32_t polls = 0;
-    uint64_t t0 = 0;
+    uint32_t polls = 0, t0 = 0;
+#pragma unroll 1
     while (!mbar_try_wait(bar, parity)) {
-      if ((++polls & 63u) == 0u) {
-        if (bars->abort_flag) return false;
-        const uint64_t now = global_timer_ns();
-        if (t0 == 0) {
-          t0 = now;
-        } else if (static_cast<long long>(now - t0) > a.wait_ns) {
-          bars->abort_flag = 1u;
-          if (a.c.status) atomicCAS(a.c.status, 0, code | (static_cast<int>(blockIdx.x) << 8));
-          return false;
-        }
+      if ((++polls & 63u) != 0u) continue;
+      if (bars->abort_flag) return false;
+      if (polls == 64u) t0 = now();
+      if (now() - t0 > a.wait_units) {
+        bars->abort_flag = code;
+        return false;
       }
     }
     return true;
   }
   // the whole warp, with one verdict
-  __device__ __forceinline__ bool operator()(uint64_t& barrier, uint32_t parity, int code) const {
+  __device__ __forceinline__ bool operator()(uint64_t& barrier, uint32_t parity, uint32_t code) const {
     return __all_sync(0xFFFFFFFFu, one(barrier, parity, code));
   }
 };
@@ -237,7 +234,7 @@ __device__ __forceinline__ void describe_piece(const CacheAttnArgs& a, const Sha
   q.tail = p.first;
   if (p.first && !p.last) {
     const int r0 = q.tok0 * a.group;
-    describe_join(a, iter, iter.item_base + 1 + item_tiles(a, p.s, p.it), min(p.s.n * a.group - r0, a.item_tokens * a.group), r0, p.s.s0, p.h);
+    describe_join(a, iter, iter.item_base + a.set_up + item_tiles(a, p.s, p.it), min(p.s.n * a.group - r0, a.item_tokens * a.group), r0, p.s.s0, p.h);
   }
 }
 
@@ -272,14 +269,14 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       mbar_init(smem_u32(&bars->ready[i]), 4);   // one arrive per helper warp
       mbar_init(smem_u32(&bars->empty[i]), 2);   // one commit per issuer
     }
-    for (int i = 0; i < R::kStaged; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&bars->staged[i]), 1);
       mbar_init(smem_u32(&bars->unstaged[i]), 4);
     }
-    mbar_init(smem_u32(&bars->q_empty), 2);
     mbar_init(smem_u32(&bars->tmem_ready), 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&bars->q_full[t]), 1);
+      mbar_init(smem_u32(&bars->q_empty[t]), 1);
       mbar_init(smem_u32(&bars->q_ready[t]), 8);
       for (int hf = 0; hf < 2; ++hf) {
         mbar_init(smem_u32(&bars->s_full[t][hf]), 1);
@@ -343,17 +340,19 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (warp >= kHelperWarp) {
     // =========================================================== helpers: thread r owns row r of every tile
-    setmaxnreg_dec<kTileOtherRegs>();
     const int row = threadIdx.x - kHelperWarp * 32;
     const uint32_t swz = row & 7;
     int cnt = 0;
     uint32_t n_done = 0;   // tiles so far, all pieces
     uint32_t n_out = 0;    // pieces whose results have left: the phase of fin
     uint32_t o_phase = 0;  // bit t: the phase of o_full[t]
+    uint32_t v_phase = 0;  // bf16: bit s: the phase of staged[s]
     bool ok = true;
     const TilePiece* held = nullptr;  // a piece whose results are still in tensor memory
+#pragma unroll 1
     for (;;) {
-      // The next piece's first tile goes ahead of this one's results, but nobody waits for a piece before results have left.
+      // The next piece's first K goes ahead of this one's results, its V between the two streams', but nobody waits for a
+      // piece before results have left.
       const TilePiece* q = nullptr;
       bool last = false;
       if (held == nullptr || __all_sync(0xFFFFFFFFu, mbar_test_wait(smem_u32(&bars->piece_full[n_pieces % kPieceRing]), (n_pieces / kPieceRing) & 1))) {
@@ -362,22 +361,18 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       const int n_tiles = q ? uniform(q->n_tiles) : 0, t0 = q ? uniform(q->t0) : 0;
       const int lim_min = q ? uniform(q->lim_min) : 0, lim_max = q ? uniform(q->lim_max) : 0;
-      int it = 0;
+      const int steps = max(2 * n_tiles, held ? 2 : 0);
 #pragma unroll 1
-      for (int round = 0; ok && round < 2; ++round) {
-#pragma unroll 1
-      for (const int stop = round == 0 && held ? min(1, n_tiles) : n_tiles; ok && it < stop; ++it, ++n_done) {
-        const int tile = t0 + it, key = tile * kKeyTile + row;
+      for (int step = 0; ok && step < steps; ++step) {
+        const int x = step & 1, tile = t0 + (step >> 1), key = tile * kKeyTile + row;  // K, then V
         const bool special = (tile + 1) * kKeyTile > lim_min;
         const bool gone = key >= lim_max;
-#pragma unroll 1
-        for (int x = 0; x < 2; ++x, ++cnt) {  // K, then V
+        if (step < 2 * n_tiles && (kFp8 || (x == 1 && special))) {
           const int s = cnt % R::kRing;
-          const uint32_t ph = (cnt / R::kRing) & 1;
           const uint32_t dst = ring + s * kTileBytes + row * 128;
           if constexpr (kFp8) {
             const int g = cnt % R::kStaged;
-            ok = wait(bars->staged[g], (cnt / R::kStaged) & 1, kTileWaitStaged) && wait(bars->empty[s], ph ^ 1u, kTileWaitEmpty);
+            ok = wait(bars->staged[g], (cnt / R::kStaged) & 1, kTileWaitStaged) && wait(bars->empty[s], ((cnt / R::kRing) & 1) ^ 1, kTileWaitEmpty);
             if (!ok) break;
             const uint32_t src = staging + g * kCodeBytes + row * 128;
             // what the producer has found out about the tile; a row that is not there may hold anything, codes for NaN
@@ -401,43 +396,44 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               mbar_arrive(smem_u32(&bars->unstaged[g]));
             }
           } else {
-            ok = wait(bars->full[s], ph, kTileWaitFull);
+            ok = wait(bars->staged[s], (v_phase >> s) & 1, kTileWaitStaged);
             if (!ok) break;
-            if (x == 1 && special) {
-              uint32_t m = 0;  // the row's largest magnitude by its bits
+            v_phase ^= 1u << s;
+            uint32_t m = 0;  // the row's largest magnitude by its bits
 #pragma unroll 4
+            for (int c = 0; c < 16; ++c) {
+              const uint32_t at = dst + (c >> 3) * kTileHalf + (((c & 7) ^ swz) << 4);
+              uint4 w = make_uint4(0, 0, 0, 0);
+              if (gone) st_shared_v4(at, 0, 0, 0, 0);
+              else ld_shared_v4(at, w);
+              m = __vmaxu2(m, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+            }
+            if (non_finite2(m)) {  // rare
+              bars->poison = 1u;
+#pragma unroll 1
               for (int c = 0; c < 16; ++c) {
                 const uint32_t at = dst + (c >> 3) * kTileHalf + (((c & 7) ^ swz) << 4);
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (gone) st_shared_v4(at, 0, 0, 0, 0);
-                else ld_shared_v4(at, w);
-                m = __vmaxu2(m, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+                uint4 w;
+                ld_shared_v4(at, w);
+                st_shared_v4(at, finite_or_zero2(w.x), finite_or_zero2(w.y), finite_or_zero2(w.z), finite_or_zero2(w.w));
               }
-              if (non_finite2(m)) {  // rare
-                bars->poison = 1u;
-#pragma unroll 1
-                for (int c = 0; c < 16; ++c) {
-                  const uint32_t at = dst + (c >> 3) * kTileHalf + (((c & 7) ^ swz) << 4);
-                  uint4 w;
-                  ld_shared_v4(at, w);
-                  st_shared_v4(at, finite_or_zero2(w.x), finite_or_zero2(w.y), finite_or_zero2(w.z), finite_or_zero2(w.w));
-                }
-              }
-              fence_proxy_async_smem();
             }
+            fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bars->ready[s]));
           }
         }
-      }
-      if (round == 1 || !held || !ok) continue;
-      // ---- results of the piece before: thread r has row r of both streams
-      const uint32_t tmem = tensor_memory(ok);
-      const bool whole = held->whole != 0, keep = held->mode != kFindMaxima;
-#pragma unroll 1
-      for (int t = 0; ok && t < 2; ++t) {
+        if (step < 2 * n_tiles) {
+          ++cnt;
+          n_done += x;
+        }
+        if (step > 1 || !held) continue;
+        // ---- results of the piece before, a stream: thread r has row r
+        const int t = step;
+        const uint32_t tmem = tensor_memory(ok);
+        const bool whole = held->whole != 0, keep = held->mode != kFindMaxima;
         const bool any = uniform(held->end[t]) > 0;
-        ok = wait(bars->fin[t], n_out & 1, kTileWaitFin) && (!any || wait(bars->o_full[t], (o_phase >> t) & 1, kTileWaitO));
+        ok = ok && wait(bars->fin[t], n_out & 1, kTileWaitFin) && (!any || wait(bars->o_full[t], (o_phase >> t) & 1, kTileWaitO));
         if (!ok) break;
         if (any) o_phase ^= 1u << t;
         tc_fence_after_sync();
@@ -462,16 +458,22 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             stat[kTileRows] = l_sum;
           }
         }
+        const uint32_t from = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 + t * 128;
+        uint32_t s[16] = {};
+        if (any) tmem_ld16(from, s);
 #pragma unroll 1
-        for (int c = 0; c < 8; ++c) {  // 16 dims at a time
-          uint32_t s[16] = {};
+        for (int c = 0; c < 8; ++c) {  // 16 dims at a time, the next 16 on their way while these are stored
+          float o[16];
           if (any) {
-            tmem_ld16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 + t * 128 + 16 * c, s);
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(s[i]));
           }
-          if (c == 7) {  // the next piece may have O and the sums
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(s[i]) * f;
+          if (c < 7) {
+            if (any) tmem_ld16(from + 16 * (c + 1), s);
+          } else {  // the next piece may have O and the sums
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
@@ -483,7 +485,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (whole) {
             uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(__uint_as_float(s[2 * i]) * f, __uint_as_float(s[2 * i + 1]) * f);
+            for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
             if (a.o_sectors) {
               stg_v8(dst + 32 * c, w);
             } else {
@@ -491,10 +493,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               *reinterpret_cast<uint4*>(dst + 32 * c + 16) = make_uint4(w[4], w[5], w[6], w[7]);
             }
           } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
-            stg_v8(dst + 64 * c, s);
-            stg_v8(dst + 64 * c + 32, s + 8);
+            stg_v8(dst + 64 * c, reinterpret_cast<const uint32_t*>(o));
+            stg_v8(dst + 64 * c + 32, reinterpret_cast<const uint32_t*>(o + 8));
           }
         }
         if (bars->poison != 0u && have_row) {  // rare: values left out above are added to the stored row, if it sees them
@@ -512,11 +512,12 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               }
             }
         }
-      }
-      ++n_out;
-      __syncwarp();
-      if (ok && lane == 0) mbar_arrive(smem_u32(&bars->piece_empty[(n_pieces - 1) % kPieceRing]));
-      held = nullptr;
+        if (t == 1) {
+          ++n_out;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bars->piece_empty[(n_pieces - 1) % kPieceRing]));
+          held = nullptr;
+        }
       }
       if (!ok || last) break;
       if (q) {
@@ -525,7 +526,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
     }
   } else if (warp >= kProducerWarp) {
-    setmaxnreg_dec<kTileOtherRegs>();
     if (warp == kProducerWarp) {
       // ========================================================= producer: lane x copies sub-box x of a tile
       const int n_boxes = kKeyTile / box_rows;
@@ -534,16 +534,15 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       int cnt = 0;
       uint32_t n_done = 0;  // tiles so far, all pieces
       int vref = 0;         // e4m3: V's unit in the piece
-      uint32_t g = 0;       // pieces with work so far: the phase of q_empty
+      uint32_t q_phase = 3;  // bit t: the phase of q_empty[t], whose first wait is for nothing
       bool ok = true;
       const TilePiece* q;
+#pragma unroll 1
       for (; ok && (q = piece()) != nullptr; piece_done()) {
         const int n_tiles = uniform(q->n_tiles), t0 = uniform(q->t0), b = uniform(q->b), h = uniform(q->h), lim_max = uniform(q->lim_max);
-        const int mode = uniform(q->mode);
+        const int mode = uniform(q->mode), lim_min = uniform(q->lim_min);
         if (n_tiles == 0) continue;
-        // Q is free late in the previous piece, ring slots earlier: the first two key tiles go ahead of Q
-        const int q_at = g > 0 ? min(2, n_tiles - 1) : 0;
-        bool q_loaded = false;
+        const int n_streams = uniform((q->end[0] > 0 ? 1 : 0) | (q->end[1] > 0 ? 2 : 0));
         // A lane looks after 4 rows of every tile, which are in one page.  Its page number is fetched two tiles ahead, the rows'
         // exponent bytes (e4m3) one tile ahead; nothing looks at either before it is needed, or the loads would be waited for.
         int id = 0, id_next = 0;
@@ -567,40 +566,18 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             raw_v[i] = key + i < lim_max ? __ldg(from_v + i * a.c.exp_token[1]) : 0u;
           }
         };
-        id = checked(fetch_id(t0));
-        id_next = fetch_id(t0 + 1);
-        if constexpr (kFp8) fetch_ex(t0, id);
+        id_next = fetch_id(t0);
         int v_most = 0;                       // largest exponent of V in the piece
         if (mode != kUseMaxima) vref = 0;     // otherwise what the pass before found
-        for (int it = 0; ok && it < n_tiles; ++it, ++n_done) {
-          if (!q_loaded) {
-            bool q_free = g == 0 || __all_sync(0xFFFFFFFFu, mbar_test_wait(smem_u32(&bars->q_empty), (g - 1) & 1));
-            if (!q_free && it >= q_at) {
-              ok = wait(bars->q_empty, (g - 1) & 1, kTileWaitQEmpty);
-              if (!ok) break;
-              q_free = true;
-            }
-            if (q_free) {
-              if (lane == 0) {
-                for (int t = 0; t < 2; ++t) {
-                  if (q->end[t] == 0) continue;
-                  const uint32_t bar = smem_u32(&bars->q_full[t]);
-                  mbar_arrive_expect_tx(bar, q_bytes);
-                  for (int hf = 0; hf < 2; ++hf)
-                    tma_load_3d(q_smem + t * kTileBytes + hf * kTileHalf, &tm_q, bar, 64 * hf, h * a.group, q->row0 + t * T);
-                }
-              }
-              __syncwarp();
-              q_loaded = true;
-            }
-          }
+#pragma unroll 1
+        for (int it = -1; ok && it < n_tiles; ++it) {
           const int tile = t0 + it;
           // sub-box x of the tile: lane x copies it; none behind the last key
           const int key = tile * kKeyTile + lane * box_rows, at = key - a.c.by_page(key) * a.c.page_size;
           const bool mine = lane < n_boxes && key < lim_max;
           const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, mine)) * box_bytes;
           const int page = __shfl_sync(0xFFFFFFFFu, id, (lane * box_rows / 4) & 31);
-          if constexpr (kFp8) {
+          if (kFp8 && it >= 0) {
             // the tile's largest exponents, and V's smallest; rows of nothing (7) and rows that are not finite (255) aside
             uint32_t k_top = 0, v_top = 0, v_low = 255;
 #pragma unroll
@@ -633,8 +610,25 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           id = checked(id_next);
           id_next = fetch_id(tile + 2);
           if constexpr (kFp8) fetch_ex(tile + 1, id);
+          if (it < 0) continue;  // only the fetches
 #pragma unroll 1
-          for (int x = 0; x < 2; ++x, ++cnt) {
+          for (int x = 0; ok && x < 2; ++x, ++cnt) {
+            // Q is free late in the previous piece, ring slots earlier: the first K tile goes ahead of Q
+            if (it == 0 && x == 1) {
+#pragma unroll 1
+              for (int t = 0; t < 2; ++t) {
+                if (((n_streams >> t) & 1) == 0) continue;
+                ok = wait(bars->q_empty[t], (q_phase >> t) & 1, kTileWaitQEmpty);
+                if (!ok) break;
+                q_phase ^= 1u << t;
+                const uint32_t bar = smem_u32(&bars->q_full[t]);
+                if (lane == 0) mbar_arrive_expect_tx(bar, q_bytes);
+                __syncwarp();
+                if (lane < 2) tma_load_3d(q_smem + t * kTileBytes + lane * kTileHalf, &tm_q, bar, 64 * lane, h * a.group, q->row0 + t * T);
+                __syncwarp();
+              }
+              if (!ok) break;
+            }
             const CUtensorMap* tm = x ? &tm_v : &tm_k;
             uint32_t dst, bar;
             if constexpr (kFp8) {
@@ -646,7 +640,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               const int s = cnt % R::kRing;
               ok = wait(bars->empty[s], ((cnt / R::kRing) & 1) ^ 1u, kTileWaitEmpty);
               dst = ring + s * kTileBytes + lane * box_rows * 128;
-              bar = smem_u32(&bars->full[s]);
+              bar = smem_u32(x == 1 && (tile + 1) * kKeyTile > lim_min ? &bars->staged[s] : &bars->full[s]);
             }
             if (!ok) break;
             __syncwarp();  // with what was left about the tile
@@ -658,9 +652,9 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             }
             __syncwarp();
           }
+          ++n_done;
         }
         if (mode == kFindMaxima) vref = v_most != 0 ? v_most : 127;
-        ++g;
       }
     } else if (warp < kPieceWarp) {
       // ========================================================= issuers, one warp per stream
@@ -702,17 +696,29 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           umma_bf16_ts_if(leader, o_tmem, s_tmem + hf * 64 + k * 8, vd + (k * 2048 >> 4), idesc, (pv_cnt > 0 || k > 0) ? 1u : 0u);
         ++pv_cnt;
       };
-      auto ready = [&](int c) {
-        const bool got = wait(bars->ready[c % R::kRing], (c / R::kRing) & 1, kTileWaitReady);
+      // bf16 tiles are read as the copies leave them, but for V tiles that a helper has to look at (which have barriers of
+      // their own: nobody has to watch a phase that is not his)
+      uint32_t full_phase = 0, ready_phase = 0;  // bit s: the phase of full[s], ready[s]
+      auto ready = [&](int c, bool looked_at) {
+        const int s = c % R::kRing;
+        bool got;
+        if (kFp8 || looked_at) {
+          got = wait(bars->ready[s], (ready_phase >> s) & 1, kTileWaitReady);
+          ready_phase ^= 1u << s;
+        } else {
+          got = wait(bars->full[s], (full_phase >> s) & 1, kTileWaitFull);
+          full_phase ^= 1u << s;
+        }
         tc_fence_after_sync();
         return got;
       };
       const TilePiece* q;
+#pragma unroll 1
       for (; ok && (q = piece()) != nullptr; piece_done()) {
-        const int n_tiles = uniform(q->n_tiles), n_mine = uniform(q->end[t]);
+        const int n_tiles = uniform(q->n_tiles), n_mine = uniform(q->end[t]), t0 = uniform(q->t0), lim_min = uniform(q->lim_min);
         if (n_tiles == 0) continue;
         if (n_mine > 0) ok = wait(kFp8 ? bars->q_ready[t] : bars->q_full[t], own & 1, kFp8 ? kTileWaitQReady : kTileWaitQFull);
-        ok = ok && ready(c0);
+        ok = ok && ready(c0, false);
         if (!ok) break;
         pv_cnt = 0;
         if (n_mine > 0) {
@@ -720,11 +726,12 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           issue_s(1, c0 % R::kRing);
         }
         umma_commit_if(leader, smem_u32(&bars->empty[c0 % R::kRing]));
+#pragma unroll 1
         for (int it = 0; ok && it < n_tiles; ++it) {
           const bool has_next = it + 1 < n_tiles;
           const int cv = c0 + 2 * it + 1, ck = cv + 1;
-          if (!has_next) umma_commit_if(leader, smem_u32(&bars->q_empty));  // every S MMA of the piece has been issued
-          ok = ready(cv);
+          if (it + 1 == n_mine) umma_commit_if(leader, smem_u32(&bars->q_empty[t]));  // every S MMA of the stream's piece has been issued
+          ok = ready(cv, (t0 + it + 1) * kKeyTile > lim_min);
           if (!ok) break;
           bool k_ready = false;
 #pragma unroll
@@ -740,7 +747,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               }
             }
             if (ok && has_next && !k_ready) {
-              ok = ready(ck);
+              ok = ready(ck, false);
               k_ready = ok;
             }
             if (ok && has_next && it + 1 < n_mine) issue_s(hf, ck % R::kRing);
@@ -760,45 +767,55 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       // ========================================================= the share's pieces, one after the other
       uint32_t n = 0;  // pieces handed out
       bool ok = true;
-      auto hand_out = [&](const ShareIter& at, int mode, int bit) {
-        const uint32_t i = n % kPieceRing;
-        ok = wait.one(bars->piece_empty[i], ((n / kPieceRing) & 1) ^ 1u, kTileWaitPiece);
-        if (!ok) return;
-        describe_piece(a, at, p, pieces[i]);
-        pieces[i].mode = mode;
-        pieces[i].bit = bit;
-        mbar_arrive(smem_u32(&bars->piece_full[i]));
-        ++n;
-      };
       auto all_done = [&]() {  // everybody has finished every piece handed out
         for (uint32_t k = n < kPieceRing ? 0 : n - kPieceRing; ok && k < n; ++k)
           ok = wait.one(bars->piece_empty[k % kPieceRing], (k / kPieceRing) & 1, kTileWaitPiece);
       };
-      bool more = bars->more != 0u;
-      int in_batch = 0;
+      bool more = bars->more != 0u, redoing = false, second = false;
+      int in_batch = 0, k = 0;  // pieces of the batch; the one that is looked at again
+      uint32_t redo = 0;
       if (more) {  // the first piece has been described already
         pieces[0].mode = kFirstTile;
         pieces[0].bit = in_batch++;
         mbar_arrive(smem_u32(&bars->piece_full[0]));
         n = 1;
       }
-      while (ok && more) {
-        while (ok && in_batch < kPieceBatch && (more = walk.next(a, p))) hand_out(walk, kFirstTile, in_batch++);
-        if (ok) all_done();
-        if (!ok) break;
-        const uint32_t redo = bars->redo;
-        bars->redo = 0;
-        for (int k = 0; ok && redo != 0u && k < in_batch; ++k) {
-          again.next(a, p);
-          if ((redo >> k) & 1u) {
-            hand_out(again, kFindMaxima, 31);
-            if (ok) hand_out(again, kUseMaxima, 31);
+#pragma unroll 1
+      while (ok && (more || redoing)) {
+        ShareIter& from = redoing ? again : walk;
+        int mode = kFirstTile, bit = 31;
+        if (second) {
+          second = false;
+          mode = kUseMaxima;
+        } else if ((redoing ? k : in_batch) < (redoing ? in_batch : kPieceBatch) && from.next(a, p)) {
+          if (redoing) {
+            if (((redo >> k++) & 1u) == 0u) continue;
+            second = true;
+            mode = kFindMaxima;
+          } else {
+            bit = in_batch++;
           }
+        } else {  // the batch, or what of it was to be done again, has been handed out
+          all_done();
+          if (!redoing) more = in_batch == kPieceBatch;
+          redo = redoing ? 0u : bars->redo;
+          bars->redo = 0;
+          redoing = redo != 0u;
+          k = 0;
+          if (!redoing) {
+            again = walk;
+            in_batch = 0;
+          }
+          continue;
         }
-        if (redo != 0u && ok) all_done();
-        bars->redo = 0;
-        again = walk;
-        in_batch = 0;
+        const uint32_t i = n % kPieceRing;
+        ok = wait.one(bars->piece_empty[i], ((n / kPieceRing) & 1) ^ 1u, kTileWaitPiece);
+        if (!ok) break;
+        describe_piece(a, from, p, pieces[i]);
+        pieces[i].mode = mode;
+        pieces[i].bit = bit;
+        mbar_arrive(smem_u32(&bars->piece_full[i]));
+        ++n;
       }
       if (ok) {
         const uint32_t i = n % kPieceRing;
@@ -811,7 +828,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     __syncwarp();
   } else {
     // =========================================================== softmax and results
-    setmaxnreg_inc<kTileSoftmaxRegs>();
     const int t = (warp >> 2) & 1, hf = warp >> 3, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
@@ -837,6 +853,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       return y;
     };
     const TilePiece* q;
+#pragma unroll 1
     for (; ok && (q = piece()) != nullptr; piece_done()) {
       const int n_mine = uniform(q->end[t]), mode = uniform(q->mode);
       const int row_i = a.by_group(row);                  // row r: token r / group, head r % group
@@ -883,6 +900,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       float l_sum = 0.f;
       bool over = false;
+#pragma unroll 1  // unrolled, it costs instruction cache: the whole kernel a sixth of its time on short pieces
       for (int it = 0; it < n_mine; ++it) {
         ok = wait(bars->s_full[t][hf], j & 1, kTileWaitS);
         if (!ok) break;
@@ -993,6 +1011,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   tc_fence_before_sync();
   __syncthreads();
   if (bars->abort_flag) {  // a wait gave up: give copies and MMAs in flight a bounded time to land
+    if (threadIdx.x == 0 && a.c.status) atomicCAS(a.c.status, 0, static_cast<int>(bars->abort_flag | (blockIdx.x << 8)));
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
     __syncthreads();

@@ -156,6 +156,10 @@ int32_t row_map(CUtensorMap* m, const void* ptr, bool codes, int n_outer, const 
 
 // log2 of the units (a tile, or an item's set-up) below which a share is not worth a CTA
 constexpr int kTileShareShift = 2, kFewShareShift = 1;
+// Units for an item's set-up: Q on its way, the first tile's maxima, the last P V.  With one unit for it the tile kernel's CTAs
+// with many items of a single key tile were the last to finish (prompts of 77 and 512 tokens: 138 us; 2: 122, 3: 125, 5: 127;
+// bf16 115, 114, 104, 111).
+constexpr int kTileSetUp = 3, kFewSetUp = 1;
 
 // What a call of this shape launches.
 struct AttnPlan {
@@ -202,12 +206,7 @@ int32_t launch_tile(const h3a_cache_attn_params* p, const h3a::CacheAttnArgs& a,
   static std::once_flag once[kMaxDevices];
   static cudaError_t err[kMaxDevices];
   std::call_once(once[dev.id], [&] {
-    cudaError_t e = cudaFuncSetAttribute(h3a::cache_attn_tile_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, h3a::kTileSmemBytes);
-    // the in-kernel register re-allocation would block forever if the launch allocation were smaller
-    cudaFuncAttributes fa;
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, h3a::cache_attn_tile_kernel<kFp8>);
-    if (e == cudaSuccess && fa.numRegs < h3a::kTileLaunchRegs) e = cudaErrorLaunchOutOfResources;
-    err[dev.id] = e;
+    err[dev.id] = cudaFuncSetAttribute(h3a::cache_attn_tile_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, h3a::kTileSmemBytes);
   });
   if (err[dev.id] != cudaSuccess) return H3A_ERR_LAUNCH;
   CUtensorMap mq, mk, mv;
@@ -301,11 +300,12 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   a.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / std::sqrt(128.0f)) * 1.4426950408889634f;
   a.desc = static_cast<int*>(p->workspace);
   a.part = reinterpret_cast<float*>(a.desc + h3a::kDescInts * n.shares);
+  a.set_up = n.item_tokens > 0 ? kTileSetUp : kFewSetUp;
   a.share_shift = n.item_tokens > 0 ? kTileShareShift : kFewShareShift;
   a.by_group = h3a::FastDiv::of(a.group);
   a.by_item_rows = h3a::FastDiv::of(n.item_rows);
   a.by_item_tokens = h3a::FastDiv::of(std::max(1, n.item_tokens));
-  a.wait_ns = p->wait_limit_ns > 0 ? p->wait_limit_ns : 2000000000ll;
+  a.wait_units = static_cast<uint32_t>(std::min<int64_t>((p->wait_limit_ns > 0 ? p->wait_limit_ns : 2000000000ll) >> 10, 0x7FFFFFFF));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (n.item_tokens > 0)
     rc = p->cache.quantised ? launch_tile<true>(p, a, n.shares, dev, st) : launch_tile<false>(p, a, n.shares, dev, st);
