@@ -158,91 +158,108 @@ __device__ __forceinline__ RowPlace place_of_row(const CacheArgs& a, int t) {
 constexpr int kRowThreads = 256;
 constexpr int kRowGroups = kRowThreads / 16;  // half-warps of a block
 
+// the larger magnitude of each half, its sign arbitrary; NaN wins
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // A half-warp moves rows of 128 values, 16 lanes x 8 values each: all heads of K and V of one token, or, when there are few
-// tokens, every `per_token`-th of them (per_token half-warps and gridDim.y blocks share a token).  The token's place is
-// looked up once; inside the loop an address is one multiplication away.  kUnroll rows are in flight per half-warp.
-// Looking every (token, head) row up by itself, with a division and a search each, took three times as long (clip of
-// 49,384 x 40 heads into e4m3: 688 us).  kWrite: packed -> cache; otherwise cache -> packed.
+// tokens, a part of them (per_token half-warps and gridDim.y blocks share a token).  The token's place is looked up once;
+// inside the loop an address is an addition away.  K and V rows of kUnroll heads are in flight per half-warp.
+// Quantising is bound by instructions rather than by memory: looking every (token, head) row up by itself, with a division
+// and a search each, took 688 us (clip of 49,384 x 40 heads into e4m3), computing every address by multiplication, with what
+// rows of NaN need in every row's way, 333 us; now it takes 277 us, 5.5 TB/s.  Reading it back takes 249 us, 6.1 TB/s;
+// unquantised 325 us in and 313 us out, 6.2 and 6.5 TB/s.
+// kWrite: packed -> cache; otherwise cache -> packed.
 template <bool kWrite, bool kQuantised>
-constexpr int kUnroll = kWrite && kQuantised ? 4 : 8;  // quantising wants registers for more warps: 301 against 314 us; reading 247 against 256
-constexpr int kExpRows = 256;  // rows of a token between two meetings of the exponent bytes
+constexpr int kUnroll = kWrite && kQuantised ? 2 : 4;  // quantising wants registers for more warps
+// Blocks per SM.  More warps hide the conversions of the quantised forms (write 277 us with 4, 286 with 3; read 249 and 268);
+// the plain copies want their registers instead (bf16 write 325 us with 2, 354 with 4; read 313 and 333).
+template <bool kQuantised>
+constexpr int kRowBlocksPerSm = kQuantised ? 4 : 2;
+constexpr int kExpHeads = 128;  // heads of a token between two meetings of the exponent bytes
 template <bool kWrite, bool kQuantised>
-__global__ void __launch_bounds__(kRowThreads) cache_rows_kernel(const __grid_constant__ RowsArgs a, const int per_token) {
+__global__ void __launch_bounds__(kRowThreads, kRowBlocksPerSm<kQuantised>) cache_rows_kernel(const __grid_constant__ RowsArgs a, const int per_token) {
   if (block_stops(a.c)) return;
-  constexpr int kRowUnroll = kUnroll<kWrite, kQuantised>;
+  constexpr int kHeads = kUnroll<kWrite, kQuantised>, kRows = 2 * kHeads;  // row i: K (i even) or V of head i / 2
   const int lane = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const uint32_t half_mask = (threadIdx.x & 16) ? 0xFFFF0000u : 0x0000FFFFu;
   const int t = blockIdx.x * (kRowGroups / per_token) + grp / per_token;
   RowPlace p{0, 0, 0};
   if (t < a.c.rows) p = place_of_row(a.c, t);
-  const int step = per_token * gridDim.y, n_rows = 2 * a.c.kv_heads;
-  uint8_t* const cached0 = a.c.pool[0] + p.id * a.c.page_bytes[0] + p.at * a.c.token_bytes[0] + lane * (kQuantised ? 8 : 16);
-  uint8_t* const cached1 = a.c.pool[1] + p.id * a.c.page_bytes[1] + p.at * a.c.token_bytes[1] + lane * (kQuantised ? 8 : 16);
-  uint8_t* const exps0 = kQuantised ? a.c.exps[0] + p.id * a.c.exp_page[0] + p.at * a.c.exp_token[0] : nullptr;
-  uint8_t* const exps1 = kQuantised ? a.c.exps[1] + p.id * a.c.exp_page[1] + p.at * a.c.exp_token[1] : nullptr;
-  uint8_t* const packed0 = a.x[0] + t * a.row_bytes[0] + lane * 16;
-  uint8_t* const packed1 = a.x[1] + t * a.row_bytes[1] + lane * 16;
-  // row y of a token: head y of K, then head y - kv_heads of V
-  auto cached_row = [&](int y) { return y < a.c.kv_heads ? cached0 + y * a.c.head_bytes[0] : cached1 + (y - a.c.kv_heads) * a.c.head_bytes[1]; };
-  auto exp_of = [&](int y, uint8_t* e0, uint8_t* e1) { return y < a.c.kv_heads ? e0 + y * a.c.exp_head[0] : e1 + (y - a.c.kv_heads) * a.c.exp_head[1]; };
-  auto packed_row = [&](int y) { return y < a.c.kv_heads ? packed0 + y * a.head_bytes[0] : packed1 + (y - a.c.kv_heads) * a.head_bytes[1]; };
+  const int step = per_token * gridDim.y, first_y = grp % per_token + per_token * blockIdx.y;
   // Exponent bytes of a write meet in shared memory, so that the 16 tokens' bytes of a head leave in one store (they are
   // neighbours in memory): a store per byte cost a fifth of the time.  With few tokens each lane stores its own.
-  const bool meet = kWrite && kQuantised && per_token == 1 && gridDim.y == 1;
-  __shared__ uint8_t exp_s[kWrite && kQuantised ? kExpRows : 1][kRowGroups];
-  __shared__ uint8_t* exp_at[kRowGroups][2];
+  const bool meet = kWrite && kQuantised && step == 1;
+  __shared__ uint8_t exp_s[kWrite && kQuantised ? 2 * kExpHeads : 1][kRowGroups];
+  __shared__ uint8_t* exp_at[2][kRowGroups];
   if (meet) {
-    if (lane == 0) {
-      exp_at[grp][0] = p.state == 2 ? exps0 : nullptr;
-      exp_at[grp][1] = exps1;
-    }
+    if (lane < 2) exp_at[lane][grp] = p.state == 2 ? a.c.exps[lane] + p.id * a.c.exp_page[lane] + p.at * a.c.exp_token[lane] : nullptr;
   } else if (p.state == 0 || (kWrite && p.state == 1)) {
     return;
   }
-  for (int c0 = 0; c0 < n_rows; c0 += kExpRows) {
-    const int c1 = min(n_rows, c0 + kExpRows);
-    for (int y0 = c0 + grp % per_token + per_token * blockIdx.y; y0 < c1; y0 += step * kRowUnroll) {
-      uint4 r[kRowUnroll];
-      uint32_t e[kRowUnroll];
+  const bool moves = p.state == 2 || (!kWrite && p.state == 1);
+  for (int c0 = 0; c0 < a.c.kv_heads; c0 += kExpHeads) {
+    const int c1 = min(a.c.kv_heads, c0 + kExpHeads);
+    const int y_first = c0 + first_y;
+    long long cache_step[2], packed_step[2], exp_step[2];
+    uint8_t *cached[2], *packed[2], *exps[2];
 #pragma unroll
-      for (int i = 0; i < kRowUnroll; ++i) {
-        const int y = y0 + i * step;
+    for (int x = 0; x < 2; ++x) {
+      cache_step[x] = step * a.c.head_bytes[x];
+      packed_step[x] = step * a.head_bytes[x];
+      exp_step[x] = step * a.c.exp_head[x];
+      cached[x] = a.c.pool[x] + p.id * a.c.page_bytes[x] + p.at * a.c.token_bytes[x] + y_first * a.c.head_bytes[x] + lane * (kQuantised ? 8 : 16);
+      packed[x] = a.x[x] + t * a.row_bytes[x] + y_first * a.head_bytes[x] + lane * 16;
+      exps[x] = kQuantised ? a.c.exps[x] + p.id * a.c.exp_page[x] + p.at * a.c.exp_token[x] + y_first * a.c.exp_head[x] : nullptr;
+    }
+#pragma unroll 1
+    for (int y0 = y_first; moves && y0 < c1; y0 += step * kHeads) {
+      uint4 r[kRows];
+      uint32_t e[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
         r[i] = make_uint4(0, 0, 0, 0);
         e[i] = 127;
-        if (y >= c1 || p.state != 2) continue;
+        const int x = i & 1;
+        const bool here = y0 + (i >> 1) * step < c1 && p.state == 2;
         if constexpr (kWrite) {
-          r[i] = ldg_stream(packed_row(y));
-        } else if constexpr (kQuantised) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(cached_row(y)));
-          r[i].x = w.x;
-          r[i].y = w.y;
-          e[i] = __ldg(exp_of(y, exps0, exps1));
+          if (here) r[i] = ldg_stream(packed[x]);
+          packed[x] += packed_step[x];
         } else {
-          r[i] = ldg_stream(cached_row(y));
+          if (here) {
+            if constexpr (kQuantised) {
+              const uint2 w = __ldg(reinterpret_cast<const uint2*>(cached[x]));
+              r[i].x = w.x;
+              r[i].y = w.y;
+              e[i] = __ldg(exps[x]);
+            } else {
+              r[i] = ldg_stream(cached[x]);
+            }
+          }
+          cached[x] += cache_step[x];
+          if constexpr (kQuantised) exps[x] += exp_step[x];
         }
       }
       if constexpr (kWrite && kQuantised) {
-        // the largest magnitude by its bits (finite values order as integers, NaN and infinity lie above them), two rows
-        // in the halves of one word
+        // the largest magnitude, two rows in the halves of one word
 #pragma unroll
-        for (int i = 0; i < kRowUnroll; i += 2) {
-          uint32_t m[2];
+        for (int i = 0; i < kRows; i += 2) {
+          const uint32_t m0 = max_abs_bf16x2(max_abs_bf16x2(r[i].x, r[i].y), max_abs_bf16x2(r[i].z, r[i].w));
+          const uint32_t m1 = max_abs_bf16x2(max_abs_bf16x2(r[i + 1].x, r[i + 1].y), max_abs_bf16x2(r[i + 1].z, r[i + 1].w));
+          uint32_t both = max_abs_bf16x2(__byte_perm(m0, m1, 0x5410), __byte_perm(m0, m1, 0x7632));
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const uint4& w = r[i + z];
-            m[z] = __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
-          }
-          uint32_t both = __vmaxu2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(half_mask, both, o));
-          e[i] = row_exponent(both & 0xFFFFu);
-          e[i + 1] = row_exponent(both >> 16);
+          for (int o = 8; o > 0; o >>= 1) both = max_abs_bf16x2(both, __shfl_xor_sync(half_mask, both, o));
+          e[i] = row_exponent(both & 0x7FFFu);
+          e[i + 1] = row_exponent((both >> 16) & 0x7FFFu);
         }
       }
 #pragma unroll
-      for (int i = 0; i < kRowUnroll; ++i) {
-        const int y = y0 + i * step;
-        if (y >= c1 || p.state == 0 || (kWrite && p.state == 1)) break;  // the same for the whole half-warp
+      for (int i = 0; i < kRows; ++i) {
+        const int x = i & 1, y = y0 + (i >> 1) * step;
+        if (y >= c1) break;  // the same for the whole half-warp
         if constexpr (!kWrite) {
           if constexpr (kQuantised) {
             const uint32_t f = e4m3_factor(e[i]) * 0x10001u, w0 = r[i].x, w1 = r[i].y;
@@ -255,36 +272,45 @@ __global__ void __launch_bounds__(kRowThreads) cache_rows_kernel(const __grid_co
               r[i] = make_uint4(mul_bf16x2(r[i].x, f2), mul_bf16x2(r[i].y, f2), mul_bf16x2(r[i].z, f2), mul_bf16x2(r[i].w, f2));
             }
           }
-          *reinterpret_cast<uint4*>(packed_row(y)) = r[i];
-        } else if constexpr (kQuantised) {
-          // 2^-k, exact in bf16 (what it takes below the type's smallest number is a zero in e4m3 anyway)
-          const uint32_t f = (254u - min(e[i], 247u)) * 0x800080u;
-          const uint32_t w[4] = {mul_bf16x2(r[i].x, f), mul_bf16x2(r[i].y, f), mul_bf16x2(r[i].z, f), mul_bf16x2(r[i].w, f)};
-          uint32_t c[4];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            float lo = __uint_as_float(w[z] << 16), hi = __uint_as_float(w[z] & 0xFFFF0000u);
-            if (e[i] == 247u) {  // the top of the range: a code of 256 would stand for 2^128, 240 is the last one that does not
-              lo = fminf(fmaxf(lo, -240.f), 240.f);
-              hi = fminf(fmaxf(hi, -240.f), 240.f);
-            }
-            c[z] = e[i] == 255u ? 0u : cvt_e4m3x2(lo, hi);  // a row that is not finite has no codes, only its byte
-          }
-          *reinterpret_cast<uint2*>(cached_row(y)) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-          if (lane == 0) {
-            if (meet) exp_s[y - c0][grp] = static_cast<uint8_t>(e[i]);
-            else *exp_of(y, exps0, exps1) = static_cast<uint8_t>(e[i]);
-          }
+          *reinterpret_cast<uint4*>(packed[x]) = r[i];
+          packed[x] += packed_step[x];
         } else {
-          *reinterpret_cast<uint4*>(cached_row(y)) = r[i];
+          if constexpr (kQuantised) {
+            // 2^-k, exact in bf16 (what it takes below the type's smallest number is a zero in e4m3 anyway)
+            const uint32_t f = (254u - min(e[i], 247u)) * 0x800080u;
+            const uint32_t w[4] = {mul_bf16x2(r[i].x, f), mul_bf16x2(r[i].y, f), mul_bf16x2(r[i].z, f), mul_bf16x2(r[i].w, f)};
+            uint32_t c[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) c[z] = cvt_e4m3x2(__uint_as_float(w[z] << 16), __uint_as_float(w[z] & 0xFFFF0000u));
+            if (e[i] >= 247u) {  // rare
+#pragma unroll
+              for (int z = 0; z < 4; ++z) {
+                // the top of the range: a code of 256 would stand for 2^128, 240 is the last one that does not
+                const float lo = fminf(fmaxf(__uint_as_float(w[z] << 16), -240.f), 240.f), hi = fminf(fmaxf(__uint_as_float(w[z] & 0xFFFF0000u), -240.f), 240.f);
+                c[z] = e[i] == 255u ? 0u : cvt_e4m3x2(lo, hi);  // a row that is not finite has no codes, only its byte
+              }
+            }
+            *reinterpret_cast<uint2*>(cached[x]) = make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
+            if (lane == 0) {
+              if (meet) exp_s[x * kExpHeads + y - c0][grp] = static_cast<uint8_t>(e[i]);
+              else *exps[x] = static_cast<uint8_t>(e[i]);
+            }
+            exps[x] += exp_step[x];
+          } else {
+            *reinterpret_cast<uint4*>(cached[x]) = r[i];
+          }
+          cached[x] += cache_step[x];
         }
       }
     }
     if (meet) {
       __syncthreads();
-      uint8_t *e0 = exp_at[lane][0], *e1 = exp_at[lane][1];  // lane: token of the block
-      if (e0 != nullptr)
-        for (int y = c0 + grp; y < c1; y += kRowGroups) *exp_of(y, e0, e1) = exp_s[y - c0][lane];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint8_t* to = exp_at[x][lane];  // lane: token of the block
+        if (to != nullptr)
+          for (int y = c0 + grp; y < c1; y += kRowGroups) to[y * a.c.exp_head[x]] = exp_s[x * kExpHeads + y - c0][lane];
+      }
       __syncthreads();
     }
   }

@@ -106,11 +106,11 @@ int32_t move_rows(bool write, const h3a_cache* c, const h3a_cache_batch* b, void
   a.head_bytes[1] = v_sh * 2;
   // Half-warps per token: one is the cheapest (a token is looked up once), but few tokens are spread over more of them,
   // up to a block's 16, and over further blocks, until about eight of them run on every SM.
-  const int64_t want = 8ll * dev.sms, n_rows = 2ll * c->heads;
+  const int64_t want = 8ll * dev.sms;
   int per_token = 1;
-  while (per_token < h3a::kRowGroups && b->rows * static_cast<int64_t>(per_token) < want && per_token < n_rows) per_token *= 2;
+  while (per_token < h3a::kRowGroups && b->rows * static_cast<int64_t>(per_token) < want && per_token < c->heads) per_token *= 2;
   const int64_t blocks_x = (b->rows + static_cast<int64_t>(h3a::kRowGroups / per_token) - 1) / (h3a::kRowGroups / per_token);
-  const int64_t more = std::max<int64_t>(1, std::min(want / std::max<int64_t>(1, b->rows * static_cast<int64_t>(per_token)), n_rows / per_token));
+  const int64_t more = std::max<int64_t>(1, std::min(want / std::max<int64_t>(1, b->rows * static_cast<int64_t>(per_token)), static_cast<int64_t>(c->heads) / per_token));
   const dim3 grid(static_cast<unsigned>(blocks_x), static_cast<unsigned>(more));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (write) {
