@@ -322,6 +322,30 @@ def test_attention_in_other_layouts(h, n, lengths, quantised):
     assert (room[c.rows :] == 5).all() and (room[:, 0] == 5).all() and (room[:, 11] == 5).all()
 
 
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("n", [1, 170])
+def test_rows_at_odd_multiples_of_16_bytes(h, n, quantised):
+    c = Case(h, [n], [n + 300], 4, 2, 16, quantised, seed=5).fill()
+    room = torch.full((n * 4 * D + 8,), 5.0, dtype=torch.bfloat16, device="cuda")
+    q = torch.empty(n * 4 * D + 8, dtype=torch.bfloat16, device="cuda")[8:].view(n, 4, D)
+    q.copy_(c.q)
+    out, lse = h.cache_attn(q, c.cache, c.batch, out=room[8:].view(n, 4, D), return_lse=True)
+    c.compare(out, lse, *c.reference(True))
+    assert (room[:8] == 5).all()
+
+
+# Items of one key tile, of none at all (rows before the sequence) and of many, on few enough heads that shares end within
+# an item's set-up as well as between its tiles; results must not depend on where the cuts are.
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("heads", [1, 3, 7])
+def test_shares_that_end_anywhere(h, heads, quantised):
+    n, lengths = [300, 700, 40, 257, 1, 900], [20, 90, 129, 3000, 1000, 128]
+    c = Case(h, n, lengths, heads, heads, 16, quantised, seed=6).fill()
+    for causal in (True, False):
+        out, lse = h.cache_attn(c.q.cuda(), c.cache, c.batch, causal=causal, return_lse=True)
+        c.compare(out, lse, *c.reference(causal))
+
+
 @pytest.mark.parametrize("n", [1, 6, 140])
 def test_rows_outside_every_sequence_are_left_alone(h, n):
     c = Case(h, [n], [400], 4, 4, 16, False).fill()
@@ -586,6 +610,10 @@ def test_refusals(h):
     with pytest.raises(_lib.H3AError) as e:
         h.cache_attn(q, c.cache, c.batch, max_new=-1)
     assert e.value.status == _lib.H3A_ERR_ARG
+    need = h.cache_attn_workspace_bytes(c.cache, c.batch, 2, 4)
+    with pytest.raises(_lib.H3AError) as e:
+        h.cache_attn(q, c.cache, c.batch, workspace=torch.empty(need + 16, dtype=torch.uint8, device="cuda")[16:])
+    assert e.value.status == _lib.H3A_ERR_ALIGN
     with pytest.raises(_lib.H3AError) as e:
         h.cache_attn(q, c.cache, c.batch, out=q)
     assert e.value.status == _lib.H3A_ERR_ARG
