@@ -203,8 +203,8 @@ def _workspace_bytes(device_index: int, rows: int, n_seqs: int, heads: int, kv_h
 
 
 def cache_attn_workspace_bytes(cache: KVCache, batch: CacheBatch, rows: int, heads: int, max_new: Optional[int] = None) -> int:
-    """Bytes of device scratch a ``cache_attn`` call of this shape needs; callers in a loop can allocate it once (one
-    per stream: calls that may run at the same time must not share it)."""
+    """Bytes of device scratch a ``cache_attn`` call of this shape needs; callers in a loop can allocate it once (32-byte
+    aligned; one per stream: calls that may run at the same time must not share it)."""
     return _workspace_bytes(cache.device.index, int(rows), batch._c.n_seqs, int(heads), cache.heads, cache.quantised, int(max_new or 0))
 
 

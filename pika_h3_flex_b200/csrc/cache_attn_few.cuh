@@ -17,6 +17,12 @@
 // 2^-31 of the row's largest, far below the rounding of P itself, as long as v - vr stays within 2^-8; a block of keys
 // whose exponents lie elsewhere takes bf16 MMAs with the power multiplied into the codes.  The integer route for every
 // block (5 instead of 1.5 instructions per pair) ran at 40 % of the HBM rate.
+//
+// Measured: one token over each of two contexts of 65,537 and 131,072 bf16 keys (40 heads on 8) 127 us, 6.3 TB/s; 64
+// contexts of 8,000 keys, 16 heads of their own, bf16 609 us, 6.9 TB/s, e4m3 361 us, 5.9 TB/s (some 500 instructions per 16
+// keys and warp, waiting for memory most of the time; reading two steps ahead into L2, and 3 or 5 blocks per SM instead of
+// 4, were not faster); 32 contexts of 200 to 16,384 e4m3 keys 59 us.  Calls of a few microseconds are latency: one token over
+// 1,023 bf16 keys takes 12 us, 3 of them memory's.
 #pragma once
 #include "cache_attn.cuh"
 
@@ -116,36 +122,39 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
     uint4 k[2 * kKW], v[4 * kVW];
     uint32_t e = 0;  // lanes 0-15: exponent byte of K row `lane`; lanes 16-31: of V row `lane - 16`
     auto raw_page = [&](int key) { return key < end_key ? __ldg(table + a.c.by_page(key)) : 0; };
-    auto check_page = [&](int id) -> long long {
+    auto check_page = [&](int id) -> int {
       if (static_cast<unsigned>(id) < static_cast<unsigned>(a.c.n_pages)) return id;
       report_cache(a.c, p.b);
       return 0;
     };
-    auto load_k = [&](long long id, int key) {
-      const int at = key - a.c.by_page(key) * a.c.page_size;
-      const uint8_t* src = a.c.pool[0] + id * a.c.page_bytes[0] + (at + gid) * a.c.token_bytes[0] + p.h * a.c.head_bytes[0] + 16 * tig;
+    // where this lane's parts of row 0 of page 0 are
+    const uint8_t* const k_at = a.c.pool[0] + p.h * a.c.head_bytes[0] + gid * a.c.token_bytes[0] + 16 * tig;
+    const uint8_t* const v_at = a.c.pool[1] + p.h * a.c.head_bytes[1] + 2 * tig * a.c.token_bytes[1] + 16 * gid;
+    const int ex = lane >> 4;
+    const uint8_t* const e_at = kFp8 ? a.c.exps[ex] + p.h * a.c.exp_head[ex] + (lane & 15) * a.c.exp_token[ex] : nullptr;
+    auto place = [&](int key) { return key - a.c.by_page(key) * a.c.page_size; };
+    auto load_k = [&](int id, int at) {
+      const uint8_t* src = k_at + id * a.c.page_bytes[0] + at * a.c.token_bytes[0];
 #pragma unroll
       for (int u = 0; u < 2; ++u, src += 8 * a.c.token_bytes[0])
 #pragma unroll
         for (int x = 0; x < kKW; ++x) k[u * kKW + x] = ldg_stream(src + 64 * x);
-      if constexpr (kFp8) {
-        const int x = lane >> 4;
-        e = __ldg(a.c.exps[x] + id * a.c.exp_page[x] + (at + (lane & 15)) * a.c.exp_token[x] + p.h * a.c.exp_head[x]);
-      }
+      if constexpr (kFp8) e = __ldg(e_at + id * a.c.exp_page[ex] + at * a.c.exp_token[ex]);
     };
-    auto load_v = [&](long long id, int key) {
-      const uint8_t* src = a.c.pool[1] + id * a.c.page_bytes[1] + (key - a.c.by_page(key) * a.c.page_size + 2 * tig) * a.c.token_bytes[1] + p.h * a.c.head_bytes[1] + 16 * gid;
+    auto load_v = [&](int id, int at) {
+      const uint8_t* src = v_at + id * a.c.page_bytes[1] + at * a.c.token_bytes[1];
 #pragma unroll
       for (int y = 0; y < 4; ++y)
 #pragma unroll
         for (int x = 0; x < kVW; ++x) v[y * kVW + x] = ldg_stream(src + ((y & 1) + 8 * (y >> 1)) * a.c.token_bytes[1] + 128 * x);
     };
 
-    long long id = 0;
+    int id = 0, at = 0;
     if (key0 < end_key) {
       id = check_page(raw_page(key0));
-      load_k(id, key0);
-      load_v(id, key0);
+      at = place(key0);
+      load_k(id, at);
+      load_v(id, at);
     }
     // ---- Q as B fragments, dims in the order of the K loads below: half-warps load rows, 8 dims per lane
 #pragma unroll
@@ -273,7 +282,8 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
       // the next 16 keys' K and exponents; their page was asked for a step ago, the page after it is asked for now
       if (next < end_key) {
         id = check_page(id_next);
-        load_k(id, next);
+        at = place(next);
+        load_k(id, at);
         id_next = raw_page(next + (1 << kFewKeyShift));
       }
       // ---- softmax: s[i][c] is key gid, s[i][2 + c] key gid + 8, of row 8 i + 2 tig + c
@@ -407,7 +417,7 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
           for (int i = 0; i < kNT; ++i) mma_bf16(o[i][j], vf, pf[i][0], pf[i][1]);
         }
       }
-      if (next < end_key) load_v(id, next);
+      if (next < end_key) load_v(id, at);
     }
 
     // ---- the warps meet.  A lane holds, of rows 8 i + 2 tig + c, dims 8 gid + [0, 8) and 64 + 8 gid + [0, 8) (e4m3:
