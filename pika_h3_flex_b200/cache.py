@@ -15,7 +15,6 @@ Packed tensors have logical shape ``[rows, heads, 128]`` like everywhere in the 
 from __future__ import annotations
 
 import ctypes as C
-from contextlib import nullcontext
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -113,12 +112,14 @@ class CacheBatch:
         return ref
 
 
-def _on(device: torch.device):
-    """Launches go to the tensors' device, whichever is current."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-_HERE = nullcontext()
+def _call(name: str, device: torch.device, *args) -> None:
+    """A C call on the tensors' device and its current stream, whichever device is current."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, _stream(device)), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream(device)), name)
 
 
 def _stream(device: torch.device) -> int:
@@ -130,6 +131,9 @@ def _stream(device: torch.device) -> int:
 def _rows(t: torch.Tensor, name: str, heads: int, device: torch.device) -> Tuple[int, int, int]:
     """Rows and the two strides of a packed [rows, heads, 128] bf16 tensor (these calls are made for single tokens too,
     so the checks are few and cheap)."""
+    if t.device != device:
+        _require_cuda(t)
+        raise ValueError(f"expected everything on {device}, got {name} on {t.device}")
     shape, stride = t.shape, t.stride()
     if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1:
         raise ValueError(f"{name}: expected logical [rows, heads, 128] with a contiguous last dim, got {tuple(shape)} / {stride}")
@@ -137,9 +141,6 @@ def _rows(t: torch.Tensor, name: str, heads: int, device: torch.device) -> Tuple
         raise TypeError(f"{name}: dtype {t.dtype} is not bfloat16")
     if shape[1] != heads:
         raise ValueError(f"{name} has {shape[1]} heads, expected {heads}")
-    if t.device != device:
-        _require_cuda(t)
-        raise ValueError(f"expected everything on {device}, got {name} on {t.device}")
     return shape[0], stride[0] if shape[0] > 1 else HEAD_DIM, stride[1] if heads > 1 else HEAD_DIM
 
 
@@ -162,16 +163,13 @@ def _move(name: str, cache: KVCache, batch: CacheBatch, k: torch.Tensor, v: torc
     status = _status_ptr(status_word, device)
     if L == 0:
         return
-    with _on(device):
-        check(getattr(_lib.load(), name)(cache._ref, batch._for(L), k.data_ptr(), ksl, ksh, v.data_ptr(), vsl, vsh, status,
-                                         _stream(device)), name)
+    _call(name, device, cache._ref, batch._for(L), k.data_ptr(), ksl, ksh, v.data_ptr(), vsl, vsh, status)
 
 
 def cache_write(cache: KVCache, batch: CacheBatch, k: torch.Tensor, v: torch.Tensor, status_word: Optional[torch.Tensor] = None) -> None:
     """Put the batch's rows ``k``, ``v`` ``[rows, heads, 128]`` bf16 into the cache, quantised if it is (per row: the
     smallest power of two that brings the largest magnitude to at most 448, then e4m3).  A page that is written to must
     belong to one sequence only; pages that are only read may be shared."""
-    _require_cuda(k, v)
     _move("h3a_cache_write", cache, batch, k, v, status_word)
 
 
@@ -185,9 +183,8 @@ def cache_read(cache: KVCache, batch: CacheBatch, rows: Optional[int] = None, ou
     if out is None:
         if rows < 0:
             raise ValueError("rows must not be negative")
-        out = [torch.empty(rows, cache.heads, HEAD_DIM, dtype=torch.bfloat16, device=cache.device) for _ in range(2)]
+        out = torch.empty(2, rows, cache.heads, HEAD_DIM, dtype=torch.bfloat16, device=cache.device).unbind()
     k, v = out
-    _require_cuda(k, v)
     _move("h3a_cache_read", cache, batch, k, v, status_word)
     return k, v
 
@@ -244,6 +241,5 @@ def cache_attn(q: torch.Tensor, cache: KVCache, batch: CacheBatch, causal: bool 
     p = _lib.CacheAttnParams(cache._c, batch._c, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, qsl, qsh, osl, osh,
                              H, 1 if causal else 0, softmax_scale, max_new or 0, workspace.data_ptr(), workspace.nbytes, status, wait_limit_ns)
     p.batch.rows = L
-    with _on(device):
-        check(_lib.load().h3a_cache_attn(C.byref(p), _stream(device)), "h3a_cache_attn")
+    _call("h3a_cache_attn", device, C.byref(p))
     return (out, lse) if return_lse else out
