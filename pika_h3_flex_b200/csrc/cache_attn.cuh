@@ -36,6 +36,7 @@ struct CacheAttnArgs {
   float scale_log2;
   float* part;                       // [share][2][item_rows] x (128 + 2) fp32
   int* desc;                         // [share][kDescInts]: the item that a share begins and does not finish
+  int shares;                        // CTAs of the kernel
   int set_up;                        // units that an item costs beside one per tile
   int share_shift;                   // a share has at least 2^this units
   uint32_t wait_units;               // longest wait, in 1,024 ns
@@ -346,11 +347,70 @@ __device__ __forceinline__ void describe_join(const CacheAttnArgs& a, const Shar
   d[4] = h;
 }
 
-// Block (share, y): rows 4 y + [0, 4), and so on, of the item that begins in the share and ends in a later one.  The kernel is a few
-// dependent loads long, so its launch overlaps the kernel before it, everything it has to know about the item is in the
-// description, and the loads of kJoinParts parts' O wait for nothing else: with the parts one after the other a row of 37
-// parts took 29 us.  16 at a time for small items (up to as many parts as shares), 4 for large ones (two or three, and
-// many rows: registers for more warps).
+// A warp's share of a row's parts, first_part, first_part + stride, ... kJoinParts at a time, whose loads wait for nothing
+// but the item's description: with the parts one after the other a row of 37 took 29 us.
+struct JoinRow {
+  float m, l;
+  float4 acc;  // dims 4 lane + [0, 4)
+};
+template <int kJoinParts>
+__device__ __forceinline__ JoinRow join_parts(const CacheAttnArgs& a, int share, int r, int n_parts, int first_part, int stride) {
+  const int lane = threadIdx.x & 31;
+  // parts of the row: the tail slot of its first share, then the head slots of the next ones
+  const long long slot = 2ll * a.item_rows * (kCacheDim + 2);
+  const float* first = part_slot(a, share, true);
+  const float* next = part_slot(a, share, false);  // + i slots for part i > 0
+  JoinRow row{kNoMax, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i0 = first_part; i0 < n_parts; i0 += stride) {
+    const int n = min(kJoinParts, n_parts - i0);
+    float4 v[kJoinParts];
+#pragma unroll
+    for (int i = 0; i < kJoinParts; ++i)
+      if (i < n) v[i] = *reinterpret_cast<const float4*>((i0 + i == 0 ? first : next + (i0 + i) * slot) + r * kCacheDim + 4 * lane);
+    float mi = kNoMax, li = 0.f;
+    if (lane < n) {
+      const float* st = (i0 + lane == 0 ? first : next + (i0 + lane) * slot) + a.item_rows * kCacheDim + r;
+      mi = st[0];
+      li = st[a.item_rows];
+    }
+    float top = mi;
+#pragma unroll
+    for (int o = kJoinParts / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    top = __shfl_sync(0xFFFFFFFFu, top, 0);
+    const float m_new = fmaxf(row.m, top), f = ex2_approx(row.m - m_new), wi = ex2_approx(mi - m_new);
+    row.m = m_new;
+    row.l *= f;
+    row.acc = make_float4(row.acc.x * f, row.acc.y * f, row.acc.z * f, row.acc.w * f);
+#pragma unroll
+    for (int i = 0; i < kJoinParts; ++i)
+      if (i < n) {
+        const float w = __shfl_sync(0xFFFFFFFFu, wi, i);
+        row.l += w * __shfl_sync(0xFFFFFFFFu, li, i);
+        row.acc.x += v[i].x * w;
+        row.acc.y += v[i].y * w;
+        row.acc.z += v[i].z * w;
+        row.acc.w += v[i].w * w;
+      }
+  }
+  return row;
+}
+// row `row` (token * group + head in the group) of the sequence whose first packed row is s0
+__device__ __forceinline__ void store_joined(const CacheAttnArgs& a, const JoinRow& x, int row, int s0, int kv_head) {
+  const int lane = threadIdx.x & 31;
+  const int i = a.by_group(row), token = s0 + i, head = kv_head * a.group + row - i * a.group;
+  const float inv = x.l == 0.f ? 0.f : 1.0f / x.l;
+  uint2 w;
+  w.x = pack_bf16x2(x.acc.x * inv, x.acc.y * inv);
+  w.y = pack_bf16x2(x.acc.z * inv, x.acc.w * inv);
+  *reinterpret_cast<uint2*>(a.o + token * a.o_stride_l + head * a.o_stride_h + 4 * lane) = w;
+  if (a.lse && lane == 0)
+    a.lse[static_cast<long long>(head) * a.c.rows + token] = x.l == 0.f ? -INFINITY : (x.m + log2f(x.l)) * 0.6931471805599453f;
+}
+
+// Block (share, y): rows 4 y + [0, 4), and so on, of the item that begins in the share and ends in a later one, a warp per
+// row.  The kernel is a few dependent loads long, so its launch overlaps the kernel before it, and everything it has to know
+// about the item is in the description.  16 parts at a time for small items, 4 for large ones (two or three, and many rows:
+// registers for more warps).
 template <int kJoinParts>
 __global__ void __launch_bounds__(kJoinRows * 32) cache_attn_join_kernel(const __grid_constant__ CacheAttnArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial results are complete from here on
@@ -358,56 +418,64 @@ __global__ void __launch_bounds__(kJoinRows * 32) cache_attn_join_kernel(const _
   const int4 d = *reinterpret_cast<const int4*>(a.desc + kDescInts * share);
   const int kv_head = a.desc[kDescInts * share + 4];
   if (a.c.status && *reinterpret_cast<volatile int*>(a.c.status) != 0) return;
-  const int lane = threadIdx.x & 31;
   const int n_parts = d.x, n_rows = d.y, r0 = d.z;
   if (n_parts <= 0) return;
-  // parts of the row: the tail slot of this share, then the head slots of the next ones
-  const long long slot = 2ll * a.item_rows * (kCacheDim + 2);
-  const float* first = part_slot(a, share, true);
-  const float* next = part_slot(a, share, false);  // + i slots for part i > 0
-  for (int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5); r < n_rows; r += kJoinRows * gridDim.y) {
-    float m = kNoMax, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < n_parts; i0 += kJoinParts) {
-      const int n = min(kJoinParts, n_parts - i0);
-      float4 v[kJoinParts];
-#pragma unroll
-      for (int i = 0; i < kJoinParts; ++i)
-        if (i < n) v[i] = *reinterpret_cast<const float4*>((i0 + i == 0 ? first : next + (i0 + i) * slot) + r * kCacheDim + 4 * lane);
-      float mi = kNoMax, li = 0.f;
-      if (lane < n) {
-        const float* st = (i0 + lane == 0 ? first : next + (i0 + lane) * slot) + a.item_rows * kCacheDim + r;
-        mi = st[0];
-        li = st[a.item_rows];
-      }
-      float top = mi;
-#pragma unroll
-      for (int o = kJoinParts / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      top = __shfl_sync(0xFFFFFFFFu, top, 0);
-      const float m_new = fmaxf(m, top), f = ex2_approx(m - m_new), wi = ex2_approx(mi - m_new);
-      m = m_new;
-      l *= f;
-      acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-#pragma unroll
-      for (int i = 0; i < kJoinParts; ++i)
-        if (i < n) {
-          const float w = __shfl_sync(0xFFFFFFFFu, wi, i);
-          l += w * __shfl_sync(0xFFFFFFFFu, li, i);
-          acc.x += v[i].x * w;
-          acc.y += v[i].y * w;
-          acc.z += v[i].z * w;
-          acc.w += v[i].w * w;
-        }
+  for (int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5); r < n_rows; r += kJoinRows * gridDim.y)
+    store_joined(a, join_parts<kJoinParts>(a, share, r, n_parts, 0, kJoinParts), r0 + r, d.w, kv_head);
+}
+
+// The same for few items in very many parts (a long context on one K/V head: a part per share): block (k, r) looks for the
+// k-th item that is in parts, and its 16 warps share the parts of the item's row r.  A warp per row went through 592 parts in
+// 37 steps.
+constexpr int kWideWarps = 16, kWideParts = 8;
+__global__ void __launch_bounds__(kWideWarps * 32, 2) cache_attn_join_wide_kernel(const __grid_constant__ CacheAttnArgs a) {
+  __shared__ int n_before[kWideWarps], found;
+  __shared__ float m_s[kWideWarps], l_s[kWideWarps];
+  __shared__ float4 acc_s[kWideWarps][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial results are complete from here on
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) found = -1;
+  if (block_stops(a.c)) return;
+  int rank = 0;  // items in parts among the shares so far
+  for (int s0 = 0; s0 < a.shares; s0 += kWideWarps * 32) {
+    const int s = s0 + threadIdx.x;
+    const bool here = s < a.shares && a.desc[kDescInts * s] > 0;
+    const uint32_t votes = __ballot_sync(0xFFFFFFFFu, here);
+    __syncthreads();  // the last round's counts have been read
+    if (lane == 0) n_before[warp] = __popc(votes);
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < kWideWarps; ++w) {
+      before += w < warp ? n_before[w] : 0;
+      if (w == warp && here && rank + before + __popc(votes & ((1u << lane) - 1u)) == static_cast<int>(blockIdx.x)) found = s;
     }
-    const int row = r0 + r, i = a.by_group(row), token = d.w + i, head = kv_head * a.group + row - i * a.group;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    uint2 w;
-    w.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-    w.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(a.o + token * a.o_stride_l + head * a.o_stride_h + 4 * lane) = w;
-    if (a.lse && lane == 0)
-      a.lse[static_cast<long long>(head) * a.c.rows + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    for (int w = 0; w < kWideWarps; ++w) rank += n_before[w];
   }
+  __syncthreads();
+  const int share = found, r = blockIdx.y;
+  if (share < 0) return;
+  const int4 d = *reinterpret_cast<const int4*>(a.desc + kDescInts * share);
+  if (r >= d.y) return;
+  const JoinRow mine = join_parts<kWideParts>(a, share, r, d.x, warp * kWideParts, kWideWarps * kWideParts);
+  acc_s[warp][lane] = mine.acc;
+  if (lane == 0) {
+    m_s[warp] = mine.m;
+    l_s[warp] = mine.l;
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  JoinRow x{kNoMax, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int w = 0; w < kWideWarps; ++w) x.m = fmaxf(x.m, m_s[w]);
+  for (int w = 0; w < kWideWarps; ++w) {
+    const float f = ex2_approx(m_s[w] - x.m);
+    const float4 v = acc_s[w][lane];
+    x.l += l_s[w] * f;
+    x.acc.x += v.x * f;
+    x.acc.y += v.y * f;
+    x.acc.z += v.z * f;
+    x.acc.w += v.w * f;
+  }
+  store_joined(a, x, d.z + r, d.w, a.desc[kDescInts * share + 4]);
 }
 
 }  // namespace h3a

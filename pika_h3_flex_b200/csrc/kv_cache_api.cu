@@ -226,18 +226,30 @@ int32_t launch_tile(const h3a_cache_attn_params* p, const h3a::CacheAttnArgs& a,
   return cudaGetLastError() == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
 }
 
-int32_t launch_join(const h3a::CacheAttnArgs& a, int shares, cudaStream_t st) {
+int32_t launch_join(const h3a::CacheAttnArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  // a warp per row where rows are few, and per two rows of larger items: 8 blocks per item instead of 32 left 20 items of
-  // 252 rows in 18 parts to too few warps (chunks of 3 to 301 tokens: 53 against 39 us in all), 64 are not faster
-  cfg.gridDim = dim3(shares, std::min(32, a.item_rows / h3a::kJoinRows));
-  cfg.blockDim = dim3(h3a::kJoinRows * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the end of the kernel before it
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  // at most so many items: sequences, and as many more as their rows fill
+  const int64_t rows = static_cast<int64_t>(a.c.rows) * a.group;
+  const int64_t items = a.c.kv_heads * (a.c.n_seqs + std::max<int64_t>(0, rows - a.c.n_seqs) / a.item_rows);
+  // ... in at most so many parts, of two units at least
+  const int64_t parts = std::min<int64_t>(a.shares / items, static_cast<int64_t>(a.c.max_pages) * a.c.page_size >> (a.key_shift + a.share_shift));
+  // More than the 16 parts that a warp takes at a time: one token over 131,072 keys, 8 heads on 1, 26 against 49 us; with
+  // fewer the other is faster (over 1,023 keys, 8 heads: 10 against 12 us).
+  if (a.item_tokens == 0 && parts > 16) {
+    cfg.gridDim = dim3(static_cast<unsigned>(items), a.item_rows);
+    cfg.blockDim = dim3(h3a::kWideWarps * 32);
+    return cudaLaunchKernelEx(&cfg, h3a::cache_attn_join_wide_kernel, a) == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
+  }
+  // a warp per row where rows are few, and per two rows of larger items: 8 blocks per item instead of 32 left 20 items of
+  // 252 rows in 18 parts to too few warps (chunks of 3 to 301 tokens: 53 against 39 us in all), 64 are not faster
+  cfg.gridDim = dim3(a.shares, std::min(32, a.item_rows / h3a::kJoinRows));
+  cfg.blockDim = dim3(h3a::kJoinRows * 32);
   const auto kernel = a.item_tokens > 0 ? h3a::cache_attn_join_kernel<4> : h3a::cache_attn_join_kernel<16>;
   return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? H3A_OK : H3A_ERR_LAUNCH;
 }
@@ -300,6 +312,7 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   a.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / std::sqrt(128.0f)) * 1.4426950408889634f;
   a.desc = static_cast<int*>(p->workspace);
   a.part = reinterpret_cast<float*>(a.desc + h3a::kDescInts * n.shares);
+  a.shares = n.shares;
   a.set_up = n.item_tokens > 0 ? kTileSetUp : kFewSetUp;
   a.share_shift = n.item_tokens > 0 ? kTileShareShift : kFewShareShift;
   a.by_group = h3a::FastDiv::of(a.group);
@@ -313,7 +326,7 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
     rc = p->cache.quantised ? launch_few<true, 1>(a, n.shares, dev, st) : launch_few<false, 1>(a, n.shares, dev, st);
   else
     rc = p->cache.quantised ? launch_few<true, 2>(a, n.shares, dev, st) : launch_few<false, 2>(a, n.shares, dev, st);
-  return rc == H3A_OK ? launch_join(a, n.shares, st) : rc;
+  return rc == H3A_OK ? launch_join(a, st) : rc;
 }
 
 }  // extern "C"

@@ -334,6 +334,16 @@ def test_rows_at_odd_multiples_of_16_bytes(h, n, quantised):
     assert (room[:8] == 5).all()
 
 
+# Few items in very many parts: every share of the device has one of the same few rows.
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("n,lengths,heads,kv_heads", [([1], [70000], 8, 1), ([2], [40001], 5, 1), ([1, 1], [30003, 17], 2, 2), ([0, 3, 0], [5, 9000, 800], 4, 2), ([7], [300], 2, 1)])
+def test_few_rows_over_long_contexts(h, n, lengths, heads, kv_heads, quantised):
+    c = Case(h, n, lengths, heads, kv_heads, 64, quantised, seed=8).fill()
+    for causal in (True, False):
+        out, lse = h.cache_attn(c.q.cuda(), c.cache, c.batch, causal=causal, return_lse=True)
+        c.compare(out, lse, *c.reference(causal))
+
+
 # Items of one key tile, of none at all (rows before the sequence) and of many, on few enough heads that shares end within
 # an item's set-up as well as between its tiles; results must not depend on where the cuts are.
 @pytest.mark.parametrize("quantised", [False, True])
