@@ -550,6 +550,23 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const int mode = uniform(q->mode), lim_min = uniform(q->lim_min);
         if (n_tiles == 0) continue;
         const int n_streams = uniform((q->end[0] > 0 ? 1 : 0) | (q->end[1] > 0 ? 2 : 0));
+        // Q is free late in the previous piece, ring slots earlier: the first K tile goes ahead of Q, but for the first piece,
+        // where it has to wait for page numbers
+        auto load_q = [&]() {
+#pragma unroll 1
+          for (int t = 0; ok && t < 2; ++t) {
+            if (((n_streams >> t) & 1) == 0) continue;
+            ok = wait(bars->q_empty[t], (q_phase >> t) & 1, kTileWaitQEmpty);
+            if (!ok) break;
+            q_phase ^= 1u << t;
+            const uint32_t bar = smem_u32(&bars->q_full[t]);
+            if (lane == 0) mbar_arrive_expect_tx(bar, q_bytes);
+            __syncwarp();
+            if (lane < 2) tma_load_3d(q_smem + t * kTileBytes + lane * kTileHalf, &tm_q, bar, 64 * lane, h * a.group, q->row0 + t * T);
+            __syncwarp();
+          }
+        };
+        if (n_pieces == 0) load_q();
         // A lane looks after 4 rows of every tile, which are in one page.  Its page number is fetched two tiles ahead, the rows'
         // exponent bytes (e4m3) one tile ahead; nothing looks at either before it is needed, or the loads would be waited for.
         int id = 0, id_next = 0;
@@ -620,22 +637,8 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (it < 0) continue;  // only the fetches
 #pragma unroll 1
           for (int x = 0; ok && x < 2; ++x, ++cnt) {
-            // Q is free late in the previous piece, ring slots earlier: the first K tile goes ahead of Q
-            if (it == 0 && x == 1) {
-#pragma unroll 1
-              for (int t = 0; t < 2; ++t) {
-                if (((n_streams >> t) & 1) == 0) continue;
-                ok = wait(bars->q_empty[t], (q_phase >> t) & 1, kTileWaitQEmpty);
-                if (!ok) break;
-                q_phase ^= 1u << t;
-                const uint32_t bar = smem_u32(&bars->q_full[t]);
-                if (lane == 0) mbar_arrive_expect_tx(bar, q_bytes);
-                __syncwarp();
-                if (lane < 2) tma_load_3d(q_smem + t * kTileBytes + lane * kTileHalf, &tm_q, bar, 64 * lane, h * a.group, q->row0 + t * T);
-                __syncwarp();
-              }
-              if (!ok) break;
-            }
+            if (it == 0 && x == 1 && n_pieces > 0) load_q();
+            if (!ok) break;
             const CUtensorMap* tm = x ? &tm_v : &tm_k;
             uint32_t dst, bar;
             if constexpr (kFp8) {
