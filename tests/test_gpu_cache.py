@@ -344,6 +344,13 @@ def test_few_rows_over_long_contexts(h, n, lengths, heads, kv_heads, quantised):
         c.compare(out, lse, *c.reference(causal))
 
 
+# Enough rows that a half-warp takes whole tokens, whose exponents leave together: more heads than meet at a time, and few.
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("n,lengths,kv_heads,page,layout", [([700, 601], [700, 640], 130, 16, "head"), ([1300, 0, 77], [1300, 9, 100], 3, 32, "token")])
+def test_many_rows_are_exact(h, quantised, n, lengths, kv_heads, page, layout):
+    test_write_and_read_are_exact(h, quantised, n, lengths, kv_heads, page, layout)
+
+
 # Items of one key tile, of none at all (rows before the sequence) and of many, on few enough heads that shares end within
 # an item's set-up as well as between its tiles; results must not depend on where the cuts are.
 @pytest.mark.parametrize("quantised", [False, True])
