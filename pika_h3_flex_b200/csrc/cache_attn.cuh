@@ -333,6 +333,10 @@ __device__ __forceinline__ float v_value(const CacheAttnArgs& a, int b, int h, i
 
 constexpr float kNoMax = -3.0e38f;  // running maximum of a row that has seen no key: finite, so that differences stay numbers
 
+// Least factor from S to logits.  A row of zeros in Q against rows of zeros in K has one that underflows, and a masked logit
+// times 0 is no longer -inf but NaN; with this one such a row's own logits, at most 2^21 times it, are still 0.
+constexpr float kLeastUnit = 1.17549435e-38f;  // 2^-126
+
 // lets the launch of the kernel that follows (the join) begin; it waits for this one's results itself
 __device__ __forceinline__ void allow_next_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
       for (int c = 0; c < 2; ++c) {
         const int r = 8 * i + 2 * tig + c;
         lim[i][c] = r < n_rows ? key_limit(a, p.s, a.by_group(r0 + r)) : 0;
-        q_unit[i][c] = kFp8 ? sm.q_scale[r] * a.scale_log2 : 0.f;
+        q_unit[i][c] = kFp8 ? fmaxf(sm.q_scale[r] * a.scale_log2, kLeastUnit) : 0.f;
       }
     int id_next = raw_page(key0 + (1 << kFewKeyShift));
     for (; key0 < end_key; key0 += 1 << kFewKeyShift) {

@@ -919,7 +919,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         bool wide = false;
         if constexpr (kFp8) {
           const TileInfo& in = info[(n_before + it) % kInfoRing];
-          c = fminf(row_unit * __uint_as_float(static_cast<uint32_t>(in.kref) << 23), 3.0e38f);
+          c = fminf(fmaxf(row_unit * __uint_as_float(static_cast<uint32_t>(in.kref) << 23), kLeastUnit), 3.0e38f);
           wide = in.wide != 0;
         }
         const bool partly = (it + 1) * kKeyTile - 64 > lim_first;
