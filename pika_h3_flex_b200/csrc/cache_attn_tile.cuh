@@ -24,9 +24,11 @@
 // (5.5 warps stalled on instruction fetch per issue); the loop here is a quarter of it.
 //
 // e4m3 tiles become fp16, two instructions per pair: a code is exact in fp16 (one conversion), and so is its product with
-// 2^(k - kref), kref being the tile's largest exponent, down to k - kref = -15 (below that a row's logits are off by less
-// than 2^-30 of the tile's largest).  2^kref goes into the tile's softmax scale, and Q into fp16 by a power of two per row
-// that joins that scale too.  V and O are in units of the largest exponent of the piece's first tile; fp16 holds codes up
+// 2^(k - kref), kref being the tile's largest exponent, down to k - kref = -15.  2^kref goes into the tile's softmax scale, and
+// Q into fp16 by a power of two per row that joins that scale too.  A K tile whose exponents lie further apart (its largest key
+// may weigh nothing, or be hidden, so that all others count with all their bits) keeps the bare codes, and the softmax warps
+// multiply each column of S by its key's power first, in tensor memory, so that the ordinary loop stays as short as it is.
+// V and O are in units of the largest exponent of the piece's first tile; fp16 holds codes up
 // to 2^7 above that, and rows 2^14 below it with all their bits.  A V tile with rows outside that is widened to bf16
 // instead, and its P rounded to bf16.  (Everything through bf16 took five instructions per pair.)
 //
@@ -167,11 +169,32 @@ struct TilePiece {
 };
 // e4m3: what a tile's rows were widened with
 struct TileInfo {
-  int kref;       // the tile's logits are in units of 2^(kref - 127)
+  int kref;       // the tile's logits are in units of 2^(kref - 127); 0: K as bare codes, each key in units of its own
   int vref;       // V, and so O, is in units of 2^(vref - 127): the same for a piece's tiles
   int wide;       // V is bf16, and P is to be
 };
 constexpr int kInfoRing = 8;  // the producer is at most four tiles ahead of the softmax warps
+// S of one row times a factor per key: 64 columns, the keys' exponent bytes at e_at.  A call of its own: in line, the hot loop
+// around it took 1.5 % longer (chunk of 2,048 over 20,011 keys 806 us against 792).
+__device__ __noinline__ void scale_columns(uint32_t s_addr, uint32_t e_at, float row_unit) {
+#pragma unroll 1
+  for (int x = 0; x < 64; x += 16) {
+    uint32_t r[16];
+    uint4 e;
+    tmem_ld16(s_addr + x, r);
+    ld_shared_v4(e_at + x, e);
+    const uint32_t ex[4] = {e.x, e.y, e.z, e.w};
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      asm volatile("" : "+r"(r[i]));  // not before the wait
+      const uint32_t power = (ex[i >> 2] >> (8 * (i & 3))) & 0xFFu;
+      r[i] = __float_as_uint(__uint_as_float(r[i]) * fminf(row_unit * __uint_as_float(power << 23), 3.0e38f));
+    }
+    tmem_st16(s_addr + x, r);
+  }
+  tmem_wait_st();
+}
 // 2^-d as an fp16 pair, d >= -15
 __device__ __forceinline__ uint32_t f16x2_pow2_neg(int d) {
   const uint32_t h = d <= 14 ? static_cast<uint32_t>(15 - d) << 10 : d <= 24 ? 1u << (24 - d) : 0u;
@@ -260,7 +283,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   __shared__ ShareIter walk, again;         // the piece warp's: where it is in the share, where its batch began
   __shared__ Piece p;
   __shared__ TileInfo info[kInfoRing];
-  __shared__ alignas(4) uint8_t exps[kInfoRing][2][kKeyTile];  // e4m3: the exponent bytes of a tile's rows of K and V
+  __shared__ alignas(16) uint8_t exps[kInfoRing][2][kKeyTile];  // e4m3: the exponent bytes of a tile's rows of K and V
   static_assert(kTileSmemBytes + sizeof(ShareStart) + sizeof(TilePiece) * kPieceRing + 2 * sizeof(ShareIter) + sizeof(Piece) + (sizeof(TileInfo) + 2 * kKeyTile) * kInfoRing <= 232448, "shared memory budget");
   using R = TileRing<kFp8>;
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -389,7 +412,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const bool put_back = x == 1 && special && !gone && e == 255;
             if (put_back) bars->poison = 1u;
             const bool none = gone || put_back;
-            const int d = (x ? in.vref : in.kref) - e;  // the row's power of two against the unit's
+            const int d = x ? in.vref - e : in.kref != 0 ? in.kref - e : 0;  // the row's power of two against the unit's
             if (x == 1 && in.wide) {
               const uint32_t f = none ? 0u : e == 255 ? 0x7FFF7FFFu : static_cast<uint32_t>(max(0, min(254, 247 - d))) * 0x800080u;
               widen_row<true>(src, dst, swz, f, none);
@@ -602,18 +625,20 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, mine)) * box_bytes;
           const int page = __shfl_sync(0xFFFFFFFFu, id, (lane * box_rows / 4) & 31);
           if (kFp8 && it >= 0) {
-            // the tile's largest exponents, and V's smallest; rows of nothing (7) and rows that are not finite (255) aside
-            uint32_t k_top = 0, v_top = 0, v_low = 255;
+            // the tile's largest and smallest exponents, rows that are not finite (255) aside, and of V rows of nothing (7) too
+            uint32_t k_top = 0, k_low = 255, v_top = 0, v_low = 255;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t x = raw_k[i], y = raw_v[i];
               if (x != 255u) k_top = max(k_top, x);
+              if (x != 0u) k_low = min(k_low, x);  // 0: no key
               if (y > 7u && y != 255u) {
                 v_top = max(v_top, y);
                 v_low = min(v_low, y);
               }
             }
             k_top = __reduce_max_sync(0xFFFFFFFFu, k_top);
+            k_low = __reduce_min_sync(0xFFFFFFFFu, k_low);
             v_top = __reduce_max_sync(0xFFFFFFFFu, v_top);
             v_low = __reduce_min_sync(0xFFFFFFFFu, v_low);
             const int vt = static_cast<int>(v_top), vl = static_cast<int>(v_low);
@@ -623,7 +648,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             *reinterpret_cast<uint32_t*>(&exps[slot][0][4 * lane]) = raw_k[0] | (raw_k[1] << 8) | (raw_k[2] << 16) | (raw_k[3] << 24);
             *reinterpret_cast<uint32_t*>(&exps[slot][1][4 * lane]) = raw_v[0] | (raw_v[1] << 8) | (raw_v[2] << 16) | (raw_v[3] << 24);
             if (lane == 0) {
-              info[slot].kref = static_cast<int>(k_top);
+              info[slot].kref = k_top > k_low + 15u ? 0 : static_cast<int>(k_top);
               info[slot].vref = vref;
               if (it == 0) const_cast<TilePiece*>(q)->vref = vref;
               info[slot].wide = vl + 14 < vref || vt > vref + 7;
@@ -918,9 +943,14 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         float c = row_unit;
         bool wide = false;
         if constexpr (kFp8) {
-          const TileInfo& in = info[(n_before + it) % kInfoRing];
-          c = fminf(fmaxf(row_unit * __uint_as_float(static_cast<uint32_t>(in.kref) << 23), kLeastUnit), 3.0e38f);
-          wide = in.wide != 0;
+          const uint32_t slot = (n_before + it) % kInfoRing;
+          const int kref = info[slot].kref;
+          wide = info[slot].wide != 0;
+          c = fminf(fmaxf(row_unit * __uint_as_float(static_cast<uint32_t>(kref) << 23), kLeastUnit), 3.0e38f);
+          if (__builtin_expect(kref == 0, 0)) {  // every key's own factor goes into S
+            c = 1.f;
+            scale_columns(s_addr, smem_u32(&exps[slot][0][hf * 64]), row_unit);
+          }
         }
         const bool partly = (it + 1) * kKeyTile - 64 > lim_first;
         const int valid = lim - it * kKeyTile;

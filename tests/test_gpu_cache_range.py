@@ -48,3 +48,55 @@ def test_hidden_nan_keys_alone_in_a_tile(h, n, length, heads, quantised):
     c.k[0][first:, :, 0] = 0  # hidden from the others: any number will do
     ro, rl, tol, ltol = c.reference(True)
     c.compare(out[~sees], lse[:, ~sees], ro[~sees], rl[:, ~sees], tol[~sees], ltol[:, ~sees])
+
+
+# ---------------------------------------------------------------------------------------------- one large key
+def by_key(c, causal, rows, scale=D ** -0.5):
+    """(out, tolerance) of the given rows of a cache of one sequence, where an error of a logit goes by ITS key, not by the
+    row's largest one: with ds_j = scale (sum_d |q_d k_jd|) 128 2^-23 it moves the result by at most
+    sum_j softmax_j 2 (ds_j + 2^-20) (|v_j| + |o|)."""
+    group, n, length = c.heads // c.kv_heads, c.n[0], c.lengths_l[0]
+    k, v = (t.cuda().repeat_interleave(group, 1).transpose(0, 1) for t in c.stored(0))
+    x = c.q.cuda().double().transpose(0, 1)
+    s = (x @ k.transpose(1, 2)) * scale
+    if causal:
+        seen = torch.arange(length, device="cuda")[None] <= (length - n + torch.arange(n, device="cuda"))[:, None]
+        s = s.masked_fill(~seen, -math.inf)
+    w = torch.softmax(s, -1)
+    ds = scale * (x.abs() @ k.abs().transpose(1, 2)) * 128 * 2.0 ** -23
+    o, a = w @ v, w @ v.abs()
+    moved = 2 * (ds + 2.0 ** -20) * w
+    tol = U * o.abs() + U * a + moved @ v.abs() + moved.sum(-1, keepdim=True) * o.abs() + (2.0 ** -23 * v.abs().sum(1, keepdim=True) if c.quantised else 0)
+    return o.transpose(0, 1)[rows], tol.transpose(0, 1)[rows]
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("power", [10, 18, 24, 30, 60, 110])
+@pytest.mark.parametrize("n,length", [(3, 200), (100, 300), (300, 900)])
+def test_one_large_key_that_counts_for_nothing(h, n, length, power, quantised):
+    """A key 2^power times as large as its neighbours, to which every query is opposed."""
+    c = Case(h, [n], [length], 4, 2, 16, quantised, seed=power)
+    c.q[..., 0] = c.q[..., 0].abs() + 1
+    for j in (5, length - n - 3):
+        c.k[0][j] = 0
+        c.k[0][j, :, 0] = -(2.0 ** power)
+    c.fill()
+    for causal in (True, False):
+        out = h.cache_attn(c.q.cuda(), c.cache, c.batch, causal=causal)
+        ro, tol = by_key(c, causal, slice(None))
+        over = (out.double() - ro).abs() - tol
+        assert float(over.max()) <= 0, float(over.max())
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("power", [10, 18, 24, 30, 60, 110])
+@pytest.mark.parametrize("n,length", [(3, 200), (100, 300), (129, 900)])
+def test_hidden_large_keys(h, n, length, power, quantised):
+    """The last key is 2^power times as large as the others: nothing of it reaches the rows that do not see it."""
+    c = Case(h, [n], [length], 4, 2, 16, quantised, seed=power)
+    c.k[0][-1] = (c.k[0][-1].double() * 2.0 ** power).bfloat16()
+    c.fill()
+    out = h.cache_attn(c.q.cuda(), c.cache, c.batch)
+    ro, tol = by_key(c, True, slice(0, n - 1))
+    over = (out[: n - 1].double() - ro).abs() - tol
+    assert float(over.max()) <= 0, float(over.max())
