@@ -206,10 +206,11 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   return r;
 }
 // A row of 128 codes (at `src`, 16-byte pieces swizzled by the row like the copies that brought them) as 128 bf16 or fp16
-// values times `f`, in the two half boxes at `dst`.  The pieces are read four at a time: one by one, a piece waited for the
+// values times `f` (bf16: and times `f2`, what of a
+// power of two the type's largest exponent leaves over), in the two half boxes at `dst`.  The pieces are read four at a time: one by one, a piece waited for the
 // one before it, and the helpers for them all (1,100 cycles for 16 KB).
 template <bool kBf16>
-__device__ __forceinline__ void widen_row(uint32_t src, uint32_t dst, uint32_t swz, uint32_t f, bool blank) {
+__device__ __forceinline__ void widen_row(uint32_t src, uint32_t dst, uint32_t swz, uint32_t f, uint32_t f2, bool blank) {
 #pragma unroll 1
   for (int c0 = 0; c0 < 8; c0 += 4) {
     uint4 w[4];
@@ -222,8 +223,8 @@ __device__ __forceinline__ void widen_row(uint32_t src, uint32_t dst, uint32_t s
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         if constexpr (kBf16) {
-          o[2 * y] = mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x1404)), f);
-          o[2 * y + 1] = mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x3424)), f);
+          o[2 * y] = mul_bf16x2(mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x1404)), f), f2);
+          o[2 * y + 1] = mul_bf16x2(mul_bf16x2(e4m3_pattern(__byte_perm(in[y], 0, 0x3424)), f), f2);
         } else {
           o[2 * y] = mul_f16x2(e4m3_to_f16x2(in[y]), f);
           o[2 * y + 1] = mul_f16x2(e4m3_high_to_f16x2(in[y]), f);
@@ -414,10 +415,11 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const bool none = gone || put_back;
             const int d = x ? in.vref - e : in.kref != 0 ? in.kref - e : 0;  // the row's power of two against the unit's
             if (x == 1 && in.wide) {
+              // 2^(120 - d) in two steps: a row may be 2^40 above the unit (beyond that the piece is done again)
               const uint32_t f = none ? 0u : e == 255 ? 0x7FFF7FFFu : static_cast<uint32_t>(max(0, min(254, 247 - d))) * 0x800080u;
-              widen_row<true>(src, dst, swz, f, none);
+              widen_row<true>(src, dst, swz, f, static_cast<uint32_t>(max(127, min(254, 120 - d))) * 0x800080u, none);
             } else {
-              widen_row<false>(src, dst, swz, none ? 0u : e == 255 ? 0x7FFF7FFFu : f16x2_pow2_neg(d), none);
+              widen_row<false>(src, dst, swz, none ? 0u : e == 255 ? 0x7FFF7FFFu : f16x2_pow2_neg(d), 0, none);
             }
             fence_proxy_async_smem();
             __syncwarp();

@@ -100,3 +100,16 @@ def test_hidden_large_keys(h, n, length, power, quantised):
     ro, tol = by_key(c, True, slice(0, n - 1))
     over = (out[: n - 1].double() - ro).abs() - tol
     assert float(over.max()) <= 0, float(over.max())
+
+
+# ---------------------------------------------------------------------------------------------- sizes of V
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("power", [6, 8, 13, 30, 39, 47, 90])
+@pytest.mark.parametrize("n,length", [(4, 640), (1000, 640)])
+def test_values_that_grow_along_the_sequence(h, n, length, power, quantised):
+    """V of the later keys is 2^power times as large as that of the first ones: pieces whose first tile has small values only."""
+    c = Case(h, [n], [length], 40, 40, 32, quantised, seed=power)
+    c.v[0][128:] = (c.v[0][128:].double() * 2.0 ** power).bfloat16()
+    c.fill()
+    for causal in (True, False):
+        c.check(causal)
