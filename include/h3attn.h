@@ -424,6 +424,9 @@ int32_t h3a_cache_read(const h3a_cache* cache, const h3a_cache_batch* batch, voi
  * h / (heads / cache.heads).  Without a causal mask the rows need not be tokens of the cache: cross attention to cached
  * states of any other length.  A row that sees no key is zeros, its log-sum-exp -inf.  What lies in a page behind a
  * sequence's last key, and values that the causal mask hides, never reach a result, NaN and infinities included.
+ * Sums are held in fp32 with terms up to 2^8 before the division: the number of keys times the largest |v| has to stay
+ * below 2^119 (6e35).  With more than 16 query rows per K/V head, values of a quantised V that are all below 2^-111 in their
+ * row count as zeros.
  */
 typedef struct h3a_cache_attn_params {
   h3a_cache cache;

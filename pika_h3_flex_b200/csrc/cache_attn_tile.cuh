@@ -18,10 +18,11 @@
 // Softmax reference.  Softmax is exact for any reference while the terms stay in range.  A row's is the maximum of its
 // logits over the piece's FIRST key tile (the warpgroups exchange it once), which later logits rarely exceed by much: terms
 // may grow to 2^60 (bf16 P), 2^14 (fp16 P).  A piece in which some row outgrows that is done again after the others: one
-// pass that only looks for the rows' maxima, then one with those as references.  Against a running maximum per warp, with O
-// rescaled when it moves (two warpgroups, both halves each, two register images of S): that loop was 1.4 K instructions and
-// the SM's instruction cache missed on every second request, with helpers and issuers running other code beside it
-// (5.5 warps stalled on instruction fetch per issue); the loop here is a quarter of it.
+// pass that only looks for the rows' maxima, then one with those as references.  So is one in which terms have grown and large
+// values of V took a row's sums out of fp32, as with the maxima for references they would not.  Against a running maximum per
+// warp, with O rescaled when it moves (two warpgroups, both halves each, two register images of S): that loop was 1.4 K
+// instructions and the SM's instruction cache missed on every second request, with helpers and issuers running other code
+// beside it (5.5 warps stalled on instruction fetch per issue); the loop here is a quarter of it.
 //
 // e4m3 tiles become fp16, two instructions per pair: a code is exact in fp16 (one conversion), and so is its product with
 // 2^(k - kref), kref being the tile's largest exponent, down to k - kref = -15.  2^kref goes into the tile's softmax scale, and
@@ -194,6 +195,17 @@ __device__ __noinline__ void scale_columns(uint32_t s_addr, uint32_t e_at, float
     tmem_st16(s_addr + x, r);
   }
   tmem_wait_st();
+}
+// whether a row of results, as it was stored (bf16 or fp32), holds a value that is not finite
+__device__ __noinline__ bool left_range(const uint8_t* row, bool bf16) {
+  bool lost = false;
+#pragma unroll 1
+  for (int c = 0; c < (bf16 ? 16 : 32); ++c) {
+    const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * c);
+    const uint32_t top = __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
+    lost |= bf16 ? non_finite2(top) : top >= 0x7F800000u;
+  }
+  return lost;
 }
 // 2^-d as an fp16 pair, d >= -15
 __device__ __forceinline__ uint32_t f16x2_pow2_neg(int d) {
@@ -528,6 +540,10 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             stg_v8(dst + 64 * c, reinterpret_cast<const uint32_t*>(o));
             stg_v8(dst + 64 * c + 32, reinterpret_cast<const uint32_t*>(o + 8));
           }
+        }
+        // rare: terms have grown (the sum is larger than one of so many terms up to the reference's own) and a sum has left fp32
+        if (l_sum > (kFp8 ? 4.f : 1.f) * kKeyTile * held->n_tiles && have_row && held->mode == kFirstTile) {
+          if (left_range(dst, whole)) atomicOr(&bars->redo, 1u << held->bit);
         }
         if (bars->poison != 0u && have_row) {  // rare: values left out above are added to the stored row, if it sees them
           const int begin = max(held->lim_min & ~(kKeyTile - 1), held->t0 * kKeyTile);

@@ -113,3 +113,19 @@ def test_values_that_grow_along_the_sequence(h, n, length, power, quantised):
     c.fill()
     for causal in (True, False):
         c.check(causal)
+
+
+@pytest.mark.parametrize("quantised,power", [(False, 20), (False, 80), (False, 112), (True, 80), (True, 112)])
+@pytest.mark.parametrize("n,length,nats", [(4, 640, 40), (1000, 640, 5), (1000, 640, 9), (1000, 640, 40), (300, 2000, 40)])
+def test_large_values_under_growing_logits(h, n, length, nats, quantised, power):
+    """Keys behind the first tile have logits far above the first ones', and V is so large that unnormalised sums of it
+    would leave fp32 if the terms could grow freely.  (The results themselves are far inside it.)"""
+    c = Case(h, [n], [length], 40, 40, 32, quantised, seed=nats, v_scale=2.0 ** power)
+    c.q[..., 0] = 8
+    for j in range(150, length, 90):
+        c.k[0][j] = 0
+        c.k[0][j, :, 0] = nats / 8 * math.sqrt(D)
+    c.fill()
+    for causal in (True, False):
+        out, _ = c.check(causal)
+        assert torch.isfinite(out.float()).all()
