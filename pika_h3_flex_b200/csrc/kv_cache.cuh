@@ -183,6 +183,9 @@ constexpr int kExpHeads = 128;  // heads of a token between two meetings of the 
 template <bool kWrite, bool kQuantised>
 __global__ void __launch_bounds__(kRowThreads, kRowBlocksPerSm<kQuantised>) cache_rows_kernel(const __grid_constant__ RowsArgs a, const int per_token) {
   if (block_stops(a.c)) return;
+  // A row looks at one sequence's numbers; what is wrong with the others' (offsets that decrease, say) shows only here.
+  if (a.c.status != nullptr && blockIdx.x == 0 && blockIdx.y == 0)
+    for (int b = threadIdx.x; b < a.c.n_seqs; b += kRowThreads) cache_seq(a.c, b);
   constexpr int kHeads = kUnroll<kWrite, kQuantised>, kRows = 2 * kHeads;  // row i: K (i even) or V of head i / 2
   const int lane = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const uint32_t half_mask = (threadIdx.x & 16) ? 0xFFFF0000u : 0x0000FFFFu;

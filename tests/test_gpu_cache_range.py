@@ -129,3 +129,48 @@ def test_large_values_under_growing_logits(h, n, length, nats, quantised, power)
     for causal in (True, False):
         out, _ = c.check(causal)
         assert torch.isfinite(out.float()).all()
+
+
+# ---------------------------------------------------------------------------------------------- batches that are wrong
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("starts,lengths", [
+    ([0, 10, 5, 20], [40, 40, 40]), ([20, 10, 5, 0], [40, 40, 40]), ([0, 0, 0, 21], [40, 40, 40]), ([-1, 4, 5, 20], [40, 40, 40]),
+    ([0, 20, 20, 20], [40, -1, 40]), ([0, 20, 20, 20], [40, 40, 1000]), ([0, 7, 7, 3], [40, 40, 40]), ([20, 20, 20, 0], [40, 40, 40])])
+def test_every_sequence_of_a_batch_is_checked(h, starts, lengths, quantised):
+    """Offsets that decrease or leave the rows and lengths outside the pages are reported by every call, also those of
+    sequences that no row is looked up in."""
+    from pika_h3_flex_b200 import _lib
+
+    c = Case(h, [8, 4, 8], [40, 40, 40], 2, 2, 16, quantised).fill()
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = h.CacheBatch(c.batch.pages, dev(lengths), dev(starts))
+    kv = torch.zeros(20, 2, D, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda s: h.cache_write(c.cache, batch, kv, kv, status_word=s),
+                 lambda s: h.cache_read(c.cache, batch, 20, status_word=s),
+                 lambda s: h.cache_attn(c.q.cuda(), c.cache, batch, status_word=s)):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        call(status)
+        with pytest.raises(_lib.H3AError) as e:
+            h.check_status(status)
+        assert e.value.status == _lib.H3A_ERR_INDEX
+
+
+def test_an_empty_sequence_among_many_is_checked(h):
+    """More sequences than a block has threads; the one that is wrong is far from the rows."""
+    from pika_h3_flex_b200 import _lib
+
+    B = 700
+    cache = h.KVCache.empty(4, 16, 2)
+    starts = torch.zeros(B + 1, dtype=torch.int32)
+    starts[1:] = 5
+    lengths = torch.full((B,), 5, dtype=torch.int32)
+    lengths[650] = 17
+    batch = h.CacheBatch(torch.zeros(B, 1, dtype=torch.int32).cuda(), lengths.cuda(), starts.cuda())
+    kv = torch.zeros(5, 2, D, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda s: h.cache_write(cache, batch, kv, kv, status_word=s), lambda s: h.cache_read(cache, batch, 5, status_word=s),
+                 lambda s: h.cache_attn(kv, cache, batch, status_word=s)):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        call(status)
+        with pytest.raises(_lib.H3AError) as e:
+            h.check_status(status)
+        assert e.value.status == _lib.H3A_ERR_INDEX
