@@ -369,9 +369,9 @@ int32_t h3a_adaln_norm(const h3a_adaln_params* p, void* stream);
  *
  * Pools are addressed x[page * stride_page + at * stride_token + head * stride_head + c], c in [0,128) contiguous, strides
  * in ELEMENTS (bf16, or bytes when quantised); [pages, heads, page_size, 128] storage keeps a head's rows of a page together.
- * Quantised: e4m3 codes (never NaN) and one byte e per row, in exps[page, at, head] with strides of their own; a code
- * stands for code * 2^(e - 127).  e - 127 is the smallest integer, at least -120, with max|row| <= 448 * 2^(e - 127); the
- * values are exact bf16 numbers.  A row that holds a NaN or an infinity has e = 255 and reads back as NaNs.
+ * Quantised: e4m3 codes (never NaN) and one byte e per row, in exps[page, at, head] with strides of their own (in a cache that
+ * is written to, none of them 0); a code stands for code * 2^(e - 127).  e - 127 is the smallest integer, at least -120, with
+ * max|row| <= 448 * 2^(e - 127); the values are exact bf16 numbers.  A row that holds a NaN or an infinity has e = 255 and reads back as NaNs.
  */
 typedef struct h3a_cache {
   void* k;

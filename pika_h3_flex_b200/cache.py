@@ -35,7 +35,8 @@ def _stride(t: torch.Tensor, dim: int) -> int:
 class KVCache:
     """Pages of cached rows of one attention layer.  ``k``, ``v``: logical ``[n_pages, page_size, heads, 128]`` with any
     page / token / head strides, bf16, or for a quantised cache e4m3 (``torch.float8_e4m3fn`` or ``uint8`` bytes) with
-    ``k_exp``, ``v_exp`` ``[n_pages, page_size, heads]`` uint8: a code stands for ``code * 2 ** (exp - 127)``."""
+    ``k_exp``, ``v_exp`` ``[n_pages, page_size, heads]`` uint8: a code stands for ``code * 2 ** (exp - 127)``.  Expanded
+    exponents (stride 0) can be read, not written."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None):
         _require_cuda(k, v, k_exp, v_exp)

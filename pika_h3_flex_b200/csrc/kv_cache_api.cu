@@ -41,8 +41,8 @@ int32_t current_device(Device* d) {
   return d->major == 10 ? H3A_OK : H3A_ERR_ARCH;
 }
 
-// Checks a cache and a batch and fills the kernels' view of them.
-int32_t cache_args(const h3a_cache* c, const h3a_cache_batch* b, int32_t* status, h3a::CacheArgs* a) {
+// Checks a cache (which the call writes to, or reads only) and a batch and fills the kernels' view of them.
+int32_t cache_args(bool write, const h3a_cache* c, const h3a_cache_batch* b, int32_t* status, h3a::CacheArgs* a) {
   if (!c || !b || !c->k || !c->v || !b->pages || !b->lengths || !b->starts) return H3A_ERR_ARG;
   if (c->quantised != 0 && c->quantised != 1) return H3A_ERR_ARG;
   if (c->quantised ? (!c->k_exp || !c->v_exp) : (c->k_exp || c->v_exp)) return H3A_ERR_ARG;
@@ -57,6 +57,9 @@ int32_t cache_args(const h3a_cache* c, const h3a_cache_batch* b, int32_t* status
   for (auto& s : strides)
     for (int64_t x : s)
       if (!rows16(x, es)) return H3A_ERR_ALIGN;
+  // an exponent byte that rows share can be read, but not take all their exponents
+  for (int64_t x : {c->k_exp_stride_page, c->k_exp_stride_token, c->k_exp_stride_head, c->v_exp_stride_page, c->v_exp_stride_token, c->v_exp_stride_head})
+    if (c->quantised && x < (write ? 1 : 0)) return H3A_ERR_ALIGN;
   std::memset(a, 0, sizeof(*a));
   a->pool[0] = static_cast<uint8_t*>(c->k);
   a->pool[1] = static_cast<uint8_t*>(c->v);
@@ -91,7 +94,7 @@ int32_t cache_args(const h3a_cache* c, const h3a_cache_batch* b, int32_t* status
 int32_t move_rows(bool write, const h3a_cache* c, const h3a_cache_batch* b, void* k, int64_t k_sl, int64_t k_sh, void* v, int64_t v_sl,
                   int64_t v_sh, int32_t* status, void* stream) {
   h3a::RowsArgs a;
-  int32_t rc = cache_args(c, b, status, &a.c);
+  int32_t rc = cache_args(write, c, b, status, &a.c);
   if (rc != H3A_OK) return rc;
   if (!k || !v) return H3A_ERR_ARG;
   if (!aligned16(k) || !aligned16(v) || !rows16(k_sl, 2, write) || !rows16(k_sh, 2, write) || !rows16(v_sl, 2, write) || !rows16(v_sh, 2, write))
@@ -283,7 +286,7 @@ int32_t h3a_cache_attn(const h3a_cache_attn_params* p, void* stream) {
   if (!p || !p->q || !p->o || p->o == p->q) return H3A_ERR_ARG;  // a piece that is done twice reads its q again
   h3a::CacheAttnArgs a;
   std::memset(&a, 0, sizeof(a));
-  int32_t rc = cache_args(&p->cache, &p->batch, p->status_word, &a.c);
+  int32_t rc = cache_args(false, &p->cache, &p->batch, p->status_word, &a.c);
   if (rc != H3A_OK) return rc;
   if (p->heads <= 0 || p->heads % p->cache.heads || static_cast<int64_t>(p->batch.rows) * p->heads >= (1ll << 31)) return H3A_ERR_SHAPE;
   if ((p->causal != 0 && p->causal != 1) || p->max_new < 0) return H3A_ERR_ARG;

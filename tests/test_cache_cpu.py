@@ -114,3 +114,29 @@ def test_wrappers_refuse_cpu_tensors(lib):
         h3.CacheBatch(i32[None], i32, torch.zeros(2, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="no CPU path"):
         h3.cache_attn(pool[0], None, None)
+
+
+@pytest.mark.parametrize("which", ["k_exp", "v_exp"])
+@pytest.mark.parametrize("dim", ["page", "token", "head"])
+def test_exponents_of_a_written_cache_must_not_repeat(lib, which, dim):
+    """A byte that several rows share cannot take all their exponents; what is only read may repeat, but not run backwards."""
+    def quantised(stride):
+        p = good()
+        c = p.cache
+        c.quantised, c.k_exp, c.v_exp = 1, BASE, BASE + 1024
+        for x in ("k", "v"):
+            for d, n in (("page", 16 * 128), ("token", 128), ("head", 128)):
+                setattr(c, f"{x}_exp_stride_{d}", n // 128)
+        setattr(c, f"{which}_stride_{dim}", stride)
+        return p
+
+    def calls(p):  # none of them gets as far as a launch: what comes after the cache's checks is refused too
+        p.heads = 0
+        c, b = C.byref(p.cache), C.byref(p.batch)
+        return (lib.h3a_cache_write(c, b, None, 128, 128, BASE, 128, 128, None, None),
+                lib.h3a_cache_read(c, b, None, 128, 128, BASE, 128, 128, None, None), lib.h3a_cache_attn(C.byref(p), None))
+
+    bad, arg, shape = _lib.H3A_ERR_ALIGN, _lib.H3A_ERR_ARG, _lib.H3A_ERR_SHAPE
+    assert calls(quantised(0)) == (bad, arg, shape)
+    assert calls(quantised(-1)) == (bad, bad, bad)
+    assert calls(quantised(1)) == (arg, arg, shape)

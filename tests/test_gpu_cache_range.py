@@ -174,3 +174,19 @@ def test_an_empty_sequence_among_many_is_checked(h):
         with pytest.raises(_lib.H3AError) as e:
             h.check_status(status)
         assert e.value.status == _lib.H3A_ERR_INDEX
+
+
+def test_expanded_exponents_are_read_but_not_written(h):
+    from pika_h3_flex_b200 import _lib
+
+    c = Case(h, [20], [20], 2, 2, 16, True)
+    codes = torch.randn(c.cache.k.shape, device="cuda").to(torch.float8_e4m3fn)
+    one = torch.full((1, 1, 1), 124, dtype=torch.uint8, device="cuda").expand(c.cache.k.shape[:3])
+    cache = h.KVCache(codes, codes, one, one)
+    kv = torch.zeros(20, 2, D, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(_lib.H3AError) as e:
+        h.cache_write(cache, c.batch, kv, kv)
+    assert e.value.status == _lib.H3A_ERR_ALIGN
+    got, _ = h.cache_read(cache, c.batch, 20)
+    rows = codes[c.batch.pages[0].long()].reshape(-1, 2, D)[:20]
+    assert torch.equal(got.double(), rows.double() / 8)
