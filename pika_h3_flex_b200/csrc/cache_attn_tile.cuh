@@ -340,7 +340,6 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     bars->redo = 0;
     bars->early_exit = (a.c.status != nullptr && *reinterpret_cast<volatile int*>(a.c.status) != 0) ? 1u : 0u;
     fence_mbar_init();
-    a.desc[kDescInts * blockIdx.x] = 0;
   }
   if (warp == kProducerWarp && lane == 0) {
     prefetch_tmap(&tm_q);
@@ -351,6 +350,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   {
     ShareIter begin = share_begin(a, &start);
     if (threadIdx.x == kPieceWarp * 32) {  // the first piece is found here, in registers: everybody waits for it
+      a.desc[kDescInts * blockIdx.x] = 0;  // by the thread that may go on to describe an item there: no other order is needed
       again = begin;
       bars->more = begin.next(a, p);
       if (bars->more) describe_piece(a, begin, p, pieces[0]);

@@ -190,3 +190,20 @@ def test_expanded_exponents_are_read_but_not_written(h):
     got, _ = h.cache_read(cache, c.batch, 20)
     rows = codes[c.batch.pages[0].long()].reshape(-1, 2, D)[:20]
     assert torch.equal(got.double(), rows.double() / 8)
+
+
+# ---------------------------------------------------------------------------------------------- a caller's workspace
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("fill", [0, 1, 127, 255])
+def test_what_a_workspace_held_before_does_not_matter(h, fill, quantised):
+    """One workspace for calls of several shapes, one after the other, each on what the one before left in it: descriptions of
+    items in parts and partial results of other shares."""
+    shapes = [([300, 40, 1], [900, 2000, 500], 6, 2), ([150], [1100], 4, 4), ([2, 1], [3000, 700], 8, 2), ([1], [40000], 8, 1), ([700], [700], 2, 2)]
+    cases = [Case(h, *s, 32, quantised, seed=i).fill() for i, s in enumerate(shapes)]
+    want = [h.cache_attn(c.q.cuda(), c.cache, c.batch, return_lse=True) for c in cases]
+    need = max(h.cache_attn_workspace_bytes(c.cache, c.batch, c.rows, c.heads) for c in cases)
+    workspace = torch.full((need,), fill, dtype=torch.uint8, device="cuda")
+    for _ in range(20):
+        for c, (out, lse) in zip(cases, want):
+            got = h.cache_attn(c.q.cuda(), c.cache, c.batch, return_lse=True, workspace=workspace)
+            assert torch.equal(got[0], out) and torch.equal(got[1], lse)
