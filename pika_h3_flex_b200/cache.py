@@ -153,6 +153,13 @@ def _status_ptr(status_word: Optional[torch.Tensor], device: torch.device) -> Op
     return status_word.data_ptr()
 
 
+def _check_workspace(workspace: torch.Tensor, device: torch.device) -> None:
+    if workspace.device != device:
+        raise ValueError(f"expected everything on {device}, got the workspace on {workspace.device}")
+    if not workspace.is_contiguous():  # its bytes are counted, and an expanded tensor has fewer than that
+        raise ValueError("the workspace must be contiguous")
+
+
 def _move(name: str, cache: KVCache, batch: CacheBatch, k: torch.Tensor, v: torch.Tensor, status_word: Optional[torch.Tensor]) -> None:
     device = cache.device
     L, ksl, ksh = _rows(k, "k", cache.heads, device)
@@ -237,8 +244,8 @@ def cache_attn(q: torch.Tensor, cache: KVCache, batch: CacheBatch, causal: bool 
         return (out, lse) if return_lse else out
     if workspace is None:
         workspace = torch.empty(_workspace_bytes(device.index, L, batch._c.n_seqs, H, cache.heads, cache.quantised, max_new or 0), dtype=torch.uint8, device=device)
-    elif workspace.device != device:
-        raise ValueError(f"expected everything on {device}, got the workspace on {workspace.device}")
+    else:
+        _check_workspace(workspace, device)
     p = _lib.CacheAttnParams(cache._c, batch._c, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, qsl, qsh, osl, osh,
                              H, 1 if causal else 0, softmax_scale, max_new or 0, workspace.data_ptr(), workspace.nbytes, status, wait_limit_ns)
     p.batch.rows = L

@@ -140,3 +140,16 @@ def test_exponents_of_a_written_cache_must_not_repeat(lib, which, dim):
     assert calls(quantised(0)) == (bad, arg, shape)
     assert calls(quantised(-1)) == (bad, bad, bad)
     assert calls(quantised(1)) == (arg, arg, shape)
+
+
+def test_a_workspace_has_to_have_its_bytes():
+    """An expanded tensor counts more bytes than it has, and a strided one has gaps."""
+    from pika_h3_flex_b200 import cache
+
+    cpu = torch.device("cpu")
+    cache._check_workspace(torch.empty(1 << 20, dtype=torch.uint8), cpu)
+    for w in (torch.empty(1, dtype=torch.uint8).expand(1 << 20), torch.empty(64, 64, dtype=torch.uint8)[:, ::2], torch.empty(64, 64)[:, :32]):
+        with pytest.raises(ValueError, match="contiguous"):
+            cache._check_workspace(w, cpu)
+    with pytest.raises(ValueError, match="workspace on cpu"):
+        cache._check_workspace(torch.empty(64, dtype=torch.uint8), torch.device("cuda:0"))

@@ -207,3 +207,11 @@ def test_what_a_workspace_held_before_does_not_matter(h, fill, quantised):
         for c, (out, lse) in zip(cases, want):
             got = h.cache_attn(c.q.cuda(), c.cache, c.batch, return_lse=True, workspace=workspace)
             assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+
+
+def test_a_workspace_must_be_contiguous(h):
+    c = Case(h, [2], [20], 4, 2, 16, False).fill()
+    need = h.cache_attn_workspace_bytes(c.cache, c.batch, 2, 4)
+    for w in (torch.empty(32, dtype=torch.uint8, device="cuda")[:1].expand(need), torch.empty(need, 2, dtype=torch.uint8, device="cuda")[:, 0]):
+        with pytest.raises(ValueError, match="contiguous"):
+            h.cache_attn(c.q.cuda(), c.cache, c.batch, workspace=w)
