@@ -215,3 +215,20 @@ def test_a_workspace_must_be_contiguous(h):
     for w in (torch.empty(32, dtype=torch.uint8, device="cuda")[:1].expand(need), torch.empty(need, 2, dtype=torch.uint8, device="cuda")[:, 0]):
         with pytest.raises(ValueError, match="contiguous"):
             h.cache_attn(c.q.cuda(), c.cache, c.batch, workspace=w)
+
+
+# ---------------------------------------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("n,length,heads,kv_heads", [([700], [900], 4, 4), ([300, 20, 400], [2000, 20, 500], 6, 2), ([257], [400], 2, 1), ([150], [150], 128, 1)])
+def test_values_that_are_not_finite_all_over(h, n, length, heads, kv_heads, quantised):
+    """NaN and infinities in V of many tokens, every item's first and last visible keys among them: each reaches the rows
+    that see it, in its own dimension (a quantised row: in all), and no other row, also in items of later sequences."""
+    c = Case(h, n, length, heads, kv_heads, 16, quantised, seed=len(n))
+    for b, (m, x) in enumerate(zip(n, length)):
+        for j in range(x - m, x, 37):
+            c.v[b][j, :, j % D] = (math.nan, math.inf, -math.inf)[j % 3]
+            c.v[b][j, 0, 5] = math.inf
+    c.fill()
+    for causal in (True, False):
+        out, lse = h.cache_attn(c.q.cuda(), c.cache, c.batch, causal=causal, return_lse=True)
+        c.compare(out, lse, *c.reference(causal))
