@@ -232,3 +232,29 @@ def test_values_that_are_not_finite_all_over(h, n, length, heads, kv_heads, quan
     for causal in (True, False):
         out, lse = h.cache_attn(c.q.cuda(), c.cache, c.batch, causal=causal, return_lse=True)
         c.compare(out, lse, *c.reference(causal))
+
+
+# ---------------------------------------------------------------------------------------------- waits that run out
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("limit_ns", [1, 2048, 4096, 8192, 16384, 65536])
+def test_a_wait_that_runs_out_is_reported(h, limit_ns, quantised):
+    """A limit shorter than what a wait takes: the call returns, with the timeout in the status word or with right results, and
+    the device is as good as before."""
+    from pika_h3_flex_b200 import _lib
+
+    c = Case(h, [500, 1, 90], [3000, 700, 90], 8, 4, 32, quantised, seed=3).fill()
+    q = c.q.cuda()
+    want = h.cache_attn(q, c.cache, c.batch, return_lse=True)
+    for _ in range(3):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out, lse = h.cache_attn(q, c.cache, c.batch, return_lse=True, status_word=status, wait_limit_ns=limit_ns)
+        try:
+            h.check_status(status)
+        except _lib.H3AError as e:
+            assert e.status == _lib.H3A_ERR_TIMEOUT
+            assert 33 <= int(status.item()) & 0xFF <= 49
+        else:
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        status.zero_()
+        out, lse = h.cache_attn(q, c.cache, c.batch, return_lse=True, status_word=status)
+        assert h.read_status(status) == 0 and torch.equal(out, want[0]) and torch.equal(lse, want[1])
