@@ -19,7 +19,7 @@
 // block (5 instead of 1.5 instructions per pair) ran at 40 % of the HBM rate.
 //
 // Measured: one token over each of two contexts of 65,537 and 131,072 bf16 keys (40 heads on 8) 127 us, 6.3 TB/s; 64
-// contexts of 8,000 keys, 16 heads of their own, bf16 609 us, 6.9 TB/s, e4m3 361 us, 5.9 TB/s (some 500 instructions per 16
+// contexts of 8,000 keys, 16 heads of their own, bf16 628 us, 6.7 TB/s, e4m3 361 us, 5.9 TB/s (some 500 instructions per 16
 // keys and warp, waiting for memory most of the time; reading two steps ahead into L2, and 3 or 5 blocks per SM instead of
 // 4, were not faster); 32 contexts of 200 to 16,384 e4m3 keys 59 us.  Calls of a few microseconds are latency: one token over
 // 1,023 bf16 keys takes 12 us, 3 of them memory's.
@@ -330,7 +330,10 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
       // ---- O^T += V^T P^T.  P is 0 where a key is masked, so V must be finite there: rows behind the sequence's last key may
       //      hold anything and count as zeros; a value that some of the item's rows see and others do not counts as zero
       //      if it is not finite, and is put back at the end for the rows that see it.
-      //      P is rounded once per term (bf16: at most 2^-8 of it, fp16 less); the row sum keeps the unrounded terms.
+      //      A bf16 P goes in two parts, the rounded one and what the rounding left, at most 2^-16 of a term lost: the MMAs wait
+      //      for memory anyway (64 contexts of 8,000 keys 628 us either way, with 16 query rows 175 against 173), and with one
+      //      part the results were half as far off again as their own rounding takes them (2.3e-3 against 1.7e-3 of the
+      //      norm).  An fp16 P has 3 bits more and goes in one.  The row sum keeps the unrounded terms.
       if (partly) {
         bool bad = false;
 #pragma unroll
@@ -373,12 +376,15 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
           }
         }
       } else {
-        uint32_t pf[kNT][2];
+        uint32_t pf[kNT][2], rest[kNT][2];
 #pragma unroll
-        for (int i = 0; i < kNT; ++i) {
-          pf[i][0] = transpose_8x8(pack_bf16x2(s[i][0], s[i][1]));
-          pf[i][1] = transpose_8x8(pack_bf16x2(s[i][2], s[i][3]));
-        }
+        for (int i = 0; i < kNT; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t w = pack_bf16x2(s[i][2 * c], s[i][2 * c + 1]);
+            rest[i][c] = transpose_8x8(pack_bf16x2(s[i][2 * c] - __uint_as_float(w << 16), s[i][2 * c + 1] - __uint_as_float(w & 0xFFFF0000u)));
+            pf[i][c] = transpose_8x8(w);
+          }
         uint32_t f_lo = 0, f_hi = 0;
         if constexpr (kFp8) {
           uint32_t f[4];
@@ -414,7 +420,10 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
           }
           const uint4 vf = make_uint4(lo[0], lo[1], hi[0], hi[1]);
 #pragma unroll
-          for (int i = 0; i < kNT; ++i) mma_bf16(o[i][j], vf, pf[i][0], pf[i][1]);
+          for (int i = 0; i < kNT; ++i) {
+            mma_bf16(o[i][j], vf, pf[i][0], pf[i][1]);
+            mma_bf16(o[i][j], vf, rest[i][0], rest[i][1]);
+          }
         }
       }
       if (next < end_key) load_v(id, at);

@@ -258,3 +258,24 @@ def test_a_wait_that_runs_out_is_reported(h, limit_ns, quantised):
         status.zero_()
         out, lse = h.cache_attn(q, c.cache, c.batch, return_lse=True, status_word=status)
         assert h.read_status(status) == 0 and torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+# ---------------------------------------------------------------------------------------------- precision
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("n,length,heads,kv_heads", [([1], [700], 8, 2), ([1, 2, 1], [50, 3000, 129], 10, 2), ([5], [500], 2, 2), ([4], [2000], 4, 1), ([1], [30000], 8, 1)])
+def test_few_rows_keep_their_probabilities(h, n, length, heads, kv_heads, quantised):
+    """Up to 16 query rows per K/V head: probabilities lose at most 2^-16 of themselves (bf16, in two parts) or 2^-11 (fp16, one
+    part), so that with ds and r of test_gpu_cache.py a result is off by u |o| + (that + 2 (ds + r)) A, and by what fp16's last
+    place takes."""
+    c = Case(h, n, length, heads, kv_heads, 32, quantised, seed=9).fill()
+    for causal in (True, False):
+        out, lse = h.cache_attn(c.q.cuda(), c.cache, c.batch, causal=causal, return_lse=True)
+        ro, rl, tol, ltol = c.reference(causal)
+        a = torch.zeros_like(ro)  # sum_j softmax_j |v_j|
+        for b, (m, x) in enumerate(zip(n, length)):
+            k, v = (t.cuda().repeat_interleave(heads // kv_heads, 1).transpose(0, 1) for t in c.stored(b))
+            s = c.q[c.starts[b] : c.starts[b] + m].cuda().double().transpose(0, 1) @ k.transpose(1, 2) * D ** -0.5
+            if causal:
+                s = s.masked_fill(torch.arange(x, device="cuda")[None] > (x - m + torch.arange(m, device="cuda"))[:, None], -math.inf)
+            a[c.starts[b] : c.starts[b] + m] = (torch.softmax(s, -1) @ v.abs()).transpose(0, 1)
+        c.compare(out, lse, ro, rl, tol - (U - (2.0 ** -11 if quantised else 2.0 ** -16)) * a, ltol)
