@@ -364,8 +364,9 @@ int32_t h3a_adaln_norm(const h3a_adaln_params* p, void* stream);
 /*
  * Paged K/V cache: rows of 128 values per token and K/V head, kept between calls in fixed-size pages, and the attention
  * of new rows over it.  The reference keeps nothing between evaluations (src/pika_h3/core/sampling.py:87-109,160-169 runs
- * the whole sequence through the model six times); this is for callers whose K and V of some tokens stay the same: text or
- * condition tokens over the sampler's evaluations, a clip that grows by a few frames at a time, a prompt model.
+ * the whole joint sequence, its text included, through the model six times, and every token's K and V change with it); this
+ * is for callers whose K and V of some tokens stay the same: fixed states that a cross attention looks at, a clip that grows
+ * by a few frames at a time and whose past does not change, a prompt model.
  *
  * Pools are addressed x[page * stride_page + at * stride_token + head * stride_head + c], c in [0,128) contiguous, strides
  * in ELEMENTS (bf16, or bytes when quantised); [pages, heads, page_size, 128] storage keeps a head's rows of a page together.
@@ -426,7 +427,8 @@ int32_t h3a_cache_read(const h3a_cache* cache, const h3a_cache_batch* batch, voi
  * sequence's last key, and values that the causal mask hides, never reach a result, NaN and infinities included.
  * Sums are held in fp32 with terms up to 2^8 before the division: the number of keys times the largest |v| has to stay
  * below 2^119 (6e35).  With more than 16 query rows per K/V head, values of a quantised V that are all below 2^-111 in their
- * row count as zeros.
+ * row count as zeros.  Probabilities over a quantised cache are fp16 numbers: a term 2^-26 of the largest (2^-30 with up to 16
+ * query rows) and smaller ones are rounded to a multiple of that or to nothing.
  */
 typedef struct h3a_cache_attn_params {
   h3a_cache cache;

@@ -1,8 +1,9 @@
 """Paged K/V cache and the attention that reads it: ``cache_write``, ``cache_read`` and ``cache_attn`` over the C ABI.
 
-For callers whose K and V of some tokens stay the same between calls, where the reference runs the whole sequence through
-the model at every evaluation (``src/pika_h3/core/sampling.py:87-109,160-169``): text or condition tokens over the
-sampler's evaluations, a clip that grows by a few frames at a time, a prompt model.
+For callers whose K and V of some tokens stay the same between calls: a model that looks at fixed states by cross attention
+at every evaluation of a sampler, a clip that grows by a few frames at a time whose past does not change, a prompt model.
+(The reference runs one joint sequence through the model at every evaluation, ``src/pika_h3/core/sampling.py:87-109,160-169``;
+text is part of it, so its K and V change from block to block and evaluation to evaluation and are nothing to keep.)
 
     cache = KVCache.empty(n_pages, page_size, kv_heads, quantised=True)
     batch = CacheBatch(pages, lengths, starts)      # lengths include the new tokens

@@ -19,10 +19,10 @@
 // block (5 instead of 1.5 instructions per pair) ran at 40 % of the HBM rate.
 //
 // Measured: one token over each of two contexts of 65,537 and 131,072 bf16 keys (40 heads on 8) 127 us, 6.3 TB/s; 64
-// contexts of 8,000 keys, 16 heads of their own, bf16 628 us, 6.7 TB/s, e4m3 361 us, 5.9 TB/s (some 500 instructions per 16
+// contexts of 8,000 keys, 16 heads of their own, bf16 607 to 628 us, 6.7 to 6.9 TB/s, e4m3 361 us, 5.9 TB/s (some 500 instructions per 16
 // keys and warp, waiting for memory most of the time; reading two steps ahead into L2, and 3 or 5 blocks per SM instead of
 // 4, were not faster); 32 contexts of 200 to 16,384 e4m3 keys 59 us.  Calls of a few microseconds are latency: one token over
-// 1,023 bf16 keys takes 12 us, 3 of them memory's.
+// 1,023 bf16 keys takes 12 to 16 us, 3 of them memory's.
 #pragma once
 #include "cache_attn.cuh"
 

@@ -31,14 +31,15 @@
 // multiply each column of S by its key's power first, in tensor memory, so that the ordinary loop stays as short as it is.
 // V and O are in units of the largest exponent of the piece's first tile; fp16 holds codes up
 // to 2^7 above that, and rows 2^14 below it with all their bits.  A V tile with rows outside that is widened to bf16
-// instead, and its P rounded to bf16.  (Everything through bf16 took five instructions per pair.)
+// instead, and its P rounded to bf16; one with rows 2^40 above the unit has its piece done again in the largest's units.  (Everything through bf16 took five instructions per pair.)
 //
 // What bounds it.  A tile of 256 rows x 128 keys is 16.8 MFLOP, 1.5 us of an SM at the rate of the fastest library product;
 // it takes 1.9 us (e4m3 2.0): four chains of MMA, 64 exponentials a thread and MMA that wait for one another, under the
-// power cap where calls are long.  4,680 rows x 40 heads over 49,384 keys: 3.7 ms, 1.27 PFLOP/s (e4m3 4.0 ms); 2,048 rows x
-// 40 heads over 20,011 keys of 8 shared heads: 0.65 ms (e4m3 0.70).  A piece costs some 3 us beside its tiles (first maxima,
-// last P V, results), which is what is left in calls of few tiles each: 6,240 rows x 40 heads over prompts of 512 and 77
-// tokens 98 us (e4m3 114), 8 new tokens x 32 heads on each of 32 contexts of 4,000 e4m3 tokens 125 us.
+// power cap where calls are long.  4,680 rows x 40 heads over 49,384 keys: 3.6 ms by itself, 4.0 ms and 1.16 PFLOP/s among
+// other work (e4m3 4.0 ms by itself); 2,048 rows x 40 heads over 20,011 keys of 8 shared heads: 0.61 ms by itself (e4m3 0.70,
+// 0.79 among other work).  A piece costs some 3 us beside its tiles (first maxima, last P V, results), which is what is left
+// in calls of few tiles each: 6,240 rows x 40 heads over prompts of 512 and 77 tokens 97 us (e4m3 115), 8 new tokens x 32
+// heads on each of 32 contexts of 4,000 e4m3 tokens 124 us.
 //
 // Every wait is bounded: when the limit runs out the CTA raises a CTA-wide flag that the other waits poll, lets copies in
 // flight land, records the wait's code in the status word, frees TMEM and returns.  Warps meet at mbarriers, never at named barriers,
