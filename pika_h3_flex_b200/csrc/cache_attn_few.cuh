@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kFewThreads, (kFewBlocksPerSm<kFp8, kNT>)) cac
       for (int i = 0; i < kNT; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          s[i][c] = ex2_approx(fmaf(s[i][c], unit[i][c & 1], -m[i][c & 1]));
+          s[i][c] = ex2_approx(__fmul_rn(s[i][c], unit[i][c & 1]) - m[i][c & 1]);  // rounded like the maximum: large ones differ by 0
           l[i][c & 1] += s[i][c];
         }
       // ---- O^T += V^T P^T.  P is 0 where a key is masked, so V must be finite there: rows behind the sequence's last key may

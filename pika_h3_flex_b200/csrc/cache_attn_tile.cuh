@@ -178,22 +178,22 @@ struct TileInfo {
   int wide;       // V is bf16, and P is to be
 };
 constexpr int kInfoRing = 8;  // the producer is at most four tiles ahead of the softmax warps
-// S of one row times a factor per key: 64 columns, the keys' exponent bytes at e_at.  A call of its own: in line, the hot loop
-// around it took 1.5 % longer (chunk of 2,048 over 20,011 keys 806 us against 792).
-__device__ __noinline__ void scale_columns(uint32_t s_addr, uint32_t e_at, float row_unit) {
+// 64 columns of one row of S times `unit`, and times a power of two per key whose exponent bytes are at e_at (0: none).  A
+// call of its own: in line, the hot loop around it took 1.5 % longer (chunk of 2,048 over 20,011 keys 806 us against 792).
+__device__ __noinline__ void scale_columns(uint32_t s_addr, uint32_t e_at, float unit) {
 #pragma unroll 1
   for (int x = 0; x < 64; x += 16) {
     uint32_t r[16];
-    uint4 e;
+    uint4 e = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
     tmem_ld16(s_addr + x, r);
-    ld_shared_v4(e_at + x, e);
+    if (e_at != 0u) ld_shared_v4(e_at + x, e);
     const uint32_t ex[4] = {e.x, e.y, e.z, e.w};
     tmem_wait_ld();
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       asm volatile("" : "+r"(r[i]));  // not before the wait
       const uint32_t power = (ex[i >> 2] >> (8 * (i & 3))) & 0xFFu;
-      r[i] = __float_as_uint(__uint_as_float(r[i]) * fminf(row_unit * __uint_as_float(power << 23), 3.0e38f));
+      r[i] = __float_as_uint(__uint_as_float(r[i]) * fminf(unit * __uint_as_float(power << 23), 3.0e38f));
     }
     tmem_st16(s_addr + x, r);
   }
@@ -992,16 +992,23 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         if (!ok) break;
         tc_fence_after_sync();
         float c = row_unit;
+        uint32_t e_at = 0;
         bool wide = false;
         if constexpr (kFp8) {
           const uint32_t slot = (n_before + it) % kInfoRing;
           const int kref = info[slot].kref;
           wide = info[slot].wide != 0;
           c = fminf(fmaxf(row_unit * __uint_as_float(static_cast<uint32_t>(kref) << 23), kLeastUnit), 3.0e38f);
-          if (__builtin_expect(kref == 0, 0)) {  // every key's own factor goes into S
-            c = 1.f;
-            scale_columns(s_addr, smem_u32(&exps[slot][0][hf * 64]), row_unit);
+          if (kref == 0) {  // every key has a factor of its own
+            c = row_unit;
+            e_at = smem_u32(&exps[slot][0][hf * 64]);
           }
+        }
+        // Where pieces are done again S is scaled first, so that the maxima and the terms are rounded alike: s c - m in one
+        // step, with m rounded, is as far off as that rounding, and far more than the exponential takes for logits of 2^31.
+        if (__builtin_expect(e_at != 0u || mode != kFirstTile, 0)) {
+          scale_columns(s_addr, e_at, c);
+          c = 1.f;
         }
         const bool partly = (it + 1) * kKeyTile - 64 > lim_first;
         const int valid = lim - it * kKeyTile;
@@ -1034,6 +1041,7 @@ cache_attn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (mode == kFirstTile) {
             m_ref = fmaxf(m_ref, exchange(m_ref)) - kLift;
             if (!ok) break;
+            over = fabsf(m_ref) > 1.0e6f && m_ref > kNoMax;  // logits too large for s c - m in one step
           }
         }
         // P = 2^(s c - m), rounded once; the row sum keeps the unrounded terms

@@ -279,3 +279,31 @@ def test_few_rows_keep_their_probabilities(h, n, length, heads, kv_heads, quanti
                 s = s.masked_fill(torch.arange(x, device="cuda")[None] > (x - m + torch.arange(m, device="cuda"))[:, None], -math.inf)
             a[c.starts[b] : c.starts[b] + m] = (torch.softmax(s, -1) @ v.abs()).transpose(0, 1)
         c.compare(out, lse, ro, rl, tol - (U - (2.0 ** -11 if quantised else 2.0 ** -16)) * a, ltol)
+
+
+# ---------------------------------------------------------------------------------------------- logits without bounds
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("power", [10, 28, 40, 90, 115])
+@pytest.mark.parametrize("n,length,j", [(1, 127, 3), (3, 700, 600), (100, 300, 5), (100, 300, 190), (300, 900, 599), (40, 40, 0)])
+def test_logits_of_any_size(h, n, length, j, power, quantised):
+    """Logits that differ by far more than fp32 resolves at their size: a row is the value of its one key, exactly."""
+    c = Case(h, [n], [length], 4, 2, 16, quantised, seed=power)
+    c.q[..., 0] = c.q[..., 0].abs() + 1
+    v = c.stored(0)[1][j].repeat_interleave(2, 0).cuda()  # [heads, 128]
+    for sign in (1, -1):
+        if sign > 0:  # one key far above the others
+            c.k[0][j] = 0
+            c.k[0][j, :, 0] = 2.0 ** power
+        else:  # all far below zero, one the least
+            c.k[0][:] = 0
+            c.k[0][:, :, 0] = -(2.0 ** (power + 1))
+            c.k[0][j, :, 0] = -(2.0 ** power)
+        c.fill()
+        for causal in (True, False):
+            out, lse = h.cache_attn(c.q.cuda(), c.cache, c.batch, causal=causal, return_lse=True)
+            sees = torch.arange(length - n, length, device="cuda") >= (j if causal else 0)
+            logit = sign * c.q[..., 0].cuda().double() * 2.0 ** power * D ** -0.5  # above the next one by its own size or so
+            assert torch.isfinite(out.float()).all() and torch.isfinite(lse).all()
+            if power > 10:
+                assert torch.equal(out[sees].double(), v.expand(n, 4, D)[sees])
+                assert ((lse.T[sees].double() - logit[sees]).abs() <= 2.0 ** -18 * logit[sees].abs()).all()
