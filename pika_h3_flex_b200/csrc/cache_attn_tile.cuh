@@ -19,7 +19,8 @@
 // logits over the piece's FIRST key tile (the warpgroups exchange it once), which later logits rarely exceed by much: terms
 // may grow to 2^60 (bf16 P), 2^14 (fp16 P).  A piece in which some row outgrows that is done again after the others: one
 // pass that only looks for the rows' maxima, then one with those as references.  So is one in which terms have grown and large
-// values of V took a row's sums out of fp32, as with the maxima for references they would not.  Against a running maximum per
+// values of V took a row's sums out of fp32, as with the maxima for references they would not, and one with logits above 10^6,
+// whose products with the scale have to be rounded like their maximum.  Against a running maximum per
 // warp, with O rescaled when it moves (two warpgroups, both halves each, two register images of S): that loop was 1.4 K
 // instructions and the SM's instruction cache missed on every second request, with helpers and issuers running other code
 // beside it (5.5 warps stalled on instruction fetch per issue); the loop here is a quarter of it.
